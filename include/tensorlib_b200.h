@@ -275,6 +275,107 @@ TL_API int tl_rmsnorm_gateup_swiglu_f16(const tl_half* x, const tl_half* norm_w,
                                  const tl_half* w3, tl_half* out, int hidden, int dim,
                                  tl_stream stream);
 
+/* ---- serving many sequences: rotary positions, the paged key-value cache, beams ---------------------------------
+ * The reference keeps one contiguous cache per layer for one sequence (Transformer.cpp:22-23), rotates interleaved pairs by
+ * consecutive positions (CPU.cpp:427-461) and samples greedily (llama2.cpp:55-61); these operators are what a server of many
+ * sequences or beams needs beside that. They only enqueue on `stream`, allocate nothing and can be captured into a graph.
+ * A workspace belongs to the caller: calls that share one must be ordered behind one another, and so must graphs that
+ * captured it. Ids that the kernels find outside their tables (rows, pages, parents, lengths) are never followed: the
+ * entry is skipped and tl_device_status() reports TL_ERR_INVALID_ARGUMENT. */
+
+/* Rotation frequencies, on the host: freqs_host[rot_dim / 2] in radians a position, pair i has base^(-2 i / rot_dim), and the
+ * factor that rotated pairs are multiplied by. scaling, for contexts `factor` times as long as the trained one:
+ *   TL_ROPE_LINEAR  every frequency / factor
+ *   TL_ROPE_BASE    base * factor^(rot_dim / (rot_dim - 2))
+ *   TL_ROPE_PARTS   with x = the pair's turns over trained_len: / factor where x <= low, kept where x >= high, and between
+ *                   them both blended linearly in x
+ *   TL_ROPE_RAMP    the same blend, linear in the pair's index between those that turn `high` and `low` times, and a
+ *                   magnitude of 0.1 ln(factor) + 1
+ * factor, trained_len, low and high are ignored where the scaling does not use them. No device needed. */
+enum { TL_ROPE_UNSCALED = 0, TL_ROPE_LINEAR = 1, TL_ROPE_BASE = 2, TL_ROPE_PARTS = 3, TL_ROPE_RAMP = 4 };
+TL_API int tl_rotary_frequencies(int rot_dim, double base, int scaling, double factor, double trained_len, double low,
+                                 double high, double* freqs_host, float* magnitude_host);
+/* Device::apply_rotary_emb (Device.hpp:91-98) with a position for every token and freqs[rot_dim / 2] in device memory: pair i of
+ * the first rot_dim elements of each head, (2i, 2i+1) or with half_layout (i, i + rot_dim / 2), is turned by
+ * positions[t] * freqs[i] (angles in 64 bits) and scaled by magnitude; the other elements pass through. inverse turns back,
+ * which is the gradient of the forward call. Strides in elements; in == out with equal strides is allowed, other overlaps are
+ * not. A token with a negative position is padding: its output is left as it was. */
+TL_API int tl_rotary_f16(const tl_half* in, tl_half* out, const int* positions, const double* freqs, float magnitude, int tokens,
+                         int n_heads, int head_dim, int rot_dim, int half_layout, int inverse, long long in_token_stride,
+                         long long in_head_stride, long long out_token_stride, long long out_head_stride, tl_stream stream);
+
+/* A paged key-value cache. All arrays are the caller's device memory. Element (layer, page, slot, head, d) of either pool is at
+ * layer * layer_stride + page * page_stride + slot * token_stride + head * head_stride + d, so pages may be laid out by token or
+ * by head. Row r (one sequence or beam) holds lengths[r] tokens; token t lies in page page_table[r * max_pages + t / page_size],
+ * slot t % page_size. Entries behind a row's last page are -1 (fill a new table with tl_memset 0xff), ref_counts[p] is the number
+ * of table entries that name page p, and a page with count 0 is free. Rows may share pages. The pointers a call does not use
+ * may be NULL. Rows of head_dim values that all start on 16 bytes take the fast kernels; any other layout works too. */
+typedef struct tl_paged_cache {
+    tl_half* k_pages; tl_half* v_pages;
+    long long layer_stride, page_stride, token_stride, head_stride;
+    int n_layers, n_pages, page_size, n_kv_heads, head_dim;
+    int n_rows, max_pages;
+    int* page_table;            /* [n_rows][max_pages] */
+    int* lengths;               /* [n_rows] */
+    int* ref_counts;            /* [n_pages] */
+} tl_paged_cache;
+
+/* Row r becomes a copy of row parents[r] by reference (its pages and its length), for all rows at once; parents[r] = r keeps a row,
+ * -1 empties it. Pages that no row names any more are free. No page is copied. Up to 49152 rows. */
+TL_API int tl_paged_fork(const tl_paged_cache* cache, const int* parents, tl_stream stream);
+/* Room for new_tokens[r] >= 0 more tokens of every row: pages are taken in ascending order of their ids, rows in order, and
+ * lengths[r] grows by new_tokens[r]. Where a row's next token falls into a partly filled page that other rows still name, the row
+ * first gets a copy of it (the filled slots, K and V of every layer; the last of the rows that write keeps the page if no other
+ * row names it). *result (device memory) = TL_OK; or TL_ERR_OUT_OF_MEMORY if the free pages or max_pages do not suffice, or
+ * TL_ERR_INVALID_ARGUMENT if a length, a count or an entry that it has to follow cannot be: then no row has changed. Workspace as
+ * tl_paged_workspace says. */
+TL_API int tl_paged_reserve_f16(const tl_paged_cache* cache, const int* new_tokens, int* result, void* workspace,
+                                size_t workspace_bytes, tl_stream stream);
+/* Page dst[i] = page src[i], K and V of every layer; pairs with src[i] == dst[i] or src[i] == -1 are skipped. No page may be a
+ * destination twice, or both a source and a destination. */
+TL_API int tl_paged_copy_f16(const tl_paged_cache* cache, const int* src, const int* dst, int n, tl_stream stream);
+/* Moves the live pages (count > 0) together into pages 0 .. live-1: the highest live page goes to the lowest free one, and so on;
+ * the table and the counts follow. moved_to[n_pages]: where each live page is now, -1 for pages that were free. *live (device
+ * memory): their number. */
+TL_API int tl_paged_compact_f16(const tl_paged_cache* cache, int* moved_to, int* live, void* workspace, size_t workspace_bytes,
+                                tl_stream stream);
+TL_API int tl_paged_workspace(int n_rows, int n_pages, size_t* bytes);
+
+/* The way into the cache for new tokens, one launch: q rotated into q_out (n_heads heads; 0: none; q_out == q with equal strides is
+ * allowed), k rotated and v as it is stored at positions[t] of row rows[t] (rows == NULL: row t). Heads of a token are
+ * contiguous in q, k and v, so that they can be parts of one fused projection; token strides in elements. rot_dim, half_layout,
+ * freqs, magnitude and padding as for tl_rotary_f16; rot_dim = 0 only stores. Room must have been made (tl_paged_reserve_f16). */
+TL_API int tl_rotary_append_f16(const tl_paged_cache* cache, int layer, const tl_half* q, tl_half* q_out, const tl_half* k,
+                                const tl_half* v, const int* rows, const int* positions, const double* freqs, float magnitude,
+                                int tokens, int n_heads, int rot_dim, int half_layout, long long q_token_stride,
+                                long long q_out_token_stride, long long kv_token_stride, tl_stream stream);
+/* Attention of one query per batch entry over all lengths[row] tokens of its row: out_h = sum_t softmax_t(scale q_h.k_t) v_t, query
+ * head h reading KV head h / (n_heads / n_kv_heads). q, out: [batch] rows of n_heads * head_dim values, row strides in elements.
+ * rows[b]: the row of entry b, -1 for a padding entry (rows == NULL: row b). lse, if not NULL: fp32 [batch, n_heads],
+ * log sum_t exp(scale q_h.k_t). An empty row gives zeros and -inf. head_dim <= 256. workspace: tl_paged_attn_workspace bytes (at
+ * most 32 MB), zeroed once before its first use; calls leave it as the next one needs it. */
+TL_API int tl_paged_attn_decode_f16(const tl_paged_cache* cache, int layer, const tl_half* q, tl_half* out, float* lse, const int* rows,
+                                    int batch, int n_heads, float scale, long long q_row_stride, long long out_row_stride,
+                                    void* workspace, size_t workspace_bytes, tl_stream stream);
+TL_API int tl_paged_attn_workspace(int n_heads, int n_kv_heads, int head_dim, size_t* bytes);
+
+/* Beam search's selection, beside Device::argmax: logits [batch * beams] rows of vocab values (row stride in elements), scores
+ * [batch * beams] fp32. Of the candidates (beam w, token j) of each batch entry, valued score_w + logit_wj - log sum_j exp logit_wj,
+ * the k best in descending order, ties to the lowest w, then the lowest j: out_scores [batch, k] fp32, out_parents [batch, k] the row
+ * batch_entry * beams + w (as tl_paged_fork and tl_beam_reorder_f16 take it), out_tokens [batch, k]. Values are compared in 64 bits.
+ * finished (may be NULL): a beam with finished[row] != 0 has one candidate, pad_token, at its score; its logits are not used. A score
+ * of -inf makes a dead beam; NaN logits count as -inf and +inf as 65504, NaN scores as -inf. beams, k <= 128. workspace:
+ * tl_beam_select_workspace bytes, zeroed once before its first use. */
+TL_API int tl_beam_select_f16(const tl_half* logits, long long row_stride, const float* scores, const unsigned char* finished,
+                              int pad_token, int batch, int beams, int vocab, int k, float* out_scores, int* out_parents,
+                              int* out_tokens, void* workspace, size_t workspace_bytes, tl_stream stream);
+TL_API int tl_beam_select_workspace(int batch, int beams, int vocab, int k, size_t* bytes);
+/* Rows of contiguous state follow their beams: the first `used` values of dst[o][r] = src[o][parents[r]] for o < outer, r < rows
+ * (strides in elements; parents[r] = -1 leaves row r). src and dst may not overlap. */
+TL_API int tl_beam_reorder_f16(const tl_half* src, tl_half* dst, const int* parents, int outer, int rows, long long used,
+                               long long src_outer_stride, long long src_row_stride, long long dst_outer_stride,
+                               long long dst_row_stride, tl_stream stream);
+
 /* ---- Llama2 model (model/llama2_7b) -------------------------------------------------------- */
 typedef struct tl_llama2_config {
     int dim, hidden_dim, n_layers, n_heads, n_kv_heads, vocab_size, max_seq_len; /* main.cpp:26-34 */

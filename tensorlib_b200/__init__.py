@@ -20,6 +20,8 @@ FAST = 1
 _vp = C.c_void_p
 _sz = C.c_size_t
 _int = C.c_int
+_ll = C.c_longlong
+_dbl = C.c_double
 
 
 class TLError(RuntimeError):
@@ -33,6 +35,15 @@ class tl_llama2_config(C.Structure):
                                        "vocab_size", "max_seq_len", "numerics", "silu_via_float",
                                        "tp_rank", "tp_world", "one_kernel_decode")]
 
+
+class tl_paged_cache(C.Structure):
+    _fields_ = ([(n, C.c_void_p) for n in ("k_pages", "v_pages")] +
+                [(n, C.c_longlong) for n in ("layer_stride", "page_stride", "token_stride", "head_stride")] +
+                [(n, C.c_int) for n in ("n_layers", "n_pages", "page_size", "n_kv_heads", "head_dim", "n_rows", "max_pages")] +
+                [(n, C.c_void_p) for n in ("page_table", "lengths", "ref_counts")])
+
+
+_cache = C.POINTER(tl_paged_cache)
 
 # name -> argtypes; every function returns int status unless listed in _OTHER_RESTYPE
 _SIGS = {
@@ -107,6 +118,19 @@ _SIGS = {
     "tl_reduce_f16": [_vp, _vp, _sz, _sz, _int, _int, _vp],
     "tl_argreduce_f16": [_vp, _vp, _sz, _sz, _int, _vp],
     "tl_cast": [_vp, _vp, _sz, _int, _vp],
+    "tl_rotary_frequencies": [_int, _dbl, _int, _dbl, _dbl, _dbl, _dbl, _vp, C.POINTER(C.c_float)],
+    "tl_rotary_f16": [_vp] * 4 + [C.c_float] + [_int] * 6 + [_ll] * 4 + [_vp],
+    "tl_rotary_append_f16": [_cache, _int] + [_vp] * 7 + [C.c_float] + [_int] * 4 + [_ll] * 3 + [_vp],
+    "tl_paged_attn_decode_f16": [_cache, _int] + [_vp] * 4 + [_int, _int, C.c_float, _ll, _ll, _vp, _sz, _vp],
+    "tl_paged_attn_workspace": [_int, _int, _int, C.POINTER(_sz)],
+    "tl_paged_fork": [_cache, _vp, _vp],
+    "tl_paged_reserve_f16": [_cache, _vp, _vp, _vp, _sz, _vp],
+    "tl_paged_copy_f16": [_cache, _vp, _vp, _int, _vp],
+    "tl_paged_compact_f16": [_cache, _vp, _vp, _vp, _sz, _vp],
+    "tl_paged_workspace": [_int, _int, C.POINTER(_sz)],
+    "tl_beam_select_f16": [_vp, _ll, _vp, _vp] + [_int] * 5 + [_vp] * 4 + [_sz, _vp],
+    "tl_beam_select_workspace": [_int] * 4 + [C.POINTER(_sz)],
+    "tl_beam_reorder_f16": [_vp] * 3 + [_int, _int] + [_ll] * 5 + [_vp],
 }
 _OTHER_RESTYPE = {"tl_strerror": (C.c_char_p, [_int]), "tl_last_error": (C.c_char_p, []),
                   "tl_version": (_int, [])}
@@ -469,6 +493,156 @@ def cast(x: np.ndarray, to) -> np.ndarray:
     dx, dy = DeviceBuffer.from_numpy(x), DeviceBuffer(max(x.size * np.dtype(to).itemsize, 4))
     check(load().tl_cast(dy.ptr, dx.ptr, x.size, kind, None), "tl_cast")
     return dy.to_numpy(np.dtype(to), x.shape)
+
+
+# -------------------------------------------------------------------------------------------------
+# serving many sequences: rotary positions, paged key-value cache, beams (numpy in, numpy out)
+# -------------------------------------------------------------------------------------------------
+ROPE_SCALINGS = {"unscaled": 0, "linear": 1, "base": 2, "parts": 3, "ramp": 4}
+
+
+def rotary_frequencies(rot_dim: int, base: float = 10000.0, scaling: str = "unscaled", factor: float = 1.0,
+                       trained_len: float = 0.0, low: float = 0.0, high: float = 0.0):
+    """Host only: (radians a position for each pair as float64, magnitude) for tl_rotary_f16."""
+    f, mag = np.empty(rot_dim // 2, np.float64), C.c_float(0)
+    check(load().tl_rotary_frequencies(rot_dim, base, ROPE_SCALINGS[scaling], factor, trained_len, low, high, _np_ptr(f), C.byref(mag)),
+          "tl_rotary_frequencies")
+    return f, mag.value
+
+
+def rotary(x: np.ndarray, positions, freqs: np.ndarray, magnitude: float = 1.0, half_layout: bool = False, inverse: bool = False,
+           out: np.ndarray | None = None, in_place: bool = False) -> np.ndarray:
+    """x [tokens, heads, head_dim] with the first 2 * len(freqs) elements of each head turned by their token's position
+    (tl_rotary_f16). Tokens at negative positions keep what `out` (default zeros) held."""
+    T, Hh, hd = x.shape
+    pos = np.ascontiguousarray(positions, dtype=np.int32)
+    dx, dp, df = DeviceBuffer.from_numpy(x), DeviceBuffer.from_numpy(pos), DeviceBuffer.from_numpy(np.asarray(freqs, np.float64))
+    do = dx if in_place else DeviceBuffer.from_numpy(np.zeros_like(x) if out is None else out)
+    check(load().tl_rotary_f16(dx.ptr, do.ptr, dp.ptr, df.ptr, magnitude, T, Hh, hd, 2 * len(freqs), int(half_layout), int(inverse),
+                               Hh * hd, hd, Hh * hd, hd, None), "tl_rotary_f16")
+    return do.to_numpy(np.float16, x.shape)
+
+
+class PagedCache:
+    """A paged key-value cache in device memory and the calls on it (tl_paged_cache). Pools are seen as
+    [layers, pages, page_size, kv_heads, head_dim] whatever their layout; by_head stores each head's slots together."""
+
+    def __init__(self, n_layers: int, n_pages: int, page_size: int, n_kv_heads: int, head_dim: int, n_rows: int, max_pages: int,
+                 by_head: bool = False, k: np.ndarray | None = None, v: np.ndarray | None = None):
+        self.shape, self.by_head = (n_layers, n_pages, page_size, n_kv_heads, head_dim), by_head
+        zeros = np.zeros(self.shape, np.float16)
+        self._k, self._v = (DeviceBuffer.from_numpy(self._stored(zeros if a is None else a)) for a in (k, v))
+        self._table = DeviceBuffer.from_numpy(np.full((n_rows, max_pages), -1, np.int32))
+        self._lengths, self._refs = (DeviceBuffer.from_numpy(np.zeros(n, np.int32)) for n in (n_rows, n_pages))
+        page = page_size * n_kv_heads * head_dim
+        token, head = (head_dim, page_size * head_dim) if by_head else (n_kv_heads * head_dim, head_dim)
+        self.c = tl_paged_cache(self._k.ptr, self._v.ptr, n_pages * page, page, token, head, n_layers, n_pages, page_size, n_kv_heads,
+                                head_dim, n_rows, max_pages, self._table.ptr, self._lengths.ptr, self._refs.ptr)
+        need = _sz(0)
+        check(load().tl_paged_workspace(n_rows, n_pages, C.byref(need)), "tl_paged_workspace")
+        self._work, self._result = DeviceBuffer(need.value), DeviceBuffer(4)
+        self._attn_work = None
+
+    def _stored(self, a):
+        return np.ascontiguousarray(a.swapaxes(2, 3) if self.by_head else a)
+
+    def pools(self):
+        L, P, s, h, d = self.shape
+        got = (b.to_numpy(np.float16, (L, P, h, s, d) if self.by_head else self.shape) for b in (self._k, self._v))
+        return tuple(a.swapaxes(2, 3) if self.by_head else a for a in got)
+
+    def set_state(self, table, lengths, refs) -> None:
+        for buf, a in ((self._table, table), (self._lengths, lengths), (self._refs, refs)):
+            a = np.ascontiguousarray(a, dtype=np.int32)
+            check(load().tl_memcpy_h2d(buf.ptr, _np_ptr(a), a.nbytes, None), "tl_memcpy_h2d")
+            synchronize()
+
+    def state(self):
+        """(page_table, lengths, ref_counts)"""
+        return (self._table.to_numpy(np.int32, (self.c.n_rows, self.c.max_pages)), self._lengths.to_numpy(np.int32, (self.c.n_rows,)),
+                self._refs.to_numpy(np.int32, (self.c.n_pages,)))
+
+    def fork(self, parents) -> None:
+        d = DeviceBuffer.from_numpy(np.ascontiguousarray(parents, dtype=np.int32))
+        check(load().tl_paged_fork(C.byref(self.c), d.ptr, None), "tl_paged_fork")
+        synchronize()
+
+    def reserve(self, new_tokens) -> int:
+        """The status that the device found: 0, or why no row has changed."""
+        d = DeviceBuffer.from_numpy(np.ascontiguousarray(new_tokens, dtype=np.int32))
+        check(load().tl_paged_reserve_f16(C.byref(self.c), d.ptr, self._result.ptr, self._work.ptr, self._work.nbytes, None),
+              "tl_paged_reserve_f16")
+        return int(self._result.to_numpy(np.int32, (1,))[0])
+
+    def copy(self, src, dst) -> None:
+        s, d = (DeviceBuffer.from_numpy(np.ascontiguousarray(a, dtype=np.int32)) for a in (src, dst))
+        check(load().tl_paged_copy_f16(C.byref(self.c), s.ptr, d.ptr, len(src), None), "tl_paged_copy_f16")
+        synchronize()
+
+    def compact(self):
+        """(where each page went, number of live pages)"""
+        moved = DeviceBuffer(4 * self.c.n_pages)
+        check(load().tl_paged_compact_f16(C.byref(self.c), moved.ptr, self._result.ptr, self._work.ptr, self._work.nbytes, None),
+              "tl_paged_compact_f16")
+        return moved.to_numpy(np.int32, (self.c.n_pages,)), int(self._result.to_numpy(np.int32, (1,))[0])
+
+    def append(self, layer: int, q, k, v, positions, freqs=None, magnitude: float = 1.0, half_layout: bool = False, rows=None):
+        """tl_rotary_append_f16: stores k (rotated) and v at (rows, positions); returns the rotated q (None: no queries)."""
+        T = k.shape[0]
+        heads = 0 if q is None else q.shape[1]
+        kv, hd = self.shape[3], self.shape[4]
+        dk, dv = DeviceBuffer.from_numpy(k), DeviceBuffer.from_numpy(v)
+        dq = None if q is None else DeviceBuffer.from_numpy(q)
+        do = None if q is None else DeviceBuffer.from_numpy(np.zeros_like(q))
+        dp = DeviceBuffer.from_numpy(np.ascontiguousarray(positions, dtype=np.int32))
+        dr = None if rows is None else DeviceBuffer.from_numpy(np.ascontiguousarray(rows, dtype=np.int32))
+        df = None if freqs is None else DeviceBuffer.from_numpy(np.asarray(freqs, np.float64))
+        ptr = lambda b: b.ptr if b is not None else None  # noqa: E731
+        check(load().tl_rotary_append_f16(C.byref(self.c), layer, ptr(dq), ptr(do), dk.ptr, dv.ptr, ptr(dr), dp.ptr, ptr(df), magnitude, T,
+                                          heads, 0 if freqs is None else 2 * len(freqs), int(half_layout), heads * hd, heads * hd, kv * hd,
+                                          None), "tl_rotary_append_f16")
+        synchronize()
+        return None if q is None else do.to_numpy(np.float16, q.shape)
+
+    def attend(self, layer: int, q: np.ndarray, scale: float | None = None, rows=None):
+        """tl_paged_attn_decode_f16: q [batch, heads, head_dim] -> (out, lse)."""
+        B, Hh, hd = q.shape
+        if self._attn_work is None or self._attn_work[0] != Hh:
+            need = _sz(0)
+            check(load().tl_paged_attn_workspace(Hh, self.shape[3], hd, C.byref(need)), "tl_paged_attn_workspace")
+            self._attn_work = (Hh, DeviceBuffer.from_numpy(np.zeros(max(need.value, 16), np.uint8)))
+        w = self._attn_work[1]
+        dq, do, dl = DeviceBuffer.from_numpy(q), DeviceBuffer(max(2 * q.size, 2)), DeviceBuffer(max(4 * B * Hh, 4))
+        dr = None if rows is None else DeviceBuffer.from_numpy(np.ascontiguousarray(rows, dtype=np.int32))
+        check(load().tl_paged_attn_decode_f16(C.byref(self.c), layer, dq.ptr, do.ptr, dl.ptr, dr.ptr if dr is not None else None, B, Hh,
+                                              hd ** -0.5 if scale is None else scale, Hh * hd, Hh * hd, w.ptr, w.nbytes, None),
+              "tl_paged_attn_decode_f16")
+        return do.to_numpy(np.float16, q.shape), dl.to_numpy(np.float32, (B, Hh))
+
+
+def beam_select(logits: np.ndarray, scores, beams: int, k: int, finished=None, pad_token: int = 0):
+    """logits [batch * beams, vocab] fp16, scores [batch * beams]: (scores, parent rows, tokens), each [batch, k]."""
+    rows, vocab = logits.shape
+    batch = rows // beams
+    need = _sz(0)
+    check(load().tl_beam_select_workspace(batch, beams, vocab, k, C.byref(need)), "tl_beam_select_workspace")
+    w = DeviceBuffer.from_numpy(np.zeros(max(need.value, 16), np.uint8))
+    dl, ds = DeviceBuffer.from_numpy(logits), DeviceBuffer.from_numpy(np.ascontiguousarray(scores, dtype=np.float32))
+    df = None if finished is None else DeviceBuffer.from_numpy(np.ascontiguousarray(finished, dtype=np.uint8))
+    out = [DeviceBuffer(max(4 * batch * k, 4)) for _ in range(3)]
+    check(load().tl_beam_select_f16(dl.ptr, vocab, ds.ptr, df.ptr if df is not None else None, pad_token, batch, beams, vocab, k, out[0].ptr,
+                                    out[1].ptr, out[2].ptr, w.ptr, w.nbytes, None), "tl_beam_select_f16")
+    return (out[0].to_numpy(np.float32, (batch, k)), out[1].to_numpy(np.int32, (batch, k)), out[2].to_numpy(np.int32, (batch, k)))
+
+
+def beam_reorder(src: np.ndarray, dst: np.ndarray, parents, used: int) -> np.ndarray:
+    """dst [outer, rows, pitch] with the first `used` values of each row from row parents[r] of src; returned."""
+    outer, rows, pitch = src.shape
+    ds, dd = DeviceBuffer.from_numpy(src), DeviceBuffer.from_numpy(dst)
+    dp = DeviceBuffer.from_numpy(np.ascontiguousarray(parents, dtype=np.int32))
+    check(load().tl_beam_reorder_f16(ds.ptr, dd.ptr, dp.ptr, outer, rows, used, rows * pitch, pitch, rows * dst.shape[2], dst.shape[2], None),
+          "tl_beam_reorder_f16")
+    return dd.to_numpy(np.float16, dst.shape)
 
 
 PLAN_NAMES = {0: "reference_order", 1: "gemv_ring", 2: "gemv_small", 3: "skinny_streamk", 4: "skinny_cluster",

@@ -40,6 +40,7 @@ int set_error(int status, const char* fmt, ...) {
     return status;
 }
 bool initialized() { return g_init; }
+int init_device() { return g_device; }
 int sm_count() { return g_sms; }
 const Tables& tables() { return g_tables; }
 int* device_status_word() { return g_status; }

@@ -1,0 +1,621 @@
+"""The operators for serving many sequences, through the C ABI, against plain forms in 64 bits (serving_oracle.py): rotary
+positions, attention over a paged cache, the pages' own operations, beam selection, and a run of them together."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+import serving_oracle as so
+from serving_cases import BEAM_SHAPES, beam_case
+
+pytestmark = pytest.mark.gpu
+
+
+def normal(r, *shape, std=1.0):
+    return (r.standard_normal(shape) * std).astype(np.float16)
+
+
+def close(got, want, tol, what=""):
+    got = got.astype(np.float64)
+    assert got.shape == want.shape
+    same = (got == want) | (np.isnan(got) & np.isnan(want))
+    with np.errstate(invalid="ignore"):
+        bad = ~(same | (np.abs(got - want) <= tol))
+    assert not bad.any(), (what, int(bad.sum()), np.argwhere(bad)[:3].tolist(), got[bad][:3], want[bad][:3])
+
+
+# ---- rotary positions ----------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("T,heads,hd,rot,half", [(1, 1, 2, 2, False), (1, 32, 128, 128, False), (5, 3, 80, 80, True), (17, 8, 128, 64, True),
+                                                 (9, 4, 64, 16, False), (3, 5, 7, 6, False), (4, 2, 9, 4, True), (300, 6, 72, 36, True),
+                                                 (2, 1, 256, 256, True), (33, 2, 48, 0, False), (2, 3, 1024, 1024, False), (70, 12, 96, 24, False)])
+@pytest.mark.parametrize("inverse", [False, True])
+def test_rotary_matches_the_formula(tl, T, heads, hd, rot, half, inverse):
+    r = np.random.default_rng([T, heads, hd, rot])
+    x = normal(r, T, heads, hd, std=2.0)
+    pos = r.integers(0, 1 << 20, T).astype(np.int32)
+    pos[0] = [0, 1, 2 ** 31 - 1][T % 3]
+    f, mag = tl.rotary_frequencies(max(rot, 2), scaling="ramp", factor=4.0, trained_len=2048, low=1, high=32)
+    f = f[:rot // 2]
+    want, tol = so.rotary(x, pos, f, mag, half, inverse)
+    close(tl.rotary(x, pos, f, mag, half, inverse), want, tol)
+    close(tl.rotary(x, pos, f, mag, half, inverse, in_place=True), want, tol, "in place")
+
+
+def test_rotary_leaves_padding_and_turns_back(tl):
+    r = np.random.default_rng(5)
+    x, f = normal(r, 12, 4, 64), tl.rotary_frequencies(64)[0]
+    pos = np.array([3, -1, 70000, -5, 0, 1, 2, -2 ** 31, 9, 8, 7, 6], np.int32)
+    old = normal(r, 12, 4, 64)
+    y = tl.rotary(x, pos, f, out=old)
+    assert np.array_equal(y[pos < 0], old[pos < 0])
+    # forward, then inverse: two roundings of at most |x| + |y| of a pair each
+    back = tl.rotary(y, pos, f, inverse=True, out=old)
+    size = np.abs(x.astype(np.float64)).reshape(12, 4, 32, 2).sum(-1).repeat(2, -1)
+    assert (np.abs(back.astype(np.float64) - x)[pos >= 0] <= (3 * so.EPS16 * size + 2 * so.TINY16)[pos >= 0]).all()
+    assert tl.device_status() == 0
+
+
+def test_rotary_gradient_is_the_inverse_turn(tl):
+    """d/dx sum(g * R x) = R^T g, checked against differences of the formula."""
+    r = np.random.default_rng(6)
+    x, g = r.standard_normal((2, 1, 16)), normal(r, 2, 1, 16)
+    pos, (f, mag) = np.array([5, 4000], np.int32), tl.rotary_frequencies(12, scaling="ramp", factor=2.0, trained_len=512, low=1, high=32)
+    for half in (False, True):
+        got = tl.rotary(g, pos, f, mag, half, inverse=True)
+        h = 1e-6
+        num = np.zeros_like(x)
+        for i in np.ndindex(*x.shape):
+            d = np.zeros_like(x)
+            d[i] = h
+            num[i] = ((so.rotary(x + d, pos, f, mag, half)[0] - so.rotary(x - d, pos, f, mag, half)[0]) * g).sum() / (2 * h)
+        tol = so.rotary(g, pos, f, mag, half, True)[1] + 1e-7
+        close(got, num, tol)
+
+
+def test_rotary_of_a_strided_slice(tl):
+    """Heads 2..4 of a wider buffer, by-head output: what lies between the rows stays."""
+    r = np.random.default_rng(7)
+    T, W, hd = 6, 9, 24
+    x, f = normal(r, T, W, hd), tl.rotary_frequencies(24)[0]
+    pos = np.arange(T, dtype=np.int32) * 1000
+    for off in (0, 1):                       # 16-byte aligned, and not
+        dx, dp, df = tl.DeviceBuffer.from_numpy(np.concatenate([x.reshape(-1), np.zeros(8, np.float16)])), tl.DeviceBuffer.from_numpy(pos), tl.DeviceBuffer.from_numpy(f)
+        do = tl.DeviceBuffer.from_numpy(np.full(3 * T * 32 + 8, 7.0, np.float16))
+        start = 2 * hd + off
+        tl.check(tl.load().tl_rotary_f16(dx.ptr + 2 * start, do.ptr + 2 * off, dp.ptr, df.ptr, 1.0, T, 3, hd, hd, 1, 0, W * hd, hd, 32, T * 32, None), "rotary")
+        flat = np.concatenate([x.reshape(-1), np.zeros(8, np.float16)])
+        xs = np.stack([[flat[start + t * W * hd + h * hd:][:hd] for h in range(3)] for t in range(T)])
+        want, tol = so.rotary(xs, pos, f, 1.0, True)
+        got = do.to_numpy(np.float16, (3 * T * 32 + 8,))[off:off + 3 * T * 32].reshape(3, T, 32).swapaxes(0, 1)
+        close(got[..., :hd], want, tol, off)
+        assert (got[..., hd:] == 7).all()
+
+
+# ---- the way into the cache ------------------------------------------------------------------------------------------
+def filled_cache(tl, r, layers, page, kv, hd, lens, by_head=False, spare=3, max_pages=None, garbage=True):
+    """A cache whose row i holds lens[i] tokens in random pages, with anything at all in the slots never written."""
+    counts = [-(-n // page) for n in lens]
+    pages = sum(counts) + spare
+    width = max_pages or max(1, max(counts) + 1)
+    k, v = normal(r, layers, pages, page, kv, hd), normal(r, layers, pages, page, kv, hd)
+    order = r.permutation(pages).astype(np.int32)
+    table, refs, at = np.full((len(lens), width), -1, np.int32), np.zeros(pages, np.int32), 0
+    for i, n in enumerate(counts):
+        table[i, :n] = order[at:at + n]
+        refs[order[at:at + n]] = 1
+        at += n
+        if garbage and lens[i] % page:
+            for a in (k, v):
+                a[:, table[i, n - 1], lens[i] % page:] = np.array([np.nan, np.inf, -np.inf, 65504], np.float16)[r.integers(0, 4, a[:, 0, lens[i] % page:].shape)]
+    c = tl.PagedCache(layers, pages, page, kv, hd, len(lens), width, by_head, k, v)
+    c.set_state(table, np.asarray(lens, np.int32), refs)
+    return c, k, v, table, refs
+
+
+def row_tokens(a, table, n, page):
+    """[n, kv, hd] of one row from a pool [pages, page, kv, hd]"""
+    t = np.arange(n)
+    return a[table[t // page], t % page]
+
+
+@pytest.mark.parametrize("page,kv,hd,heads,rot,half,by_head", [(16, 8, 128, 32, 128, False, False), (1, 1, 64, 1, 64, True, False),
+                                                               (24, 3, 80, 15, 40, True, True), (5, 2, 7, 4, 6, False, False),
+                                                               (16, 2, 64, 0, 64, False, True), (8, 4, 32, 8, 0, False, False)])
+def test_append_stores_at_the_row_and_position(tl, page, kv, hd, heads, rot, half, by_head):
+    r = np.random.default_rng([page, kv, hd])
+    lens = [3 * page, 1, 2 * page + 1, 0, page, 4]
+    c, k, v, table, refs = filled_cache(tl, r, 2, page, kv, hd, lens, by_head)
+    rows = np.array([2, 0, 0, 1, 4, 2, 5, 5], np.int32)
+    pos = np.array([2 * page, 0, 3 * page - 1, 0, page - 1, 0, -1, 3], np.int32)
+    q = normal(r, 8, heads, hd) if heads else None
+    nk, nv = normal(r, 8, kv, hd), normal(r, 8, kv, hd)
+    f = tl.rotary_frequencies(rot)[0] if rot else None
+    got_q = c.append(1, q, nk, nv, pos, f, 1.25, half, rows)
+    fr = np.zeros(0) if f is None else f
+    wk, tk = so.rotary(nk, pos, fr, 1.25, half)
+    if heads:
+        wq, tq = so.rotary(q, pos, fr, 1.25, half)
+        live = pos >= 0
+        close(got_q[live], wq[live], tq[live], "q")
+        assert (got_q[~live] == 0).all()
+    gk, gv = c.pools()
+    seen = np.zeros(k.shape[1:3], bool)
+    for i in range(8):
+        if pos[i] >= 0:
+            at = (1, table[rows[i], pos[i] // page], pos[i] % page)
+            seen[at[1:]] = True
+            close(gk[at], wk[i], tk[i], "k")
+            assert np.array_equal(gv[at], nv[i])
+    for got, old in ((gk, k), (gv, v)):          # nothing else has changed
+        assert np.array_equal(got[0].view(np.uint16), old[0].view(np.uint16))
+        assert np.array_equal(got[1][~seen].view(np.uint16), old[1][~seen].view(np.uint16))
+    assert tl.device_status() == 0
+
+
+def test_append_never_follows_bad_ids(tl):
+    r = np.random.default_rng(9)
+    page, kv, hd = 8, 2, 32
+    c, k, v, table, refs = filled_cache(tl, r, 1, page, kv, hd, [8, 8, 8, 8, 8], garbage=False)
+    table[3, 0], table[4, 0] = k.shape[1], -7
+    c.set_state(table, [8] * 5, refs)
+    rows = np.array([0, 5, -1, 3, 4, 1, 2], np.int32)
+    pos = np.array([1, 0, 0, 0, 0, 16, 2 ** 31 - 1], np.int32)     # row 1 has room for 16 tokens, entry 1 is -1
+    nk, nv = normal(r, 7, kv, hd), normal(r, 7, kv, hd)
+    c.append(0, None, nk, nv, pos, None, rows=rows)
+    gk, gv = c.pools()
+    assert tl.device_status() == 1
+    k[0, table[0, 0], 1], v[0, table[0, 0], 1] = nk[0], nv[0]
+    assert np.array_equal(gk, k) and np.array_equal(gv, v)
+
+
+# ---- attention over pages --------------------------------------------------------------------------------------------
+def check_attention(tl, c, k, v, table, lens, page, q, scale=None, rows=None, got=None):
+    B, heads, hd = q.shape
+    kv = k.shape[2]
+    out, lse = c.attend(0, q, scale, rows) if got is None else got
+    for b in range(B):
+        row = b if rows is None else rows[b]
+        n = 0 if row < 0 else lens[row]
+        kk, vv = (row_tokens(a, table[row], n, page) for a in (k, v)) if n else (np.zeros((0, kv, hd)),) * 2
+        for h in range(heads):
+            j = h // (heads // kv)
+            o, l, to, tl_ = so.attend(q[b, h], kk[:, j], vv[:, j], hd ** -0.5 if scale is None else scale)
+            close(out[b, h], o, to, (b, h, n))
+            if n == 0:
+                assert (out[b, h] == 0).all() and lse[b, h] == -np.inf
+            else:
+                assert abs(lse[b, h] - l) <= tl_, (b, h, n, lse[b, h], l, tl_)
+    return out, lse
+
+
+LENS = [1, 0, 15, 16, 17, 33, 2, 64, 129, 300, 1000]
+
+
+@pytest.mark.parametrize("hd,kv,group,page,by_head", [(128, 8, 4, 16, False), (64, 1, 1, 16, False), (80, 3, 5, 24, True), (128, 2, 8, 1, False),
+                                                      (256, 2, 3, 64, False), (96, 2, 16, 16, True), (40, 1, 7, 100, False), (8, 2, 2, 3, False),
+                                                      (192, 1, 12, 32, False), (128, 4, 1, 16, False), (64, 1, 40, 16, False), (256, 1, 20, 8, True),
+                                                      (7, 2, 3, 5, False), (33, 1, 17, 16, True), (136, 2, 9, 16, False)])
+def test_attention_over_pages(tl, hd, kv, group, page, by_head):
+    r = np.random.default_rng([hd, kv, group, page])
+    c, k, v, table, _ = filled_cache(tl, r, 1, page, kv, hd, LENS, by_head)
+    q = normal(r, len(LENS), kv * group, hd, std=1.5)
+    out, lse = check_attention(tl, c, k[0], v[0], table, LENS, page, q)
+    again = c.attend(0, q)
+    assert np.array_equal(out, again[0]) and np.array_equal(lse, again[1])       # the same call, the same bits
+    assert tl.device_status() == 0
+
+
+@pytest.mark.parametrize("B,low,high,kv,group,hd,page", [(1, 1, 1, 32, 1, 128, 16), (1, 333, 333, 32, 1, 128, 16), (1, 20011, 20011, 1, 8, 128, 16),
+                                                         (1, 9000, 9000, 8, 4, 64, 64), (3, 1, 7000, 2, 4, 128, 24), (200, 1, 90, 2, 2, 64, 16),
+                                                         (65, 30, 500, 4, 3, 80, 32), (300, 0, 3, 1, 1, 128, 16)])
+def test_attention_split_over_the_length(tl, B, low, high, kv, group, hd, page):
+    r = np.random.default_rng([B, high, kv])
+    lens = r.integers(low, high + 1, B).tolist()
+    c, k, v, table, _ = filled_cache(tl, r, 1, page, kv, hd, lens)
+    q = normal(r, B, kv * group, hd, std=1.5)
+    check_attention(tl, c, k[0], v[0], table, lens, page, q)
+    assert tl.device_status() == 0
+
+
+def test_attention_of_large_scores_and_values(tl):
+    """Scores over hundreds apart, growing and falling, and values at the type's limits."""
+    r = np.random.default_rng(12)
+    hd, page = 128, 16
+    for order in (1, -1):
+        c, k, v, table, _ = filled_cache(tl, r, 1, page, 1, hd, [777, 64], garbage=False)
+        ramp = np.linspace(-20, 20, 777)[::order]
+        t = np.arange(777)
+        k[0, table[0, t // page], t % page, 0] = (ramp[:, None] * np.sign(r.standard_normal(hd))[None]).astype(np.float16)
+        v[0, table[0, t // page], t % page, 0] = (r.choice([-65504.0, 65504.0, 1.0], (777, hd))).astype(np.float16)
+        state = c.state()
+        c = tl.PagedCache(1, k.shape[1], page, 1, hd, 2, table.shape[1], k=k, v=v)
+        c.set_state(*state)
+        q = normal(r, 2, 6, hd, std=4.0)
+        check_attention(tl, c, k[0], v[0], table, [777, 64], page, q)
+
+
+def test_attention_takes_a_row_list_with_padding(tl):
+    r = np.random.default_rng(13)
+    lens = [40, 7, 0, 300]
+    c, k, v, table, _ = filled_cache(tl, r, 1, 16, 2, 64, lens)
+    rows = [3, -1, 0, 3, 2, 1, -1]
+    q = normal(r, len(rows), 6, 64)
+    check_attention(tl, c, k[0], v[0], table, lens, 16, q, rows=rows)
+    assert tl.device_status() == 0
+
+
+@pytest.mark.parametrize("hd", [64, 7])
+def test_attention_never_follows_bad_ids(tl, hd):
+    """Pages outside the pool count as tokens that are not there; rows and lengths outside their tables as empty or cut."""
+    r = np.random.default_rng(14)
+    lens = [50, 50, 16, 50, 30, 20]
+    c, k, v, table, refs = filled_cache(tl, r, 1, 16, 1, hd, lens, max_pages=4, garbage=False)
+    bad = table.copy()
+    bad[0, 1] = k.shape[1]
+    bad[1, :4] = [-1, -9, 2 ** 31 - 1, -2 ** 31]
+    c.set_state(bad, [50, 50, -4, 50, 1 << 20, 20], refs)
+    q = normal(r, 8, 4, hd)
+    rows = [0, 1, 2, 3, 4, 5, 6, -3]
+    out, lse = c.attend(0, q, rows=rows)
+    assert tl.device_status() == 1
+    sound = {0: [t for t in range(50) if t // 16 != 1], 1: [], 2: [], 3: list(range(50)), 4: list(range(32)), 5: list(range(20)), 6: [], 7: []}
+    for b, ts in sound.items():
+        t = np.array(ts, int)
+        kk, vv = (a[0][table[rows[b], t // 16], t % 16, 0] if len(ts) else np.zeros((0, hd)) for a in (k, v))
+        for h in range(4):
+            o, l, to, tl_ = so.attend(q[b, h], kk, vv, hd ** -0.5)
+            close(out[b, h], o, to, (b, h))
+            assert (lse[b, h] == l) if not ts else abs(lse[b, h] - l) <= tl_
+    out, lse = c.attend(0, q[3:4], rows=[3])                                      # and nothing is left behind
+    check_attention(tl, c, k[0], v[0], table, lens, 16, q[3:4], rows=[3], got=(out, lse))
+    assert tl.device_status() == 0
+
+
+def test_attention_with_padded_rows_of_q_and_out_and_no_lse(tl):
+    r = np.random.default_rng(15)
+    lens, heads, hd = [70, 3, 0], 8, 64
+    c, k, v, table, _ = filled_cache(tl, r, 1, 16, 2, hd, lens)
+    pitch = heads * hd + 24
+    q = normal(r, 3, pitch)
+    dq, do = tl.DeviceBuffer.from_numpy(q), tl.DeviceBuffer.from_numpy(np.full((3, pitch), 5, np.float16))
+    w = tl.DeviceBuffer.from_numpy(np.zeros(32 << 20, np.uint8))
+    tl.check(tl.load().tl_paged_attn_decode_f16(C.byref(c.c), 0, dq.ptr, do.ptr, None, None, 3, heads, hd ** -0.5, pitch, pitch, w.ptr, w.nbytes, None), "attn")
+    got = do.to_numpy(np.float16, (3, pitch))
+    assert (got[:, heads * hd:] == 5).all()
+    ref = c.attend(0, np.ascontiguousarray(q[:, :heads * hd].reshape(3, heads, hd)))
+    assert np.array_equal(got[:, :heads * hd].reshape(3, heads, hd), ref[0])
+    check_attention(tl, c, k[0], v[0], table, lens, 16, q[:, :heads * hd].reshape(3, heads, hd), got=ref)
+
+
+def test_attention_beyond_32_bit_offsets(tl):
+    """Pages whose values lie more than 2^32 elements into the pool (a stride between small pages makes it so)."""
+    r = np.random.default_rng(16)
+    page, kv, hd, pages, stride = 16, 1, 128, 9, 1 << 29
+    lib = tl.load()
+    bytes_ = ((pages - 1) * stride + page * hd) * 2
+    kbuf, vbuf = tl.DeviceBuffer(bytes_), tl.DeviceBuffer(bytes_)
+    k, v = normal(r, pages, page, kv, hd), normal(r, pages, page, kv, hd)
+    for buf, a in ((kbuf, k), (vbuf, v)):
+        for p in range(pages):
+            x = np.ascontiguousarray(a[p])
+            tl.check(lib.tl_memcpy_h2d(buf.ptr + 2 * p * stride, x.ctypes.data, x.nbytes, None), "h2d")
+            tl.synchronize()
+    lens = [page * 8, 5]
+    table = np.full((2, 8), -1, np.int32)
+    table[0] = [8, 1, 2, 3, 7, 5, 6, 0]
+    table[1, 0] = 4
+    c = tl.PagedCache(1, pages, page, kv, hd, 2, 8)
+    refs = np.ones(pages, np.int32)
+    c.set_state(table, lens, refs)
+    c.c.k_pages, c.c.v_pages, c.c.page_stride, c.c.layer_stride = kbuf.ptr, vbuf.ptr, stride, pages * stride
+    q = normal(r, 2, 4, hd)
+    check_attention(tl, c, k, v, table, lens, page, q)
+    nk, nv = normal(r, 1, kv, hd), normal(r, 1, kv, hd)
+    c.append(0, None, nk, nv, [page * 8 - 1 - 7 * page], None, rows=[0])         # slot 15 of page 8
+    k[8, page - 1], v[8, page - 1] = nk[0], nv[0]
+    c.copy([8], [4])
+    k[4], v[4] = k[8], v[8]
+    check_attention(tl, c, k, v, table, lens, page, q)
+    assert tl.device_status() == 0
+
+
+# ---- the pages' own operations ------------------------------------------------------------------------------------------
+def same_books(c, pg):
+    for got, want, name in zip(c.state(), (pg.table, pg.lengths, pg.refs), ("table", "lengths", "refs")):
+        assert np.array_equal(got, want), name
+
+
+@pytest.mark.parametrize("seed,pages,page,rows,width,layers,kv,hd,by_head", [(1, 40, 4, 6, 9, 2, 2, 16, False), (2, 300, 16, 40, 12, 1, 1, 8, True),
+                                                                            (3, 2500, 3, 1500, 5, 1, 1, 7, False), (4, 9, 1, 3, 4, 3, 3, 24, False),
+                                                                            (5, 1024, 8, 64, 40, 1, 2, 8, False)])
+def test_pages_over_many_steps(tl, seed, pages, page, rows, width, layers, kv, hd, by_head):
+    r = np.random.default_rng(seed)
+    k, v = normal(r, layers, pages, page, kv, hd), normal(r, layers, pages, page, kv, hd)
+    c, pg = tl.PagedCache(layers, pages, page, kv, hd, rows, width, by_head, k, v), so.Pages(pages, page, rows, width)
+    refused = 0
+    for step in range(40):
+        what = step % 4
+        if what == 1:
+            parents = np.arange(rows)
+            some = r.random(rows) < 0.4
+            parents[some] = r.integers(-1, rows, some.sum())
+            pg.fork(parents)
+            c.fork(parents)
+        elif what == 3 and step % 8 == 3:
+            drop = np.where(r.random(rows) < 0.4, -1, np.arange(rows))
+            pg.fork(drop)
+            c.fork(drop)
+            moved, live, moves = pg.compact()
+            got = c.compact()
+            assert np.array_equal(got[0], moved) and got[1] == live
+            for s, d in moves:
+                k[:, d], v[:, d] = k[:, s], v[:, s]
+        else:
+            new = r.integers(0, 2 if what else page + 2, rows)
+            want, copies = pg.reserve(new)
+            assert c.reserve(new) == want
+            refused += want != 0
+            for s, d, n in copies:
+                k[:, d, :n], v[:, d, :n] = k[:, s, :n], v[:, s, :n]
+        same_books(c, pg)
+        if want_contents(step):
+            gk, gv = c.pools()
+            assert np.array_equal(gk, k) and np.array_equal(gv, v), step
+    assert tl.device_status() == 0
+
+
+def want_contents(step):
+    return step % 5 == 4 or step > 36
+
+
+def test_pages_refuse_without_changing_anything(tl):
+    c, pg = tl.PagedCache(1, 6, 4, 1, 8, 4, 3), so.Pages(6, 4, 4, 3)
+    for new in ([5, 3, 0, 0], [1, 1, 1, 1]):
+        assert c.reserve(new) == pg.reserve(new)[0] == 0
+    c.fork([0, 1, 0, 0])
+    pg.fork([0, 1, 0, 0])
+    for new in ([1, 1, 1, 1], [9, 0, 0, 0], [0, 9, 0, 0], [2, 2, 2, 2]):           # no page left for every copy; more than max_pages
+        want, _ = pg.reserve(new)
+        assert c.reserve(new) == want
+        same_books(c, pg)
+    assert tl.device_status() == 0
+    assert c.reserve([0, -1, 0, 0]) == 1                                         # no such number of tokens
+    assert tl.device_status() == 1
+    same_books(c, pg)
+    table, lengths, refs = c.state()
+    bad = table.copy()
+    assert lengths[0] % 4                                                        # its next token goes into its last page
+    bad[0, lengths[0] // 4] = 77
+    c.set_state(bad, lengths, refs)
+    assert c.reserve([1, 0, 0, 0]) == 1 and tl.device_status() == 1               # an entry that names no page
+    c.set_state(table, lengths, refs)
+    c.fork([0, 4, -2, 3])                                                        # parents that are no rows: those rows stay
+    assert tl.device_status() == 1
+    same_books(c, pg)
+    c.copy([0, 9, 2], [3, 1, -1])
+    assert tl.device_status() == 1
+
+
+@pytest.mark.parametrize("shape,by_head", [((2, 30, 16, 4, 64), False), ((3, 12, 5, 3, 7), False), ((1, 40, 8, 2, 24), True)])
+def test_page_copies(tl, shape, by_head):
+    r = np.random.default_rng(21)
+    k, v = normal(r, *shape), normal(r, *shape)
+    c = tl.PagedCache(*shape, 2, 4, by_head, k, v)
+    src, dst = [1, 3, -1, 5, 9, 0], [2, 4, 6, 5, 8, 11]
+    c.copy(src, dst)
+    for s, d in zip(src, dst):
+        if s >= 0:
+            k[:, d], v[:, d] = k[:, s], v[:, s]
+    gk, gv = c.pools()
+    assert np.array_equal(gk, k) and np.array_equal(gv, v) and tl.device_status() == 0
+
+
+def test_pages_with_gaps_between_tokens_and_heads(tl):
+    """Strides wider than the rows: contents move, gaps stay."""
+    r = np.random.default_rng(22)
+    L, P, s, H, d = 2, 6, 4, 3, 8
+    for hs, ts in ((8, 40), (16, 48), (80, 16)):          # heads packed; neither; by head with gaps
+        ps = max(ts * s, hs * H) + 8
+        flat = normal(r, 2, L * P * ps)
+        bufs = [tl.DeviceBuffer.from_numpy(a) for a in flat]
+        c = tl.PagedCache(L, P, s, H, d, 3, 4)
+        c.c.k_pages, c.c.v_pages, c.c.layer_stride, c.c.page_stride, c.c.token_stride, c.c.head_stride = bufs[0].ptr, bufs[1].ptr, P * ps, ps, ts, hs
+        pg = so.Pages(P, s, 3, 4)
+        for new in ([3, 0, 0],):
+            assert c.reserve(new) == pg.reserve(new)[0] == 0
+        c.fork([0, 0, 0])
+        pg.fork([0, 0, 0])
+        want, copies = pg.reserve([1, 1, 0])
+        assert c.reserve([1, 1, 0]) == want == 0 and len(copies) == 2
+        c.copy([copies[0][1]], [5])
+        for a in flat:
+            def at(l, p, t, h):
+                return slice(l * P * ps + p * ps + t * ts + h * hs, l * P * ps + p * ps + t * ts + h * hs + d)
+            for src, dst, n in copies + [(copies[0][1], 5, s)]:
+                for l in range(L):
+                    for t in range(n):
+                        for h in range(H):
+                            a[at(l, dst, t, h)] = a[at(l, src, t, h)]
+        for a, b in zip(flat, bufs):
+            assert np.array_equal(b.to_numpy(np.float16, a.shape), a), (hs, ts)
+        same_books(c, pg)
+
+
+# ---- beams ---------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("batch,beams,vocab,k", BEAM_SHAPES)
+@pytest.mark.parametrize("with_finished", [False, True])
+def test_beam_selection(tl, batch, beams, vocab, k, with_finished):
+    x, s, fin = beam_case(batch, beams, vocab, 1)
+    pad = min(2, vocab - 1)
+    with np.errstate(all="ignore"):
+        want = so.beam_select(x, s, beams, k, fin if with_finished else None, pad)
+    got = tl.beam_select(x, s, beams, k, fin if with_finished else None, pad)
+    assert np.array_equal(got[1], want[1]) and np.array_equal(got[2], want[2])
+    # the log of the sum is good to 2^-21 (32-bit exponentials), and the result rounded once
+    close(got[0], want[0], np.abs(want[0]) * 2.0 ** -24 + 2.0 ** -21)
+    again = tl.beam_select(x, s, beams, k, fin if with_finished else None, pad)
+    assert all(np.array_equal(a, b) for a, b in zip(got, again))
+
+
+def test_beam_selection_first_step_and_nothing_left(tl):
+    r = np.random.default_rng(31)
+    x = normal(r, 8, 1000, std=3)
+    x[:4] = x[0]                                                     # all beams of an entry start out alike, one is live
+    s = np.array([0, -np.inf, -np.inf, -np.inf, -1, -np.inf, -np.inf, np.nan], np.float32)
+    want = so.beam_select(x, s, 4, 8)
+    got = tl.beam_select(x, s, 4, 8)
+    assert np.array_equal(got[1], want[1]) and np.array_equal(got[2], want[2])
+    got = tl.beam_select(x, np.full(8, -np.inf, np.float32), 4, 5)      # no live beam: the first candidates, at -inf
+    assert (got[0] == -np.inf).all() and np.array_equal(got[2], [np.arange(5)] * 2) and np.array_equal(got[1], [[0] * 5, [4] * 5])
+    got = tl.beam_select(np.full((2, 1000), -np.inf, np.float16), np.zeros(2, np.float32), 2, 3)
+    assert (got[0] == -np.inf).all() and np.array_equal(got[2], [[0, 1, 2]]) and np.array_equal(got[1], [[0, 0, 0]])
+    got = tl.beam_select(np.zeros((3, 700), np.float16), np.zeros(3, np.float32), 3, 70)   # every candidate equal: the lowest indices
+    assert np.array_equal(got[2][0], np.arange(70)) and (got[1] == 0).all()
+    z = np.full((1, 700), -0.0, np.float16)
+    z[0, 500:] = 0.0
+    assert np.array_equal(tl.beam_select(z, [0.0], 1, 9)[2][0], np.arange(9))              # -0 equals +0
+
+
+@pytest.mark.parametrize("stride,off", [(1004, 0), (1001, 0), (1008, 3)])
+def test_beam_selection_with_row_strides(tl, stride, off):
+    """Rows that start at any 2-byte boundary; what lies behind a row is not read as a candidate."""
+    r = np.random.default_rng(32)
+    rows, vocab, k = 6, 1000, 6
+    flat = np.full(rows * stride + 8, 60000, np.float16)
+    x = normal(r, rows, vocab, std=3)
+    for i in range(rows):
+        flat[off + i * stride: off + i * stride + vocab] = x[i]
+    s = (-r.random(rows)).astype(np.float32)
+    need = C.c_size_t(0)
+    lib = tl.load()
+    tl.check(lib.tl_beam_select_workspace(2, 3, vocab, k, C.byref(need)), "ws")
+    w = tl.DeviceBuffer.from_numpy(np.zeros(max(16, need.value), np.uint8))
+    dx, ds, outs = tl.DeviceBuffer.from_numpy(flat), tl.DeviceBuffer.from_numpy(s), [tl.DeviceBuffer(2 * k * 4) for _ in range(3)]
+    tl.check(lib.tl_beam_select_f16(dx.ptr + 2 * off, stride, ds.ptr, None, 0, 2, 3, vocab, k, outs[0].ptr, outs[1].ptr, outs[2].ptr, w.ptr, w.nbytes, None), "select")
+    want = so.beam_select(x, s, 3, k)
+    assert np.array_equal(outs[1].to_numpy(np.int32, (2, k)), want[1]) and np.array_equal(outs[2].to_numpy(np.int32, (2, k)), want[2])
+
+
+@pytest.mark.parametrize("outer,rows,pitch,used", [(1, 1, 8, 8), (2, 5, 24, 17), (3, 4, 70000, 69993), (2, 7, 33, 33), (4, 64, 4096, 1000)])
+def test_beam_reorder(tl, outer, rows, pitch, used):
+    r = np.random.default_rng([outer, rows, pitch])
+    src, dst = normal(r, outer, rows, pitch), normal(r, outer, rows, pitch)
+    parents = r.integers(0, rows, rows).astype(np.int32)
+    if rows > 3:
+        parents[2] = -1
+    got = tl.beam_reorder(src, dst, parents, used)
+    want = dst.copy()
+    for i, p in enumerate(parents):
+        if p >= 0:
+            want[:, i, :used] = src[:, p, :used]
+    assert np.array_equal(got, want) and tl.device_status() == 0
+    if rows > 3:
+        parents[0], parents[1] = rows, -2
+        got = tl.beam_reorder(src, dst, parents, used)
+        want[:, :2] = dst[:, :2]
+        assert np.array_equal(got, want) and tl.device_status() == 1
+
+
+# ---- together ------------------------------------------------------------------------------------------------------
+def test_a_beam_search_over_pages_matches_one_over_copied_sequences(tl):
+    """Select, fork, reserve, append and attend for 3 entries of 4 beams over 2 layers and 30 steps, against beams that carry
+    their whole history with them. Queries, keys, values and logits are functions of the token and step alone."""
+    r = np.random.default_rng(41)
+    batch, beams, vocab, layers, kv, heads, hd, page, steps = 3, 4, 50, 2, 2, 6, 64, 8, 30
+    rows = batch * beams
+    emb = normal(r, vocab, 2, heads + 2 * kv, hd)
+    lm = normal(r, vocab, vocab, std=2)
+    f, mag = tl.rotary_frequencies(hd, scaling="parts", factor=4.0, trained_len=16, low=1, high=4)
+    c = tl.PagedCache(layers, 120, page, kv, hd, rows, 8)
+    hist = [[] for _ in range(rows)]
+    scores = np.where(np.arange(rows) % beams == 0, 0.0, -np.inf).astype(np.float32)
+    fin = np.zeros(rows, np.uint8)
+    tokens = np.arange(rows) // beams
+    for step in range(steps):
+        assert c.reserve(np.ones(rows, np.int32)) == 0
+        hist = [h + [int(t)] for h, t in zip(hist, tokens)]
+        pos = np.full(rows, step, np.int32)
+        e = emb[tokens]
+        for layer in range(layers):
+            q = c.append(layer, np.ascontiguousarray(e[:, layer, :heads]), np.ascontiguousarray(e[:, layer, heads:heads + kv]),
+                         np.ascontiguousarray(e[:, layer, heads + kv:]), pos, f, mag, True)
+            out, lse = c.attend(layer, q)
+            if step % 7 == 6 or step == steps - 1:
+                for i in range(rows):
+                    k = np.stack([so.rotary(emb[t, layer, heads:heads + kv][None], [s], f, mag, True)[0][0] for s, t in enumerate(hist[i])]).astype(np.float16)
+                    v = np.stack([emb[t, layer, heads + kv:] for t in hist[i]])
+                    for h in range(heads):
+                        o, l, to, tl_ = so.attend(q[i, h], k[:, h // 3], v[:, h // 3], hd ** -0.5)
+                        # keys here are rounded from 64 bits, there from 32: a step of fp16 apart where the two fall apart
+                        slack = 2 * 2 * so.EPS16 * (np.abs(k[:, h // 3]).astype(np.float64) @ np.abs(q[i, h]).astype(np.float64)).max() * hd ** -0.5
+                        close(out[i, h], o, to + slack * np.abs(v[:, h // 3]).astype(np.float64).max(0), (step, i, h))
+                        assert abs(lse[i, h] - l) <= tl_ + slack
+        logits = np.stack([lm[t] + np.float16(0.01 * (step % 3)) for t in tokens]).astype(np.float16)
+        want = so.beam_select(logits, scores, beams, beams, fin, 1)
+        got = tl.beam_select(logits, scores, beams, beams, fin, 1)
+        assert np.array_equal(got[1], want[1]) and np.array_equal(got[2], want[2]), step
+        parents, tokens, scores = got[1].reshape(-1), got[2].reshape(-1), got[0].reshape(-1)
+        c.fork(parents)
+        hist = [list(hist[p]) for p in parents]
+        fin = fin[parents] | (tokens == 1)
+        table, lengths, refs = c.state()
+        want_refs = np.zeros_like(refs)
+        np.add.at(want_refs, table[table >= 0], 1)
+        assert np.array_equal(refs, want_refs)
+        if step % 10 == 9:
+            c.compact()
+    assert tl.device_status() == 0
+
+
+def test_on_two_streams_and_from_a_graph(tl):
+    """The calls enqueue on the stream that they are given; captured once, replayed on changed inputs."""
+    torch = pytest.importorskip("torch")
+    r = np.random.default_rng(51)
+    lib = tl.load()
+    lens, heads, hd, page = [900, 31, 0, 2000], 8, 64, 16
+    c, k, v, table, _ = filled_cache(tl, r, 1, page, 2, hd, lens)
+    beams, vocab, kk = 4, 5000, 8
+    need = C.c_size_t(0)
+    tl.check(lib.tl_beam_select_workspace(1, beams, vocab, kk, C.byref(need)), "ws")
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    state = []
+    for i in range(2):
+        q, x = normal(r, 4, heads, hd), normal(r, beams, vocab, std=3)
+        s = dict(q=torch.from_numpy(q).cuda(), out=torch.zeros(4, heads, hd, dtype=torch.float16, device="cuda"),
+                 w=torch.zeros(32 << 20, dtype=torch.uint8, device="cuda"), x=torch.from_numpy(x).cuda(), s=torch.zeros(beams, device="cuda"),
+                 v=torch.zeros(kk, device="cuda"), p=torch.zeros(kk, dtype=torch.int32, device="cuda"), t=torch.zeros(kk, dtype=torch.int32, device="cuda"),
+                 bw=torch.zeros(max(need.value, 16), dtype=torch.uint8, device="cuda"))
+        state.append((q, x, s))
+    torch.cuda.synchronize()
+
+    def call(s, stream):
+        tl.check(lib.tl_paged_attn_decode_f16(C.byref(c.c), 0, s["q"].data_ptr(), s["out"].data_ptr(), None, None, 4, heads, hd ** -0.5, heads * hd,
+                                              heads * hd, s["w"].data_ptr(), s["w"].numel(), stream), "attn")
+        tl.check(lib.tl_beam_select_f16(s["x"].data_ptr(), vocab, s["s"].data_ptr(), None, 0, 1, beams, vocab, kk, s["v"].data_ptr(), s["p"].data_ptr(),
+                                        s["t"].data_ptr(), s["bw"].data_ptr(), s["bw"].numel(), stream), "select")
+
+    def verify(i):
+        q, x, s = state[i]
+        ref = c.attend(0, q)[0]
+        assert np.array_equal(s["out"].cpu().numpy(), ref)
+        assert np.array_equal(s["t"].cpu().numpy(), so.beam_select(x, np.zeros(beams), beams, kk)[2][0])
+    for rep in range(20):
+        for i in range(2):
+            call(state[i][2], streams[i].cuda_stream)
+    torch.cuda.synchronize()
+    verify(0)
+    verify(1)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=streams[0]):
+        call(state[0][2], torch.cuda.current_stream().cuda_stream)
+    for rep in range(3):
+        q, x = normal(r, 4, heads, hd), normal(r, beams, vocab, std=3)
+        state[0] = (q, x, state[0][2])
+        state[0][2]["q"].copy_(torch.from_numpy(q))
+        state[0][2]["x"].copy_(torch.from_numpy(x))
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        verify(0)
+    del g
+    assert tl.device_status() == 0
