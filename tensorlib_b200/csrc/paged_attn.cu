@@ -98,9 +98,457 @@ __global__ void __launch_bounds__(ANY_WARPS * 32) k_paged_attn_any(AttnLaunch p)
     if (threadIdx.x == 0 && p.lse) p.lse[(long long)b * p.n_heads + h] = L > 0.f ? M + logf(L) : -INFINITY;
 }
 
+
+// ---- the tensor-core kernel ----------------------------------------------------------------------------------------
+// For rows of head_dim values that start on 16 bytes. Per KV head the `group` query heads are the columns of the products
+//   S^T [16 tokens x 8 heads] = K_tile Q^T,   O^T [dims x 8 heads] += V_tile^T P^T        (mma.m16n8k16, fp32 sums)
+// so that eight heads cost what one does. P^T leaves the accumulators of the first product through a transposing register
+// move and enters the second as its B operand; it is split into two fp16 parts, which keeps the weights to 2^-22.
+//
+// HBM bound: K and V are read once, and a tile of 16 tokens costs some 250 warp instructions against the 360 cycles that an
+// SM's share of the memory needs for its 8 KB. Each warp streams its own tiles through a private ring of shared memory
+// (cp.async, zero-filled behind the last token and for ids outside the pool, so nothing unwritten is ever multiplied);
+// page ids are looked up one tile further ahead. Warps meet only at the end of a (sequence, head group).
+//
+// The work of all sequences, counted in units of 64 tokens, is cut into equal contiguous ranges, one a CTA: ragged batches
+// fill the machine whatever their lengths, one long sequence as well as many. A (sequence, head group) that falls into one
+// range is finished there; one that is cut leaves partial results (max, sum, sums of values) in the workspace, and the CTA
+// that comes last joins them, in order of the ranges.
+constexpr int FL_WARPS = 4;
+constexpr int FL_THREADS = FL_WARPS * 32;
+constexpr int FL_TILE = 16;                       // tokens of a warp's tile
+constexpr int FL_UNIT = FL_TILE * FL_WARPS;
+constexpr int FL_MAX_SMS = 160;
+
+struct FlashLaunch {
+    AttnLaunch a;
+    int chunk, chunks, groups;                    // query heads of a head group, head groups a KV head, head groups in all
+    float scale_log2;
+    unsigned int* counters; float* partial;       // workspace: [CTAs], [2 CTAs][chunk][head_dim + 2]
+};
+
+template <int HDP, int NT>
+struct FlashShape {
+    static constexpr int STAGES = HDP == 64 ? 4 : (HDP == 128 ? 3 : 2);
+    static constexpr int CTAS = HDP == 64 ? 3 : (HDP == 128 ? 2 : 1);     // per SM
+    static constexpr int TILE_BYTES = FL_TILE * HDP * 2;
+    static constexpr int RING = FL_WARPS * STAGES * 2 * TILE_BYTES;
+    static constexpr int HEADS = 8 * NT;
+    // words between heads: + 4 makes the accumulator stores conflict-free, + 2 lets two CTAs of 16 heads fit an SM
+    static constexpr int PITCH = NT == 1 ? HDP + 4 : HDP + 2;
+    static constexpr int SLAB = HEADS * PITCH * 4;
+    static constexpr int SMEM = RING + 2 * SLAB + FL_WARPS * HEADS * 8 + FL_WARPS * STAGES * 4;
+};
+
+__device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
+    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
+// a place in the flattened (sequence, head group, unit) space
+struct Cursor {
+    int b, row, len, units, hg, i;
+    long long left;                               // units of this CTA's range from here on
+};
+
+__device__ __forceinline__ int units_of(int len) { return (len + FL_UNIT - 1) / FL_UNIT; }
+
+__device__ __forceinline__ void advance(const FlashLaunch& p, Cursor& c) {
+    if (--c.left <= 0) return;
+    if (++c.i < c.units) return;
+    c.i = 0;
+    if (++c.hg < p.groups) return;
+    c.hg = 0;
+    do {
+        c.b++;
+        c.len = row_tokens(p.a, c.b, c.row);
+        c.units = units_of(c.len);
+    } while (c.units == 0);
+}
+
+template <int HDP, int NT>
+__global__ void __launch_bounds__(FL_THREADS, FlashShape<HDP, NT>::CTAS) k_paged_attn(FlashLaunch p) {
+    using F = FlashShape<HDP, NT>;
+    extern __shared__ __align__(128) unsigned char sm[];
+    float* slabs = reinterpret_cast<float*>(sm + F::RING);
+    float2* stats = reinterpret_cast<float2*>(sm + F::RING + 2 * F::SLAB);                                   // [warp][head]: max, sum
+    uint32_t* masks = reinterpret_cast<uint32_t*>(sm + F::RING + 2 * F::SLAB + FL_WARPS * F::HEADS * 8);     // [warp][stage]
+    __shared__ unsigned long long scan_sh[FL_WARPS];
+    __shared__ unsigned long long start_sh[2];
+    __shared__ int last_sh;
+    const AttnLaunch& a = p.a;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, hd = a.head_dim;
+    pdl_launch_dependents();
+    pdl_wait();
+
+    // 1: this CTA's range. Every CTA adds up the units of all sequences; a thread takes a run of them.
+    const int per_thread = (a.batch + FL_THREADS - 1) / FL_THREADS;
+    const int b0 = min(a.batch, tid * per_thread), b1 = min(a.batch, b0 + per_thread);
+    unsigned long long mine = 0;
+    for (int b = b0; b < b1; b++) {
+        int row;
+        mine += units_of(row_tokens(a, b, row));
+    }
+    unsigned long long upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const unsigned long long y = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += y;
+    }
+    if (lane == 31) scan_sh[warp] = upto;
+    __syncthreads();
+    unsigned long long before = upto - mine, total = 0;
+#pragma unroll
+    for (int w = 0; w < FL_WARPS; w++) {
+        if (w < warp) before += scan_sh[w];
+        total += scan_sh[w];
+    }
+    const unsigned long long U = total * p.groups;
+    const unsigned long long per = (U + gridDim.x - 1) / gridDim.x;
+    const unsigned long long u0 = per * blockIdx.x, u1 = u0 + per < U ? u0 + per : U;
+    // sequences with nothing to attend to
+    for (int b = blockIdx.x; b < a.batch; b += gridDim.x) {
+        int row;
+        if (row_tokens(a, b, row) == 0) {
+            for (int i = tid; i < a.n_heads * hd; i += FL_THREADS) a.out[b * a.o_row + i] = __float2half_rn(0.f);
+            if (a.lse)
+                for (int h = tid; h < a.n_heads; h += FL_THREADS) a.lse[(long long)b * a.n_heads + h] = -INFINITY;
+        }
+    }
+    if (u0 >= u1) return;
+    if (u0 >= before * p.groups && u0 < (before + mine) * p.groups) {      // one thread's run holds the start
+        unsigned long long at = before;
+        for (int b = b0; b < b1; b++) {
+            int row;
+            const int n = units_of(row_tokens(a, b, row));
+            if (u0 < (at + n) * p.groups) {
+                start_sh[0] = (unsigned long long)b;
+                start_sh[1] = at;
+                break;
+            }
+            at += n;
+        }
+    }
+    __syncthreads();
+    Cursor cur;                                   // what is computed next
+    cur.b = (int)start_sh[0];
+    cur.len = row_tokens(a, cur.b, cur.row);
+    cur.units = units_of(cur.len);
+    {
+        const unsigned long long in = u0 - start_sh[1] * p.groups;
+        cur.hg = (int)(in / cur.units);
+        cur.i = (int)(in - (unsigned long long)cur.hg * cur.units);
+    }
+    cur.left = (long long)(u1 - u0);
+    Cursor ahead = cur;                           // what is looked up next
+
+    // 2: loads. lookup(): the page id of this lane's token (lanes 16.. repeat 0..15); issue(): the tile's rows.
+    int raw = 0, slot = -1, raw_hg = 0;
+    auto lookup = [&]() {
+        slot = -1;
+        if (ahead.left > 0) {
+            const int tok = ahead.i * FL_UNIT + warp * FL_TILE + (lane & 15);
+            raw_hg = ahead.hg;
+            if (tok < ahead.len) {
+                unsigned pg, s;
+                a.by_page.divmod((unsigned)tok, pg, s);
+                slot = (int)s;
+                raw = a.table[(long long)ahead.row * a.max_pages + pg];
+            }
+            advance(p, ahead);
+        }
+    };
+    constexpr int CPR = HDP / 8;                  // 16-byte chunks a row
+    constexpr int ROWS = 32 / CPR;                // rows an instruction
+    const int chunk = lane % CPR;
+    const bool in_row = chunk * 8 < hd;
+    unsigned char* ring = sm + warp * F::STAGES * 2 * F::TILE_BYTES;
+    auto issue = [&](int stage) {
+        long long off = -1;
+        if (slot >= 0) {
+            if ((unsigned)raw < (unsigned)a.n_pages) off = raw * a.page_stride + slot * a.token_stride + (long long)(raw_hg / p.chunks) * a.head_stride;
+            else atomicExch(a.status, TL_ERR_INVALID_ARGUMENT);
+        }
+        const uint32_t mask = __ballot_sync(0xffffffffu, off >= 0) & 0xffffu;
+        if (lane == 0) masks[warp * F::STAGES + stage] = mask;
+        if (mask) {
+            const uint32_t kd = smem_addr(ring + stage * 2 * F::TILE_BYTES), vd = kd + F::TILE_BYTES;
+#pragma unroll
+            for (int r0 = 0; r0 < FL_TILE; r0 += ROWS) {
+                const int r = r0 + lane / CPR;
+                const long long o = __shfl_sync(0xffffffffu, off, r);
+                const bool ok = o >= 0 && in_row;
+                const long long at = ok ? o + chunk * 8 : 0;
+                const uint32_t d = r * (HDP * 2) + ((chunk ^ (r & 7)) << 4);
+                cp_async16(kd + d, a.k + at, ok ? 16 : 0);
+                cp_async16(vd + d, a.v + at, ok ? 16 : 0);
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll
+    for (int s = 0; s < F::STAGES - 1; s++) {
+        lookup();
+        issue(s);
+    }
+    lookup();
+
+    // 3: the range, segment by segment (one (sequence, head group) each)
+    const int g = lane >> 2, t = lane & 3;        // fragment row and column pair
+    int stage = 0;
+    while (cur.left > 0) {
+        const int kvh = cur.hg / p.chunks, h0 = kvh * a.group + (cur.hg - kvh * p.chunks) * p.chunk;
+        const int heads = min(p.chunk, (kvh + 1) * a.group - h0);
+        const long long seg_units = min((long long)(cur.units - cur.i), cur.left);
+        const int seg_b = cur.b, seg_hg = cur.hg, seg_i = cur.i, seg_n = cur.units;
+        uint32_t q[NT][HDP / 16][2];
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int ks = 0; ks < HDP / 16; ks++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    const int h = n * 8 + g, d = ks * 16 + j * 8 + t * 2;
+                    q[n][ks][j] = h < heads && d < hd ? *reinterpret_cast<const uint32_t*>(a.q + seg_b * a.q_row + (long long)(h0 + h) * hd + d) : 0u;
+                }
+        float o[NT][HDP / 16][4], m[NT][2], l[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            m[n][0] = m[n][1] = -INFINITY;
+            l[n][0] = l[n][1] = 0.f;
+#pragma unroll
+            for (int j = 0; j < HDP / 16; j++) o[n][j][0] = o[n][j][1] = o[n][j][2] = o[n][j][3] = 0.f;
+        }
+        for (long long u = 0; u < seg_units; u++) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(F::STAGES - 2) : "memory");
+            __syncwarp();
+            const uint32_t mask = masks[warp * F::STAGES + stage];
+            {
+                const int next = stage == 0 ? F::STAGES - 1 : stage - 1;       // the stage computed last
+                issue(next);
+                lookup();
+            }
+            if (mask) {
+                const uint32_t ks_base = smem_addr(ring + stage * 2 * F::TILE_BYTES), vs_base = ks_base + F::TILE_BYTES;
+                float s[NT][4];
+#pragma unroll
+                for (int n = 0; n < NT; n++) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+                const int kr = lane & 15;
+#pragma unroll
+                for (int ks = 0; ks < HDP / 16; ks++) {
+                    uint32_t f[4];
+                    ldsm4(f, ks_base + kr * (HDP * 2) + (((2 * ks + (lane >> 4)) ^ (kr & 7)) << 4));
+#pragma unroll
+                    for (int n = 0; n < NT; n++) mma16816(s[n], f, q[n][ks][0], q[n][ks][1]);
+                }
+                const bool in0 = mask >> g & 1, in1 = mask >> (g + 8) & 1;
+                uint32_t ph[NT][2], pl[NT][2];
+                float keep[NT][2];
+                bool moved = false;
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+#pragma unroll
+                    for (int j = 0; j < 2; j++) {
+                        const float x0 = in0 ? s[n][j] * p.scale_log2 : -INFINITY, x1 = in1 ? s[n][j + 2] * p.scale_log2 : -INFINITY;
+                        float mx = fmaxf(x0, x1);
+                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+                        const float mn = fmaxf(m[n][j], mx);
+                        const float ref = mn == -INFINITY ? 0.f : mn;
+                        keep[n][j] = exp2f(m[n][j] - ref);
+                        moved |= mn != m[n][j];
+                        m[n][j] = mn;
+                        s[n][j] = exp2f(x0 - ref);
+                        s[n][j + 2] = exp2f(x1 - ref);
+                        l[n][j] = l[n][j] * keep[n][j] + (s[n][j] + s[n][j + 2]);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 2; j++) {
+                        const __half2 hi = __floats2half2_rn(s[n][2 * j], s[n][2 * j + 1]);
+                        const float2 hf = __half22float2(hi);
+                        const __half2 lo = __floats2half2_rn(s[n][2 * j] - hf.x, s[n][2 * j + 1] - hf.y);
+                        ph[n][j] = transpose8x8(*reinterpret_cast<const uint32_t*>(&hi));
+                        pl[n][j] = transpose8x8(*reinterpret_cast<const uint32_t*>(&lo));
+                    }
+                }
+                if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+                    for (int n = 0; n < NT; n++)
+#pragma unroll
+                        for (int j = 0; j < HDP / 16; j++) {
+                            o[n][j][0] *= keep[n][0];
+                            o[n][j][1] *= keep[n][1];
+                            o[n][j][2] *= keep[n][0];
+                            o[n][j][3] *= keep[n][1];
+                        }
+                }
+                const int vr = (lane & 7) + ((lane >> 4) << 3), vc = (lane >> 3) & 1;
+#pragma unroll
+                for (int j = 0; j < HDP / 16; j++) {
+                    uint32_t f[4];
+                    ldsm4t(f, vs_base + vr * (HDP * 2) + (((2 * j + vc) ^ (vr & 7)) << 4));
+#pragma unroll
+                    for (int n = 0; n < NT; n++) {
+                        mma16816(o[n][j], f, ph[n][0], ph[n][1]);
+                        mma16816(o[n][j], f, pl[n][0], pl[n][1]);
+                    }
+                }
+            }
+            __syncwarp();
+            stage = stage + 1 == F::STAGES ? 0 : stage + 1;
+            advance(p, cur);
+        }
+        // 4: the warps' results become one. Sums of the weights over the eight rows of lanes first.
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                l[n][j] += __shfl_xor_sync(0xffffffffu, l[n][j], 4);
+                l[n][j] += __shfl_xor_sync(0xffffffffu, l[n][j], 8);
+                l[n][j] += __shfl_xor_sync(0xffffffffu, l[n][j], 16);
+                if (g == 0) stats[warp * F::HEADS + n * 8 + 2 * t + j] = make_float2(m[n][j], l[n][j]);
+            }
+        __syncthreads();
+        float top[NT][2], fac[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                float M = -INFINITY;
+#pragma unroll
+                for (int w = 0; w < FL_WARPS; w++) M = fmaxf(M, stats[w * F::HEADS + n * 8 + 2 * t + j].x);
+                top[n][j] = M == -INFINITY ? 0.f : M;
+                fac[n][j] = exp2f(m[n][j] - top[n][j]);
+            }
+        auto store_slab = [&](int slab, bool add) {
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int j = 0; j < HDP / 16; j++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const int h = n * 8 + 2 * t + (e & 1), d = j * 16 + g + (e >> 1) * 8;
+                        float* at = slabs + slab * (F::SLAB / 4) + h * F::PITCH + d;
+                        const float x = o[n][j][e] * fac[n][e & 1];
+                        *at = add ? *at + x : x;
+                    }
+        };
+        if (warp >= 2) store_slab(warp - 2, false);
+        __syncthreads();
+        if (warp < 2) store_slab(warp, true);
+        __syncthreads();
+        const bool whole = seg_i == 0 && seg_units == seg_n;
+        const int slot_index = 2 * (int)blockIdx.x + (seg_i == 0);
+        float* part = p.partial + (long long)slot_index * p.chunk * (hd + 2);
+        for (int i = tid; i < heads * hd; i += FL_THREADS) {
+            const int h = i / hd, d = i - h * hd;
+            const float x = slabs[h * F::PITCH + d] + slabs[F::SLAB / 4 + h * F::PITCH + d];
+            if (whole) {
+                float M = -INFINITY, L = 0.f;
+#pragma unroll
+                for (int w = 0; w < FL_WARPS; w++) M = fmaxf(M, stats[w * F::HEADS + h].x);
+                const float ref = M == -INFINITY ? 0.f : M;
+#pragma unroll
+                for (int w = 0; w < FL_WARPS; w++) L += stats[w * F::HEADS + h].y * exp2f(stats[w * F::HEADS + h].x - ref);
+                a.out[seg_b * a.o_row + (long long)(h0 + h) * hd + d] = __float2half_rn(L > 0.f ? x / L : 0.f);
+            } else {
+                part[h * (hd + 2) + 2 + d] = x;
+            }
+        }
+        if (tid < heads) {
+            float M = -INFINITY, L = 0.f;
+#pragma unroll
+            for (int w = 0; w < FL_WARPS; w++) M = fmaxf(M, stats[w * F::HEADS + tid].x);
+            const float ref = M == -INFINITY ? 0.f : M;
+#pragma unroll
+            for (int w = 0; w < FL_WARPS; w++) L += stats[w * F::HEADS + tid].y * exp2f(stats[w * F::HEADS + tid].x - ref);
+            if (whole) {
+                if (a.lse) a.lse[(long long)seg_b * a.n_heads + h0 + tid] = L > 0.f ? (M + log2f(L)) * 0.69314718055994531f : -INFINITY;
+            } else {
+                part[tid * (hd + 2)] = M;
+                part[tid * (hd + 2) + 1] = L;
+            }
+        }
+        if (!whole) {
+            // the ranges that hold a piece of it: CTAs first .. last; the last to arrive joins them
+            const unsigned long long base = (cur.left > 0 ? u1 - cur.left : u1) - seg_units - seg_i;
+            const int first = (int)(base / per), last = (int)((base + seg_n - 1) / per);
+            __threadfence();
+            __syncthreads();
+            if (tid == 0) {
+                last_sh = atomicAdd(p.counters + first, 1u) == (unsigned)(last - first);
+                if (last_sh) p.counters[first] = 0;
+            }
+            __syncthreads();
+            if (last_sh) {
+                __threadfence();
+                const long long step = 2ll * p.chunk * (hd + 2);          // from a CTA's slot to the next one's
+                const float* p0 = p.partial + (2ll * first + 1) * p.chunk * (hd + 2);
+                const float* p1 = p.partial + (2ll * first) * p.chunk * (hd + 2);      // + c * step for the others
+                for (int i = tid; i < heads * hd; i += FL_THREADS) {
+                    const int h = i / hd, d = i - h * hd;
+                    const int at = h * (hd + 2);
+                    float M = __ldcg(p0 + at);
+                    for (int c = 1; c <= last - first; c++) M = fmaxf(M, __ldcg(p1 + c * step + at));
+                    const float ref = M == -INFINITY ? 0.f : M;
+                    float w = exp2f(__ldcg(p0 + at) - ref);
+                    float L = __ldcg(p0 + at + 1) * w, x = __ldcg(p0 + at + 2 + d) * w;
+                    for (int c = 1; c <= last - first; c++) {
+                        const float* q1 = p1 + c * step + at;
+                        w = exp2f(__ldcg(q1) - ref);
+                        L += __ldcg(q1 + 1) * w;
+                        x += __ldcg(q1 + 2 + d) * w;
+                    }
+                    a.out[seg_b * a.o_row + (long long)(h0 + h) * hd + d] = __float2half_rn(L > 0.f ? x / L : 0.f);
+                    if (d == 0 && a.lse) a.lse[(long long)seg_b * a.n_heads + h0 + h] = L > 0.f ? (M + log2f(L)) * 0.69314718055994531f : -INFINITY;
+                }
+            }
+        }
+        (void)seg_hg;
+        __syncthreads();
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+}
+
+template <int HDP, int NT>
+int launch_flash(const FlashLaunch& p, cudaStream_t st) {
+    using F = FlashShape<HDP, NT>;
+    static PerDeviceOnce once;
+    if (once.needed()) TL_CUDA(cudaFuncSetAttribute(k_paged_attn<HDP, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::SMEM));
+    const int grid = (sm_count() < FL_MAX_SMS ? sm_count() : FL_MAX_SMS) * F::CTAS;
+    return launch_pdl(k_paged_attn<HDP, NT>, grid, FL_THREADS, F::SMEM, st, true, p);
+}
+
+// query heads of a head group: as few groups as 16 columns allow (8 at 256 elements a head, where 16 would not fit the
+// registers), of even size
+int flash_chunk(int group, int head_dim) {
+    const int most = head_dim > 128 ? 8 : 16;
+    const int chunks = (group + most - 1) / most;
+    return (group + chunks - 1) / chunks;
+}
+
 }  // namespace
 
-size_t paged_attn_workspace_bytes(int, int, int) { return 0; }
+size_t paged_attn_workspace_bytes(int n_heads, int n_kv_heads, int head_dim) {
+    const int ctas = FL_MAX_SMS * (head_dim <= 64 ? FlashShape<64, 1>::CTAS : (head_dim <= 128 ? FlashShape<128, 1>::CTAS : FlashShape<256, 1>::CTAS));
+    return 4096 + 2 * (size_t)ctas * flash_chunk(n_heads / n_kv_heads, head_dim) * (head_dim + 2) * 4;
+}
 
 int launch_paged_attn(const PagedView& c, const PagedAttnArgs& a, cudaStream_t st) {
     if (a.batch == 0) return TL_OK;
@@ -112,7 +560,19 @@ int launch_paged_attn(const PagedView& c, const PagedAttnArgs& a, cudaStream_t s
     p.q = a.q; p.out = a.out; p.lse = a.lse; p.q_row = a.q_row; p.o_row = a.o_row;
     p.batch = a.batch; p.n_heads = a.n_heads; p.group = a.n_heads / c.n_kv_heads; p.scale = a.scale;
     p.status = device_status_word();
-    return launch_pdl(k_paged_attn_any, dim3(a.n_heads, a.batch), ANY_WARPS * 32, 0, st, true, p);
+    const bool fast = c.aligned16() && (reinterpret_cast<uintptr_t>(a.q) & 3) == 0 && a.q_row % 2 == 0;
+    if (!fast) return launch_pdl(k_paged_attn_any, dim3(a.n_heads, a.batch), ANY_WARPS * 32, 0, st, true, p);
+    FlashLaunch f{};
+    f.a = p;
+    f.chunk = flash_chunk(p.group, p.head_dim);
+    f.chunks = (p.group + f.chunk - 1) / f.chunk;
+    f.groups = p.n_kv * f.chunks;
+    f.scale_log2 = a.scale * 1.4426950408889634f;
+    f.counters = static_cast<unsigned int*>(a.work);
+    f.partial = reinterpret_cast<float*>(static_cast<char*>(a.work) + 4096);
+    if (p.head_dim <= 64) return f.chunk <= 8 ? launch_flash<64, 1>(f, st) : launch_flash<64, 2>(f, st);
+    if (p.head_dim <= 128) return f.chunk <= 8 ? launch_flash<128, 1>(f, st) : launch_flash<128, 2>(f, st);
+    return launch_flash<256, 1>(f, st);
 }
 
 }  // namespace tlb
