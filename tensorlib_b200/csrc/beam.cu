@@ -103,6 +103,7 @@ struct SelStat { double sum; float max; float pad; };
 struct SelLaunch {
     BeamArgs a;
     int splits, chunk;                            // chunks of a row, logits of a chunk (a multiple of 8)
+    int groups;                                   // the power of two from 8 to 128 at or above k
     unsigned int* counters; SelStat* stats; unsigned int* keys;     // [batch], [row][split], [row][split][k]
 };
 
@@ -129,10 +130,11 @@ __device__ __forceinline__ bool dead_row(const BeamArgs& a, int row) {
 
 // keys: (ord16 of the logit) << 16 | 0xffff - index in the chunk: unique, larger = earlier in the order
 template <int VPT>
-__global__ void __launch_bounds__(SEL_THREADS) k_beam_select(SelLaunch p) {
+__global__ void __launch_bounds__(SEL_THREADS, VPT <= 2 ? 6 : (VPT == 4 ? 4 : (VPT == 8 ? 2 : 1))) k_beam_select(SelLaunch p) {
     extern __shared__ unsigned char dyn[];        // the join's candidates
     __shared__ unsigned list[SEL_CAP];
-    __shared__ float red_f[SEL_THREADS / 32];
+    __shared__ __align__(16) unsigned short tops[SEL_THREADS];
+    __shared__ int red_i[SEL_THREADS / 32];
     __shared__ double red_d[SEL_THREADS / 32];
     __shared__ int count_sh, last_sh;
     const BeamArgs& a = p.a;
@@ -187,15 +189,25 @@ __global__ void __launch_bounds__(SEL_THREADS) k_beam_select(SelLaunch p) {
                 if (e + 2 * i + 1 >= n) v[j][i] |= NONE << 16;
             }
         }
-        // 2: maximum and sum
-        const float my_max = fmaxf(__low2float(mx), __high2float(mx));
-        float M = warp_max(my_max);
-        if (lane == 0) red_f[warp] = M;
+        // 2: the maximum, and a border that at least k values reach: the threads form `groups` >= k groups (by their index modulo
+        // that number, so none is empty where as many threads hold values), and the least of the groups' maxima is one. About
+        // k ln k values reach it. Fewer threads than groups: the border is below every value, and they hold less than SEL_CAP.
+        unsigned mine = tid * 8 < n ? ord16(__half_as_ushort(__hmax(__low2half(mx), __high2half(mx)))) : 0u;
+        for (int o = 16; o >= p.groups; o >>= 1) mine = max(mine, __shfl_xor_sync(0xffffffffu, mine, o));
+        tops[tid] = (unsigned short)mine;
         if (tid == 0) count_sh = 0;
         __syncthreads();
-        M = red_f[0];
+        unsigned e[8];
 #pragma unroll
-        for (int w = 1; w < SEL_THREADS / 32; w++) M = fmaxf(M, red_f[w]);
+        for (int i = 0; i < 8; i++) e[i] = tops[i * 32 + lane];
+        unsigned g4[4], border;
+#pragma unroll
+        for (int i = 0; i < 4; i++) g4[i] = max(e[i], e[i + 4]);                    // threads equal modulo 128
+        if (p.groups == 128) border = min(min(g4[0], g4[1]), min(g4[2], g4[3]));
+        else border = p.groups == 64 ? min(max(g4[0], g4[2]), max(g4[1], g4[3])) : max(max(g4[0], g4[2]), max(g4[1], g4[3]));
+        border = __reduce_min_sync(0xffffffffu, border);
+        const float M = ord16_value(__reduce_max_sync(0xffffffffu, max(max(g4[0], g4[2]), max(g4[1], g4[3]))));
+        // 3: the sum
         double sum = 0.0;
         if (M > -INFINITY) {
             constexpr float L2E = 1.4426950408889634f;
@@ -214,57 +226,61 @@ __global__ void __launch_bounds__(SEL_THREADS) k_beam_select(SelLaunch p) {
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         if (lane == 0) red_d[warp] = sum;
-        // 3: the k-th largest of the threads' maxima, bit by bit
-        const unsigned mine = tid * 8 < n ? ord16(__half_as_ushort(__float2half_rn(my_max))) : 0u;
-        unsigned border = 0;
+        // 4: what reaches the border
+        const int want = min(a.k, n);
+        {
+            // compared in pairs; a border below every value lets all pass (NONE is a NaN and never does)
+            const __half2 edge = __half2half2(__float2half_rn(border <= 0x3ffu ? -INFINITY : ord16_value(border)));
 #pragma unroll
-        for (int bit = 15; bit >= 0; bit--) {
-            const unsigned c = border | 1u << bit;
-            if (__syncthreads_count(mine >= c) >= a.k) border = c;
+            for (int j = 0; j < VPT; j++) {
+                unsigned hit[4], any = 0;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    hit[i] = __hge2_mask(*reinterpret_cast<__half2*>(&v[j][i]), edge);
+                    any |= hit[i];
+                }
+                if (any) {
+#pragma unroll
+                    for (int i = 0; i < 8; i++)
+                        if (hit[i >> 1] >> (16 * (i & 1)) & 1u) {
+                            const int at = atomicAdd(&count_sh, 1);
+                            const unsigned h = (v[j][i >> 1] >> (16 * (i & 1))) & 0xffffu;
+                            if (at < SEL_CAP) list[at] = ord16(h) << 16 | (0xffffu - (unsigned)((tid + j * SEL_THREADS) * 8 + i));
+                        }
+                }
+            }
         }
+        __syncthreads();
+        int found = count_sh;
         if (tid == 0) {
             double S = 0.0;
 #pragma unroll
             for (int w = 0; w < SEL_THREADS / 32; w++) S += red_d[w];
             p.stats[(long long)row * p.splits + split] = SelStat{S, M, 0.f};
         }
-        // 4: what reaches it
-        auto each = [&](auto&& f) {
-#pragma unroll
-            for (int j = 0; j < VPT; j++)
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const unsigned h = (v[j][i >> 1] >> (16 * (i & 1))) & 0xffffu;
-                    if (h != NONE) f(ord16(h) << 16 | (0xffffu - (unsigned)((tid + j * SEL_THREADS) * 8 + i)));
-                }
-        };
-        unsigned least = border << 16;
-        const int want = min(a.k, n);
-        {
-            int c = 0;
-            if (mine >= border) each([&](unsigned key) { c += key >= least; });
-            const int at = c ? atomicAdd(&count_sh, c) : 0;
-            if (c && at + c <= SEL_CAP) {
-                int q = at;
-                each([&](unsigned key) { if (key >= least) list[q++] = key; });
-            }
-        }
-        __syncthreads();
-        int found = count_sh;
         if (found > SEL_CAP) {                    // many equal ones: the exact border among the unique keys
+            auto each = [&](auto&& f) {
+#pragma unroll
+                for (int j = 0; j < VPT; j++)
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const unsigned h = (v[j][i >> 1] >> (16 * (i & 1))) & 0xffffu;
+                        if (h != NONE) f(ord16(h) << 16 | (0xffffu - (unsigned)((tid + j * SEL_THREADS) * 8 + i)));
+                    }
+            };
+            unsigned least = 0;
             for (int bit = 31; bit >= 0; bit--) {
-                const unsigned c = (bit == 31 ? 0u : least) | 1u << bit;
-                if (bit == 31) least = 0;
+                const unsigned c = least | 1u << bit;
                 int have = 0;
                 each([&](unsigned key) { have += key >= c; });
 #pragma unroll
                 for (int o = 16; o > 0; o >>= 1) have += __shfl_xor_sync(0xffffffffu, have, o);
                 __syncthreads();
-                if (lane == 0) red_f[warp] = __int_as_float(have);
+                if (lane == 0) red_i[warp] = have;
                 __syncthreads();
                 int all = 0;
 #pragma unroll
-                for (int w = 0; w < SEL_THREADS / 32; w++) all += __float_as_int(red_f[w]);
+                for (int w = 0; w < SEL_THREADS / 32; w++) all += red_i[w];
                 if (all >= want) least = c;
             }
             if (tid == 0) count_sh = 0;
@@ -278,41 +294,43 @@ __global__ void __launch_bounds__(SEL_THREADS) k_beam_select(SelLaunch p) {
         for (int i = tid; i < found; i += SEL_THREADS) {
             const unsigned key = list[i];
             int rank = 0;
+#pragma unroll 8
             for (int j = 0; j < found; j++) rank += list[j] > key;
             if (rank < a.k) out[rank] = key;
         }
     }
-    // 6: the last CTA of the entry joins
-    __threadfence();
+    // 6: the last CTA of the entry joins (the barrier before the fence makes it cover all threads' results)
     __syncthreads();
     if (tid == 0) {
+        __threadfence();
         last_sh = atomicAdd(p.counters + entry, 1u) == (unsigned)(a.beams * p.splits - 1);
         if (last_sh) p.counters[entry] = 0;
+        __threadfence();
+        count_sh = 0;
     }
     __syncthreads();
     if (!last_sh) return;
-    __threadfence();
     const int lists = a.beams * p.splits, total = lists * a.k;
     unsigned long long* val = reinterpret_cast<unsigned long long*>(dyn);           // [total]
-    double* lse = reinterpret_cast<double*>(val + total);                           // [beams]
+    unsigned long long* some_val = val + total;                                     // [total]
+    double* lse = reinterpret_cast<double*>(some_val + total);                      // [beams]
     unsigned* idx = reinterpret_cast<unsigned*>(lse + a.beams);                     // [total] flat index, ~0 where a list is short
-    unsigned* picked = idx + total;                                                 // [total]
-    for (int w = tid; w < a.beams; w += SEL_THREADS) {
+    unsigned* some_idx = idx + total;                                               // [total]
+    for (int w = warp; w < a.beams; w += SEL_THREADS / 32) {                        // a warp a row, a lane a chunk
         const int r = entry * a.beams + w;
         if (dead_row(a, r) || (a.finished && a.finished[r])) continue;
         const SelStat* s = p.stats + (long long)r * p.splits;
-        float M = -INFINITY;
-        for (int i = 0; i < p.splits; i++) M = fmaxf(M, __ldcg(&s[i].max));
-        double S = 0.0;
-        if (M > -INFINITY)
-            for (int i = 0; i < p.splits; i++) {
-                const float m = __ldcg(&s[i].max);
-                if (m > -INFINITY) S += __ldcg(&s[i].sum) * (m == M ? 1.0 : exp((double)m - (double)M));
-            }
-        lse[w] = M > -INFINITY ? (double)M + log(S) : 0.0;
+        const float m = lane < p.splits ? __ldcg(&s[lane].max) : -INFINITY;
+        double S = lane < p.splits ? __ldcg(&s[lane].sum) : 0.0;
+        const float M = warp_max(m);
+        S = m > -INFINITY ? S * (double)expf(m - M) : 0.0;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) S += __shfl_xor_sync(0xffffffffu, S, o);
+        if (lane == 0) lse[w] = M > -INFINITY ? (double)M + log(S) : 0.0;
     }
-    if (tid == 0) count_sh = 0;
     __syncthreads();
+    // the heads of the lists (as many of each as make k candidates): their k-th bounds the result from below
+    const int heads = (a.k + lists - 1) / lists, some = heads * lists;
     for (int i = tid; i < total; i += SEL_THREADS) {
         const int l = i / a.k, j = i - l * a.k, w = l / p.splits, s = l - w * p.splits, r = entry * a.beams + w;
         const double score = beam_score(a.scores[r]);
@@ -340,39 +358,52 @@ __global__ void __launch_bounds__(SEL_THREADS) k_beam_select(SelLaunch p) {
         }
         val[i] = o;
         idx[i] = at;
-    }
-    __syncthreads();
-    auto before = [&](int x, int y) { return val[x] > val[y] || (val[x] == val[y] && idx[x] < idx[y]); };
-    // the heads of the lists (as many as make k candidates): their k-th bounds the result from below
-    const int heads = (a.k + lists - 1) / lists, some = heads * lists;
-    __shared__ int border_sh;
-    if (tid == 0) border_sh = -1;
-    __syncthreads();
-    for (int i = tid; i < some; i += SEL_THREADS) {
-        const int x = i / heads * a.k + i % heads;
-        int rank = 0;
-        for (int j = 0; j < some; j++) {
-            const int y = j / heads * a.k + j % heads;
-            rank += y != x && before(y, x);
+        if (j < heads) {
+            some_val[l * heads + j] = o;
+            some_idx[l * heads + j] = at;
         }
-        if (rank == a.k - 1 && idx[x] != ~0u) border_sh = x;
     }
+    __shared__ unsigned long long border_val;
+    __shared__ unsigned border_idx;
+    if (tid == 0) { border_val = 0; border_idx = ~0u; }
     __syncthreads();
-    const int border = border_sh;
-    for (int i = tid; i < total; i += SEL_THREADS)
-        if (idx[i] != ~0u && (border < 0 || i == border || before(i, border))) picked[atomicAdd(&count_sh, 1)] = (unsigned)i;
+    auto rank_among = [&](unsigned long long o, unsigned at, int n) {
+        int rank = 0;
+#pragma unroll 8
+        for (int j = 0; j < n; j++) {
+            const unsigned long long y = some_val[j];
+            rank += (int)(y > o) | ((int)(y == o) & (int)(some_idx[j] < at));
+        }
+        return rank;
+    };
+    unsigned long long bv = 0;
+    unsigned bi = ~0u;
+    for (int i = tid; i < some; i += SEL_THREADS)
+        if (some_idx[i] != ~0u && rank_among(some_val[i], some_idx[i], some) == a.k - 1) { border_val = some_val[i]; border_idx = some_idx[i]; }
+    __syncthreads();
+    bv = border_val;
+    bi = border_idx;
+    for (int i = tid; i < total; i += SEL_THREADS) {
+        const unsigned long long o = val[i];
+        const unsigned at = idx[i];
+        if (at != ~0u && (o > bv || (o == bv && at <= bi))) {
+            const int q = atomicAdd(&count_sh, 1);
+            some_val[q] = o;
+            some_idx[q] = at;
+        }
+    }
     __syncthreads();
     const int n = count_sh;
     for (int i = tid; i < n; i += SEL_THREADS) {
-        const int x = (int)picked[i];
-        int rank = 0;
-        for (int j = 0; j < n; j++) rank += before((int)picked[j], x);
+        const unsigned long long o = some_val[i];
+        const unsigned x = some_idx[i];
+        const int rank = rank_among(o, x, n);
         if (rank < a.k) {
             const long long at = (long long)entry * a.k + rank;
-            const unsigned w = idx[x] / (unsigned)a.vocab;
-            a.out_scores[at] = (float)ord64_value(val[x]);
+            const unsigned w = x / (unsigned)a.vocab;
+            a.out_scores[at] = (float)ord64_value(o);
             a.out_parents[at] = entry * a.beams + (int)w;
-            a.out_tokens[at] = (int)(idx[x] - w * (unsigned)a.vocab);
+            a.out_tokens[at] = (int)(x - w * (unsigned)a.vocab);
         }
     }
 }
@@ -394,7 +425,7 @@ int sel_chunk(int vocab, int splits) { return ((vocab + splits - 1) / splits + 7
 template <int VPT>
 int launch_sel(const SelLaunch& p, size_t smem, cudaStream_t st) {
     static PerDeviceOnce once;
-    if (once.needed()) TL_CUDA(cudaFuncSetAttribute(k_beam_select<VPT>, cudaFuncAttributeMaxDynamicSharedMemorySize, SEL_MAX_MERGE * 16 + 1024 + 64));
+    if (once.needed()) TL_CUDA(cudaFuncSetAttribute(k_beam_select<VPT>, cudaFuncAttributeMaxDynamicSharedMemorySize, SEL_MAX_MERGE * 24 + 128 * 8));
     return launch_pdl(k_beam_select<VPT>, p.a.batch * p.a.beams * p.splits, SEL_THREADS, smem, st, true, p);
 }
 
@@ -414,12 +445,14 @@ int launch_beam_select(const BeamArgs& a, cudaStream_t st) {
     if (p.splits == 0 || (long long)a.batch * a.beams * p.splits >= (1ll << 31))
         return launch_pdl(k_beam_any, a.batch, BEAM_THREADS, (size_t)a.beams * 8, st, true, a);
     p.chunk = sel_chunk(a.vocab, p.splits);
+    p.groups = 8;
+    while (p.groups < a.k) p.groups *= 2;
     char* w = static_cast<char*>(a.work);
     const size_t lists = (size_t)a.batch * a.beams * p.splits;
     p.counters = reinterpret_cast<unsigned int*>(w);
     p.stats = reinterpret_cast<SelStat*>(w + ((size_t)a.batch * 4 + 15) / 16 * 16);
     p.keys = reinterpret_cast<unsigned int*>(p.stats + lists);
-    const size_t total = (size_t)a.beams * p.splits * a.k, smem = total * 16 + (size_t)a.beams * 8;
+    const size_t total = (size_t)a.beams * p.splits * a.k, smem = total * 24 + (size_t)a.beams * 8;
     const int vecs = (p.chunk + SEL_THREADS * 8 - 1) / (SEL_THREADS * 8);
     if (vecs <= 1) return launch_sel<1>(p, smem, st);
     if (vecs <= 2) return launch_sel<2>(p, smem, st);
