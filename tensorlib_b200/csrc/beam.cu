@@ -86,16 +86,17 @@ __global__ void __launch_bounds__(BEAM_THREADS) k_beam_any(BeamArgs a) {
 
 
 // ---- one pass over the logits ----------------------------------------------------------------------------------------
-// A CTA holds a chunk of one row in registers: its maximum and its sum of exponentials (32-bit exponentials, 64-bit sums),
-// and the k best of the chunk under the order (logit descending, index ascending). The K-th largest of the threads' maxima
-// bounds the K-th largest logit from below, so what reaches it is a short list, ranked by counting; only where that list is
-// long (many equal or masked logits) is the exact border searched. The last CTA of a batch entry joins: the rows' log-sums,
-// the candidates' values in 64 bits, and the same bound-and-rank over the sorted lists.
+// A CTA streams a chunk of one row through registers, a window of W vectors a thread at a time, the next window's loads under
+// way: the maximum and sum of exponentials (32-bit exponentials, 64-bit sums), and the k best of the chunk under the order
+// (logit descending, index ascending). The first window gives a border that at least k values reach; what reaches it goes on
+// a list in shared memory, cut back to its k best when it grows long. The last CTA of a batch entry joins: the rows'
+// log-sums, the candidates' values in 64 bits, and a border and ranks over the sorted lists.
 //
 // Bound: HBM with many rows (each logit is read once); with few rows the chain load -> maximum -> sum -> list -> join.
 constexpr int SEL_THREADS = 256;
-constexpr int SEL_CAP = 1024;                     // candidates of a chunk that are ranked by counting
-constexpr int SEL_MAX_SPLITS = 16;
+constexpr int SEL_LONG = 1024;                    // a list longer than this is cut back
+constexpr int SEL_MAX_SPLITS = 32;                // a lane each in the join
+constexpr int SEL_MAX_CHUNK = 65536;              // indices in a chunk have 16 bits
 constexpr int SEL_MAX_MERGE = 8192;               // candidates that one CTA joins
 
 struct SelStat { double sum; float max; float pad; };
@@ -123,18 +124,38 @@ __device__ __forceinline__ unsigned long long ord64(double v) {
 __device__ __forceinline__ double ord64_value(unsigned long long o) {
     return __longlong_as_double((long long)(o >> 63 ? o & ~(1ull << 63) : ~o));
 }
+// two 32-bit operations in one instruction
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 c;
+    asm("{.reg .b64 x, y, z; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %5}; add.rn.f32x2 z, x, y; mov.b64 {%0, %1}, z;}"
+        : "=f"(c.x), "=f"(c.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return c;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 c;
+    asm("{.reg .b64 x, y, z; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %5}; mul.rn.f32x2 z, x, y; mov.b64 {%0, %1}, z;}"
+        : "=f"(c.x), "=f"(c.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return c;
+}
+// 2^x to 2^-22, results below the normal range as 0
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 __device__ __forceinline__ bool dead_row(const BeamArgs& a, int row) {
     const float s = a.scores[row];
     return !(s > -INFINITY);
 }
 
 // keys: (ord16 of the logit) << 16 | 0xffff - index in the chunk: unique, larger = earlier in the order
-template <int VPT>
-__global__ void __launch_bounds__(SEL_THREADS, VPT <= 2 ? 6 : (VPT == 4 ? 4 : (VPT == 8 ? 2 : 1))) k_beam_select(SelLaunch p) {
-    extern __shared__ unsigned char dyn[];        // the join's candidates
-    __shared__ unsigned list[SEL_CAP];
+template <int W>
+__global__ void __launch_bounds__(SEL_THREADS, 4) k_beam_select(SelLaunch p) {
+    extern __shared__ __align__(16) unsigned char dyn[];         // the list; later the join's candidates
     __shared__ __align__(16) unsigned short tops[SEL_THREADS];
+    __shared__ unsigned kept[128];
     __shared__ int red_i[SEL_THREADS / 32];
+    __shared__ float red_f[SEL_THREADS / 32];
     __shared__ double red_d[SEL_THREADS / 32];
     __shared__ int count_sh, last_sh;
     const BeamArgs& a = p.a;
@@ -143,156 +164,241 @@ __global__ void __launch_bounds__(SEL_THREADS, VPT <= 2 ? 6 : (VPT == 4 ? 4 : (V
     pdl_launch_dependents();
     pdl_wait();
     if (!dead_row(a, row) && !(a.finished && a.finished[row])) {
-        // 1: the chunk into registers. A thread's values go by their index in the chunk, not by where the row happens to start,
-        // so equal rows give equal sums to the last bit: rows off the 16-byte grid take each vector from the two aligned ones
-        // that it lies in (which hold at least one value of the row each, so nothing beyond its 16-byte neighbours is touched).
+        constexpr int SPAN = SEL_THREADS * 8 * W;
+        constexpr float L2E = 1.4426950408889634f;
+        unsigned* list = reinterpret_cast<unsigned*>(dyn);       // [SPAN + SEL_LONG]: a window's values always fit
         const int first = split * p.chunk, n = min(p.chunk, a.vocab - first);
         const __half* x = a.logits + row * a.pitch + first;
         const int skew = (int)((reinterpret_cast<uintptr_t>(x) & 15) >> 1);
         const uint4* xv = reinterpret_cast<const uint4*>(x - skew);
-        // values cleaned (NaN -> -inf, +inf -> 65504, -0 -> +0); outside: bit pattern NONE, a NaN that cleaning never leaves
-        constexpr unsigned NONE = 0xffffu;
-        unsigned v[VPT][4];
-        const __half2 ninf = __half2half2(__ushort_as_half(0xfc00)), top = __half2half2(__ushort_as_half(0x7bff)), zero = __half2half2(__ushort_as_half(0));
-        __half2 mx = ninf;
+        // cut the list back to its k best (it holds more): the k-th largest of the unique keys, bit by bit
+        unsigned border = 0;
+        auto shrink = [&](int have) {
+            unsigned least = 0;
+            for (int bit = 31; bit >= 0; bit--) {
+                const unsigned c = least | 1u << bit;
+                int reach = 0;
+                for (int i = tid; i < have; i += SEL_THREADS) reach += list[i] >= c;
+                reach = __reduce_add_sync(0xffffffffu, reach);
+                __syncthreads();
+                if (lane == 0) red_i[warp] = reach;
+                __syncthreads();
+                int all = 0;
 #pragma unroll
-        for (int j = 0; j < VPT; j++) {
-            const int e = (tid + j * SEL_THREADS) * 8;                              // chunk index of the vector's first value
-            uint4 raw = make_uint4(~0u, ~0u, ~0u, ~0u);
-            if (e < n) raw = __ldcs(xv + tid + j * SEL_THREADS);
-            if (skew) {
-                uint4 hi = make_uint4(~0u, ~0u, ~0u, ~0u);
-                if (e + 8 - skew < n) hi = __ldcs(xv + tid + j * SEL_THREADS + 1);
-                unsigned w[8] = {raw.x, raw.y, raw.z, raw.w, hi.x, hi.y, hi.z, hi.w};
-                if (skew & 4) {
-#pragma unroll
-                    for (int i = 0; i < 6; i++) w[i] = w[i + 2];
-                }
-                if (skew & 2) {
-#pragma unroll
-                    for (int i = 0; i < 5; i++) w[i] = w[i + 1];
-                }
-                const unsigned odd = (skew & 1) * 16;
-                raw = make_uint4(__funnelshift_r(w[0], w[1], odd), __funnelshift_r(w[1], w[2], odd), __funnelshift_r(w[2], w[3], odd),
-                                 __funnelshift_r(w[3], w[4], odd));
+                for (int w = 0; w < SEL_THREADS / 32; w++) all += red_i[w];
+                if (all >= a.k) least = c;
             }
-            v[j][0] = raw.x; v[j][1] = raw.y; v[j][2] = raw.z; v[j][3] = raw.w;
+            if (tid == 0) count_sh = 0;
+            __syncthreads();
+            for (int i = tid; i < have; i += SEL_THREADS)
+                if (list[i] >= least) kept[atomicAdd(&count_sh, 1)] = list[i];
+            __syncthreads();
+            if (tid < a.k) list[tid] = kept[tid];
+            border = max(border, least >> 16);
+            __syncthreads();
+        };
+        // A thread's values go by their index in the chunk, not by where the row happens to start, so equal rows give equal
+        // sums to the last bit: rows off the 16-byte grid take each vector from the two aligned ones that it lies in (each
+        // holds at least one value of the row, so nothing beyond its 16-byte neighbours is touched).
+        auto index_of = [&](int w, int j) { return (w * W + j) * SEL_THREADS + tid; };     // in vectors
+        uint4 next[W];
+        auto fetch = [&](int w) {
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                if (e + 2 * i >= n) v[j][i] = 0xfc00fc00u;
-                else if (e + 2 * i + 1 >= n) v[j][i] = (v[j][i] & 0xffffu) | 0xfc000000u;
-                __half2 y = *reinterpret_cast<__half2*>(&v[j][i]);
-                y = __hadd2(__hmin2(__hmax2(y, ninf), top), zero);
-                mx = __hmax2(mx, y);
-                v[j][i] = *reinterpret_cast<unsigned*>(&y);
-                if (e + 2 * i >= n) v[j][i] |= NONE;
-                if (e + 2 * i + 1 >= n) v[j][i] |= NONE << 16;
+            for (int j = 0; j < W; j++) {
+                const int i = index_of(w, j);
+                if (i * 8 < n) next[j] = __ldcs(xv + i);
             }
-        }
-        // 2: the maximum, and a border that at least k values reach: the threads form `groups` >= k groups (by their index modulo
-        // that number, so none is empty where as many threads hold values), and the least of the groups' maxima is one. About
-        // k ln k values reach it. Fewer threads than groups: the border is below every value, and they hold less than SEL_CAP.
-        unsigned mine = tid * 8 < n ? ord16(__half_as_ushort(__hmax(__low2half(mx), __high2half(mx)))) : 0u;
-        for (int o = 16; o >= p.groups; o >>= 1) mine = max(mine, __shfl_xor_sync(0xffffffffu, mine, o));
-        tops[tid] = (unsigned short)mine;
-        if (tid == 0) count_sh = 0;
-        __syncthreads();
-        unsigned e[8];
+        };
+        if (skew == 0) fetch(0);
+        const int windows = (n + SPAN - 1) / SPAN;
+        const __half2 ninf = __half2half2(__ushort_as_half(0xfc00)), top = __half2half2(__ushort_as_half(0x7bff));
+        // The border: a value that at least k values seen so far reach. The threads form `groups` >= k groups (by their index
+        // modulo that number, so none is empty where as many threads hold values); the least of the groups' maxima is one, and
+        // about k ln k values reach it. Fewer threads than groups: it stays below every value. Also the largest value.
+        unsigned best = 0;                        // largest value of this thread so far, as ord16; 0: it holds none
+        auto publish = [&] {
+            unsigned mine = best;
+            for (int o = 16; o >= p.groups; o >>= 1) mine = max(mine, __shfl_xor_sync(0xffffffffu, mine, o));
+            tops[tid] = (unsigned short)mine;
+        };
+        auto raise_border = [&] {
+            unsigned g[8];
 #pragma unroll
-        for (int i = 0; i < 8; i++) e[i] = tops[i * 32 + lane];
-        unsigned g4[4], border;
+            for (int i = 0; i < 8; i++) g[i] = tops[i * 32 + lane];
 #pragma unroll
-        for (int i = 0; i < 4; i++) g4[i] = max(e[i], e[i + 4]);                    // threads equal modulo 128
-        if (p.groups == 128) border = min(min(g4[0], g4[1]), min(g4[2], g4[3]));
-        else border = p.groups == 64 ? min(max(g4[0], g4[2]), max(g4[1], g4[3])) : max(max(g4[0], g4[2]), max(g4[1], g4[3]));
-        border = __reduce_min_sync(0xffffffffu, border);
-        const float M = ord16_value(__reduce_max_sync(0xffffffffu, max(max(g4[0], g4[2]), max(g4[1], g4[3]))));
-        // 3: the sum
+            for (int i = 0; i < 4; i++) g[i] = max(g[i], g[i + 4]);                 // threads equal modulo 128
+            const unsigned all = max(max(g[0], g[2]), max(g[1], g[3]));
+            const unsigned b = p.groups == 128 ? min(min(g[0], g[1]), min(g[2], g[3])) : (p.groups == 64 ? min(max(g[0], g[2]), max(g[1], g[3])) : all);
+            border = max(border, __reduce_min_sync(0xffffffffu, b));
+            return __reduce_max_sync(0xffffffffu, all);
+        };
+        float ref = -INFINITY;                    // what this thread's sum is relative to
         double sum = 0.0;
-        if (M > -INFINITY) {
-            constexpr float L2E = 1.4426950408889634f;
+        for (int w = 0; w < windows; w++) {
+            // 1: the window; -inf outside the row
+            __half2 v[W][4];
 #pragma unroll
-            for (int j = 0; j < VPT; j++) {
-                float s8 = 0.f;
+            for (int j = 0; j < W; j++) {
+                const int i = index_of(w, j), e = i * 8;
+                uint4 raw = next[j];
+                if (skew) {
+                    unsigned q[8] = {};
+                    if (e < n) {
+                        const uint4 lo = __ldcs(xv + i);
+                        q[0] = lo.x; q[1] = lo.y; q[2] = lo.z; q[3] = lo.w;
+                    }
+                    if (e + 8 - skew < n) {
+                        const uint4 hi = __ldcs(xv + i + 1);
+                        q[4] = hi.x; q[5] = hi.y; q[6] = hi.z; q[7] = hi.w;
+                    }
+                    if (skew & 4) {
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const float2 f = __half22float2(*reinterpret_cast<__half2*>(&v[j][i]));
-                    // NONE is a NaN: fmaxf leaves -inf, whose exponential is 0
-                    s8 += exp2f((fmaxf(f.x, -INFINITY) - M) * L2E) + exp2f((fmaxf(f.y, -INFINITY) - M) * L2E);
+                        for (int r = 0; r < 6; r++) q[r] = q[r + 2];
+                    }
+                    if (skew & 2) {
+#pragma unroll
+                        for (int r = 0; r < 5; r++) q[r] = q[r + 1];
+                    }
+                    const unsigned odd = (skew & 1) * 16;
+                    raw = make_uint4(__funnelshift_r(q[0], q[1], odd), __funnelshift_r(q[1], q[2], odd), __funnelshift_r(q[2], q[3], odd),
+                                     __funnelshift_r(q[3], q[4], odd));
                 }
-                sum += (double)s8;
+                unsigned word[4] = {raw.x, raw.y, raw.z, raw.w};
+                if (e + 8 > n) {
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        if (e + 2 * r >= n) word[r] = 0xfc00fc00u;
+                        else if (e + 2 * r + 1 >= n) word[r] = (word[r] & 0xffffu) | 0xfc000000u;
+                    }
+                }
+#pragma unroll
+                for (int r = 0; r < 4; r++) v[j][r] = *reinterpret_cast<__half2*>(&word[r]);
+            }
+            if (skew == 0 && w + 1 < windows) fetch(w + 1);
+            // 2: its maximum (NaN loses against any value). +inf counts as 65504, NaN as -inf: cleaned where one turns up, +inf by
+            // the maximum, NaN by the sum.
+            auto clean = [&] {
+#pragma unroll
+                for (int j = 0; j < W; j++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) v[j][r] = __hmin2(__hmax2(v[j][r], ninf), top);
+            };
+            __half2 vm[W], mx = ninf;
+#pragma unroll
+            for (int j = 0; j < W; j++) {
+                vm[j] = __hmax2(__hmax2(v[j][0], v[j][1]), __hmax2(v[j][2], v[j][3]));
+                mx = __hmax2(mx, vm[j]);
+            }
+            float my_max = fmaxf(__low2float(mx), __high2float(mx));
+            if (my_max == INFINITY) {
+                clean();
+                my_max = 65504.f;
+            }
+            if ((w * W * SEL_THREADS + tid) * 8 < n) best = max(best, ord16(__half_as_ushort(__float2half_rn(my_max + 0.f))));
+            if (w == 0) {
+                publish();
+                if (tid == 0) count_sh = 0;
+                __syncthreads();
+                ref = ord16_value(raise_border());
+                if (windows > 1) __syncthreads();  // before tops is written again
+            } else if (my_max > ref) {
+                if (ref > -INFINITY) sum *= (double)exp2f((ref - my_max) * L2E);
+                ref = my_max;
+            }
+            // 3: the sum: exp2((x - ref) * log2 e), two at a time (x - ref is exact or nearly so, and small where it counts)
+            if (ref > -INFINITY) {
+                auto add_up = [&] {
+                    double total = 0.0;
+                    const float2 minus = make_float2(-ref, -ref), scale = make_float2(L2E, L2E);
+#pragma unroll
+                    for (int j = 0; j < W; j++) {
+                        float2 s2 = make_float2(0.f, 0.f);
+#pragma unroll
+                        for (int r = 0; r < 4; r++) {
+                            const float2 f = mul2(add2(__half22float2(v[j][r]), minus), scale);
+                            s2 = add2(s2, make_float2(ex2(f.x), ex2(f.y)));
+                        }
+                        total += (double)(s2.x + s2.y);
+                    }
+                    return total;
+                };
+                double part = add_up();
+                if (part != part) {
+                    clean();
+                    part = add_up();
+                }
+                sum += part;
+            }
+            // 4: what reaches the border goes on the list. Compared in pairs, first the maximum of a vector; a border below every
+            // value lets all pass, NaN too, which then counts.
+            const bool all_pass = border <= 0x3ffu;
+            if (all_pass) clean();
+            const __half2 edge = __half2half2(__float2half_rn(all_pass ? -INFINITY : ord16_value(border)));
+#pragma unroll
+            for (int j = 0; j < W; j++) {
+                if (all_pass || __hge2_mask(vm[j], edge)) {
+                    unsigned hits = 0;
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        const unsigned h = __hge2_mask(v[j][r], edge);
+                        hits |= ((h & 1u) | (h >> 30 & 2u)) << (2 * r);
+                    }
+                    const int e0 = index_of(w, j) * 8;
+                    if (e0 + 8 > n) hits &= e0 < n ? (1u << (n - e0)) - 1u : 0u;
+                    if (hits) {
+                        int at = atomicAdd(&count_sh, __popc(hits));
+#pragma unroll
+                        for (int i = 0; i < 8; i++)
+                            if (hits >> i & 1u) {
+                                const unsigned short h = __half_as_ushort(i & 1 ? __high2half(v[j][i >> 1]) : __low2half(v[j][i >> 1]));
+                                list[at++] = ord16(h == 0x8000u ? 0u : h) << 16 | (0xffffu - (unsigned)(e0 + i));
+                            }
+                    }
+                }
+            }
+            if (w + 1 < windows) {
+                publish();
+                __syncthreads();
+                const int have = count_sh;
+                raise_border();
+                __syncthreads();
+                if (have > SEL_LONG) shrink(have);
             }
         }
+        // 5: the chunk's statistics and its k best, in order
+        const float M = [&] {
+            const float m = warp_max(ref);
+            if (lane == 0) red_f[warp] = m;
+            __syncthreads();
+            float all = red_f[0];
+#pragma unroll
+            for (int w = 1; w < SEL_THREADS / 32; w++) all = fmaxf(all, red_f[w]);
+            return all;
+        }();
+        if (ref > -INFINITY) sum *= (double)exp2f((ref - M) * L2E);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         if (lane == 0) red_d[warp] = sum;
-        // 4: what reaches the border
-        const int want = min(a.k, n);
-        {
-            // compared in pairs; a border below every value lets all pass (NONE is a NaN and never does)
-            const __half2 edge = __half2half2(__float2half_rn(border <= 0x3ffu ? -INFINITY : ord16_value(border)));
-#pragma unroll
-            for (int j = 0; j < VPT; j++) {
-                unsigned hit[4], any = 0;
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    hit[i] = __hge2_mask(*reinterpret_cast<__half2*>(&v[j][i]), edge);
-                    any |= hit[i];
-                }
-                if (any) {
-#pragma unroll
-                    for (int i = 0; i < 8; i++)
-                        if (hit[i >> 1] >> (16 * (i & 1)) & 1u) {
-                            const int at = atomicAdd(&count_sh, 1);
-                            const unsigned h = (v[j][i >> 1] >> (16 * (i & 1))) & 0xffffu;
-                            if (at < SEL_CAP) list[at] = ord16(h) << 16 | (0xffffu - (unsigned)((tid + j * SEL_THREADS) * 8 + i));
-                        }
-                }
-            }
-        }
-        __syncthreads();
+        publish();
         int found = count_sh;
+        __syncthreads();
+        raise_border();
+        if (found > SEL_LONG) {
+            shrink(found);
+            found = a.k;
+        }
         if (tid == 0) {
             double S = 0.0;
 #pragma unroll
             for (int w = 0; w < SEL_THREADS / 32; w++) S += red_d[w];
             p.stats[(long long)row * p.splits + split] = SelStat{S, M, 0.f};
         }
-        if (found > SEL_CAP) {                    // many equal ones: the exact border among the unique keys
-            auto each = [&](auto&& f) {
-#pragma unroll
-                for (int j = 0; j < VPT; j++)
-#pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        const unsigned h = (v[j][i >> 1] >> (16 * (i & 1))) & 0xffffu;
-                        if (h != NONE) f(ord16(h) << 16 | (0xffffu - (unsigned)((tid + j * SEL_THREADS) * 8 + i)));
-                    }
-            };
-            unsigned least = 0;
-            for (int bit = 31; bit >= 0; bit--) {
-                const unsigned c = least | 1u << bit;
-                int have = 0;
-                each([&](unsigned key) { have += key >= c; });
-#pragma unroll
-                for (int o = 16; o > 0; o >>= 1) have += __shfl_xor_sync(0xffffffffu, have, o);
-                __syncthreads();
-                if (lane == 0) red_i[warp] = have;
-                __syncthreads();
-                int all = 0;
-#pragma unroll
-                for (int w = 0; w < SEL_THREADS / 32; w++) all += red_i[w];
-                if (all >= want) least = c;
-            }
-            if (tid == 0) count_sh = 0;
-            __syncthreads();
-            each([&](unsigned key) { if (key >= least) list[atomicAdd(&count_sh, 1)] = key; });
-            __syncthreads();
-            found = count_sh;
-        }
-        // 5: their ranks
+        // the border over the whole chunk, and the ranks of what reaches it
         unsigned* out = p.keys + ((long long)row * p.splits + split) * a.k;
+        const unsigned edge = border << 16;
         for (int i = tid; i < found; i += SEL_THREADS) {
             const unsigned key = list[i];
+            if (key < edge) continue;
             int rank = 0;
 #pragma unroll 8
             for (int j = 0; j < found; j++) rank += list[j] > key;
@@ -408,25 +514,26 @@ __global__ void __launch_bounds__(SEL_THREADS, VPT <= 2 ? 6 : (VPT == 4 ? 4 : (V
     }
 }
 
-// Chunks of a row: enough CTAs for the machine, at most SEL_MAX_SPLITS and what the join can hold; 0 = the plain kernel.
+// Chunks of a row: four CTAs an SM where the rows alone are fewer, but no chunk below one vector a thread, and no more
+// candidates than the join holds; 0 = the plain kernel.
 int sel_splits(int batch, int beams, int vocab, int k) {
-    const int widest = SEL_THREADS * 8 * 16;      // logits that fit the registers of a CTA
-    const int least = (vocab + widest - 1) / widest;
+    const int least = (int)(((long long)vocab + SEL_MAX_CHUNK - 1) / SEL_MAX_CHUNK);
     if (least > SEL_MAX_SPLITS || (long long)beams * least * k > SEL_MAX_MERGE) return 0;
-    long long want = (4 * 148 + (long long)batch * beams - 1) / ((long long)batch * beams);
-    const int light = (vocab + 8191) / 8192;      // four vectors a thread: several CTAs fit an SM
-    if (want < light) want = light;
-    want = want < SEL_MAX_SPLITS ? want : SEL_MAX_SPLITS;
-    while (want > least && (beams * want * k > 1024 || vocab / want < SEL_THREADS * 8)) want--;
+    const long long rows = (long long)batch * beams;
+    long long want = 4 * 148 / rows;
+    want = want < 16 ? want : 16;
+    while (want > least && (beams * want * k > 1024 || vocab / want < SEL_THREADS * 4)) want--;
     return (int)(want > least ? want : least);
 }
 int sel_chunk(int vocab, int splits) { return ((vocab + splits - 1) / splits + 7) / 8 * 8; }
 
-template <int VPT>
-int launch_sel(const SelLaunch& p, size_t smem, cudaStream_t st) {
+template <int W>
+int launch_sel(const SelLaunch& p, cudaStream_t st) {
+    const size_t total = (size_t)p.a.beams * p.splits * p.a.k, join = total * 24 + (size_t)p.a.beams * 8;
+    const size_t list = (SEL_THREADS * 8 * W + SEL_LONG) * 4, smem = list > join ? list : join;
     static PerDeviceOnce once;
-    if (once.needed()) TL_CUDA(cudaFuncSetAttribute(k_beam_select<VPT>, cudaFuncAttributeMaxDynamicSharedMemorySize, SEL_MAX_MERGE * 24 + 128 * 8));
-    return launch_pdl(k_beam_select<VPT>, p.a.batch * p.a.beams * p.splits, SEL_THREADS, smem, st, true, p);
+    if (once.needed()) TL_CUDA(cudaFuncSetAttribute(k_beam_select<W>, cudaFuncAttributeMaxDynamicSharedMemorySize, SEL_MAX_MERGE * 24 + 128 * 8));
+    return launch_pdl(k_beam_select<W>, p.a.batch * p.a.beams * p.splits, SEL_THREADS, smem, st, true, p);
 }
 
 }  // namespace
@@ -452,13 +559,8 @@ int launch_beam_select(const BeamArgs& a, cudaStream_t st) {
     p.counters = reinterpret_cast<unsigned int*>(w);
     p.stats = reinterpret_cast<SelStat*>(w + ((size_t)a.batch * 4 + 15) / 16 * 16);
     p.keys = reinterpret_cast<unsigned int*>(p.stats + lists);
-    const size_t total = (size_t)a.beams * p.splits * a.k, smem = total * 24 + (size_t)a.beams * 8;
-    const int vecs = (p.chunk + SEL_THREADS * 8 - 1) / (SEL_THREADS * 8);
-    if (vecs <= 1) return launch_sel<1>(p, smem, st);
-    if (vecs <= 2) return launch_sel<2>(p, smem, st);
-    if (vecs <= 4) return launch_sel<4>(p, smem, st);
-    if (vecs <= 8) return launch_sel<8>(p, smem, st);
-    return launch_sel<16>(p, smem, st);
+    // one vector a thread where that covers the chunk: the shortest chain; else four, loaded ahead
+    return p.chunk <= SEL_THREADS * 8 ? launch_sel<1>(p, st) : launch_sel<4>(p, st);
 }
 
 }  // namespace tlb
