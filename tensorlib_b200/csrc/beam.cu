@@ -88,13 +88,17 @@ __global__ void __launch_bounds__(BEAM_THREADS) k_beam_any(BeamArgs a) {
 // ---- one pass over the logits ----------------------------------------------------------------------------------------
 // A CTA streams a chunk of one row through registers, a window of W vectors a thread at a time, the next window's loads under
 // way: the maximum and sum of exponentials (32-bit exponentials, 64-bit sums), and the k best of the chunk under the order
-// (logit descending, index ascending). The first window gives a border that at least k values reach; what reaches it goes on
-// a list in shared memory, cut back to its k best when it grows long. The last CTA of a batch entry joins: the rows'
-// log-sums, the candidates' values in 64 bits, and a border and ranks over the sorted lists.
+// (logit descending, index ascending). The first window gives a border that at least k values reach, later ones raise it;
+// vectors that reach it are set aside whole in shared memory (taking them apart at once, in diverged warps, cost as much as all
+// the rest), and what reaches the last border is ranked at the end. Many of them (equal or masked logits) are taken apart in
+// between and cut back to the k best. The last CTA of a batch entry joins: the rows' log-sums, the candidates' values in 64
+// bits, and a border and ranks over the sorted lists.
 //
 // Bound: HBM with many rows (each logit is read once); with few rows the chain load -> maximum -> sum -> list -> join.
 constexpr int SEL_THREADS = 256;
-constexpr int SEL_LONG = 1024;                    // a list longer than this is cut back
+constexpr int SEL_ASIDE = 256;                    // vectors set aside that wait for the end; more are taken apart
+constexpr int SEL_BATCH = SEL_THREADS / 2;        // vectors taken apart at a time, two threads each
+constexpr int SEL_LONG = 1024;                    // a list of values longer than this is cut back
 constexpr int SEL_MAX_SPLITS = 32;                // a lane each in the join
 constexpr int SEL_MAX_CHUNK = 65536;              // indices in a chunk have 16 bits
 constexpr int SEL_MAX_MERGE = 8192;               // candidates that one CTA joins
@@ -157,7 +161,7 @@ __global__ void __launch_bounds__(SEL_THREADS, 4) k_beam_select(SelLaunch p) {
     __shared__ int red_i[SEL_THREADS / 32];
     __shared__ float red_f[SEL_THREADS / 32];
     __shared__ double red_d[SEL_THREADS / 32];
-    __shared__ int count_sh, last_sh;
+    __shared__ int count_sh, listed_sh, last_sh;
     const BeamArgs& a = p.a;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int row = blockIdx.x / p.splits, split = blockIdx.x - row * p.splits, entry = row / a.beams;
@@ -166,7 +170,9 @@ __global__ void __launch_bounds__(SEL_THREADS, 4) k_beam_select(SelLaunch p) {
     if (!dead_row(a, row) && !(a.finished && a.finished[row])) {
         constexpr int SPAN = SEL_THREADS * 8 * W;
         constexpr float L2E = 1.4426950408889634f;
-        unsigned* list = reinterpret_cast<unsigned*>(dyn);       // [SPAN + SEL_LONG]: a window's values always fit
+        uint4* aside = reinterpret_cast<uint4*>(dyn);            // [W * SEL_THREADS + SEL_ASIDE]: a window's vectors always fit
+        unsigned* aside_at = reinterpret_cast<unsigned*>(aside + W * SEL_THREADS + SEL_ASIDE);
+        unsigned* list = aside_at + W * SEL_THREADS + SEL_ASIDE; // [SEL_LONG + 8 * SEL_BATCH]
         const int first = split * p.chunk, n = min(p.chunk, a.vocab - first);
         const __half* x = a.logits + row * a.pitch + first;
         const int skew = (int)((reinterpret_cast<uintptr_t>(x) & 15) >> 1);
@@ -188,14 +194,34 @@ __global__ void __launch_bounds__(SEL_THREADS, 4) k_beam_select(SelLaunch p) {
                 for (int w = 0; w < SEL_THREADS / 32; w++) all += red_i[w];
                 if (all >= a.k) least = c;
             }
-            if (tid == 0) count_sh = 0;
+            if (tid == 0) listed_sh = 0;
             __syncthreads();
             for (int i = tid; i < have; i += SEL_THREADS)
-                if (list[i] >= least) kept[atomicAdd(&count_sh, 1)] = list[i];
+                if (list[i] >= least) kept[atomicAdd(&listed_sh, 1)] = list[i];
             __syncthreads();
             if (tid < a.k) list[tid] = kept[tid];
             border = max(border, least >> 16);
             __syncthreads();
+        };
+        // take `have` vectors apart: what reaches the border goes on the list
+        auto take_apart = [&](int have) {
+            for (int i0 = 0; i0 < have; i0 += SEL_BATCH) {
+                const int i = i0 + (tid >> 1);
+                if (i < have) {
+                    const uint2 half = reinterpret_cast<const uint2*>(aside + i)[tid & 1];
+                    const unsigned e0 = aside_at[i] * 8 + (tid & 1) * 4;
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        const unsigned h = ((r < 2 ? half.x : half.y) >> (16 * (r & 1))) & 0xffffu;
+                        const unsigned o = (h & 0x7fffu) > 0x7c00u ? 0x3ffu : ord16(h == 0x8000u ? 0u : h);     // NaN is -inf, -0 is 0
+                        if (e0 + r < (unsigned)n && o >= border) list[atomicAdd(&listed_sh, 1)] = o << 16 | (0xffffu - (e0 + r));
+                    }
+                }
+                __syncthreads();
+                const int listed = listed_sh;
+                __syncthreads();
+                if (listed > SEL_LONG) shrink(listed);
+            }
         };
         // A thread's values go by their index in the chunk, not by where the row happens to start, so equal rows give equal
         // sums to the last bit: rows off the 16-byte grid take each vector from the two aligned ones that it lies in (each
@@ -297,7 +323,7 @@ __global__ void __launch_bounds__(SEL_THREADS, 4) k_beam_select(SelLaunch p) {
             if ((w * W * SEL_THREADS + tid) * 8 < n) best = max(best, ord16(__half_as_ushort(__float2half_rn(my_max + 0.f))));
             if (w == 0) {
                 publish();
-                if (tid == 0) count_sh = 0;
+                if (tid == 0) count_sh = listed_sh = 0;
                 __syncthreads();
                 ref = ord16_value(raise_border());
                 if (windows > 1) __syncthreads();  // before tops is written again
@@ -329,31 +355,16 @@ __global__ void __launch_bounds__(SEL_THREADS, 4) k_beam_select(SelLaunch p) {
                 }
                 sum += part;
             }
-            // 4: what reaches the border goes on the list. Compared in pairs, first the maximum of a vector; a border below every
-            // value lets all pass, NaN too, which then counts.
+            // 4: vectors that reach the border are set aside; a border below every value lets all pass
             const bool all_pass = border <= 0x3ffu;
-            if (all_pass) clean();
             const __half2 edge = __half2half2(__float2half_rn(all_pass ? -INFINITY : ord16_value(border)));
 #pragma unroll
             for (int j = 0; j < W; j++) {
-                if (all_pass || __hge2_mask(vm[j], edge)) {
-                    unsigned hits = 0;
-#pragma unroll
-                    for (int r = 0; r < 4; r++) {
-                        const unsigned h = __hge2_mask(v[j][r], edge);
-                        hits |= ((h & 1u) | (h >> 30 & 2u)) << (2 * r);
-                    }
-                    const int e0 = index_of(w, j) * 8;
-                    if (e0 + 8 > n) hits &= e0 < n ? (1u << (n - e0)) - 1u : 0u;
-                    if (hits) {
-                        int at = atomicAdd(&count_sh, __popc(hits));
-#pragma unroll
-                        for (int i = 0; i < 8; i++)
-                            if (hits >> i & 1u) {
-                                const unsigned short h = __half_as_ushort(i & 1 ? __high2half(v[j][i >> 1]) : __low2half(v[j][i >> 1]));
-                                list[at++] = ord16(h == 0x8000u ? 0u : h) << 16 | (0xffffu - (unsigned)(e0 + i));
-                            }
-                    }
+                const int i = index_of(w, j);
+                if ((all_pass || __hge2_mask(vm[j], edge)) && i * 8 < n) {
+                    const int at = atomicAdd(&count_sh, 1);
+                    aside[at] = *reinterpret_cast<const uint4*>(&v[j][0]);
+                    aside_at[at] = (unsigned)i;
                 }
             }
             if (w + 1 < windows) {
@@ -362,7 +373,11 @@ __global__ void __launch_bounds__(SEL_THREADS, 4) k_beam_select(SelLaunch p) {
                 const int have = count_sh;
                 raise_border();
                 __syncthreads();
-                if (have > SEL_LONG) shrink(have);
+                if (have > SEL_ASIDE) {
+                    take_apart(have);
+                    if (tid == 0) count_sh = 0;
+                    __syncthreads();
+                }
             }
         }
         // 5: the chunk's statistics and its k best, in order
@@ -380,22 +395,19 @@ __global__ void __launch_bounds__(SEL_THREADS, 4) k_beam_select(SelLaunch p) {
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         if (lane == 0) red_d[warp] = sum;
         publish();
-        int found = count_sh;
+        const int have = count_sh;
         __syncthreads();
-        raise_border();
-        if (found > SEL_LONG) {
-            shrink(found);
-            found = a.k;
-        }
+        raise_border();                           // over the whole chunk now
+        take_apart(have);
+        const int found = listed_sh;
         if (tid == 0) {
             double S = 0.0;
 #pragma unroll
             for (int w = 0; w < SEL_THREADS / 32; w++) S += red_d[w];
             p.stats[(long long)row * p.splits + split] = SelStat{S, M, 0.f};
         }
-        // the border over the whole chunk, and the ranks of what reaches it
         unsigned* out = p.keys + ((long long)row * p.splits + split) * a.k;
-        const unsigned edge = border << 16;
+        const unsigned edge = border << 16;       // values listed before the border rose
         for (int i = tid; i < found; i += SEL_THREADS) {
             const unsigned key = list[i];
             if (key < edge) continue;
@@ -530,7 +542,7 @@ int sel_chunk(int vocab, int splits) { return ((vocab + splits - 1) / splits + 7
 template <int W>
 int launch_sel(const SelLaunch& p, cudaStream_t st) {
     const size_t total = (size_t)p.a.beams * p.splits * p.a.k, join = total * 24 + (size_t)p.a.beams * 8;
-    const size_t list = (SEL_THREADS * 8 * W + SEL_LONG) * 4, smem = list > join ? list : join;
+    const size_t list = (size_t)(SEL_THREADS * W + SEL_ASIDE) * 20 + (SEL_LONG + 8 * SEL_BATCH) * 4, smem = list > join ? list : join;
     static PerDeviceOnce once;
     if (once.needed()) TL_CUDA(cudaFuncSetAttribute(k_beam_select<W>, cudaFuncAttributeMaxDynamicSharedMemorySize, SEL_MAX_MERGE * 24 + 128 * 8));
     return launch_pdl(k_beam_select<W>, p.a.batch * p.a.beams * p.splits, SEL_THREADS, smem, st, true, p);
