@@ -124,7 +124,8 @@ struct FlashLaunch {
     AttnLaunch a;
     int chunk, chunks, groups;                    // query heads of a head group, head groups a KV head, head groups in all
     float scale_log2;
-    unsigned int* counters; float* partial;       // workspace: [CTAs], [2 CTAs][chunk][head_dim + 2]
+    bool out8;                                    // out can be stored 8 bytes at a time
+    unsigned int* counters; float* partial;       // workspace: [CTAs], [2 CTAs] partial results
 };
 
 template <int HDP, int NT>
@@ -134,11 +135,12 @@ struct FlashShape {
     static constexpr int TILE_BYTES = FL_TILE * HDP * 2;
     static constexpr int RING = FL_WARPS * STAGES * 2 * TILE_BYTES;
     static constexpr int HEADS = 8 * NT;
-    // words between heads: + 4 makes the accumulator stores conflict-free, + 2 lets two CTAs of 16 heads fit an SM
-    static constexpr int PITCH = NT == 1 ? HDP + 4 : HDP + 2;
-    static constexpr int SLAB = HEADS * PITCH * 4;
-    static constexpr int SMEM = RING + 2 * SLAB + FL_WARPS * HEADS * 8 + FL_WARPS * STAGES * 4;
+    static constexpr int SMEM = RING + FL_WARPS * HEADS * 8 + FL_WARPS * STAGES * 4;
+    static_assert(HEADS * HDP * 4 <= 2 * TILE_BYTES, "a warp's sums go into one free stage of its ring");
 };
+
+// a partial result: [chunk][head_dim] sums, [chunk] (max, sum of weights), 16-byte aligned
+__host__ __device__ __forceinline__ long long flash_slot_floats(int chunk, int head_dim) { return ((long long)chunk * (head_dim + 2) + 3) / 4 * 4; }
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
@@ -185,11 +187,11 @@ template <int HDP, int NT>
 __global__ void __launch_bounds__(FL_THREADS, FlashShape<HDP, NT>::CTAS) k_paged_attn(FlashLaunch p) {
     using F = FlashShape<HDP, NT>;
     extern __shared__ __align__(128) unsigned char sm[];
-    float* slabs = reinterpret_cast<float*>(sm + F::RING);
-    float2* stats = reinterpret_cast<float2*>(sm + F::RING + 2 * F::SLAB);                                   // [warp][head]: max, sum
-    uint32_t* masks = reinterpret_cast<uint32_t*>(sm + F::RING + 2 * F::SLAB + FL_WARPS * F::HEADS * 8);     // [warp][stage]
+    float2* stats = reinterpret_cast<float2*>(sm + F::RING);                                 // [warp][head]: max, sum
+    uint32_t* masks = reinterpret_cast<uint32_t*>(sm + F::RING + FL_WARPS * F::HEADS * 8);   // [warp][stage]
     __shared__ unsigned long long scan_sh[FL_WARPS];
-    __shared__ unsigned long long start_sh[2];
+    __shared__ unsigned long long start_sh;
+    __shared__ int start_b, start_row, start_len;
     __shared__ int last_sh;
     const AttnLaunch& a = p.a;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, hd = a.head_dim;
@@ -218,27 +220,35 @@ __global__ void __launch_bounds__(FL_THREADS, FlashShape<HDP, NT>::CTAS) k_paged
         if (w < warp) before += scan_sh[w];
         total += scan_sh[w];
     }
+    // (counts of units that fit 32 bits, the ordinary case, are divided there: a 64-bit division takes a tenth of a microsecond)
     const unsigned long long U = total * p.groups;
-    const unsigned long long per = (U + gridDim.x - 1) / gridDim.x;
+    const unsigned long long per = U < (1ull << 31) ? ((unsigned)U + gridDim.x - 1) / gridDim.x : (U + gridDim.x - 1) / gridDim.x;
     const unsigned long long u0 = per * blockIdx.x, u1 = u0 + per < U ? u0 + per : U;
     // sequences with nothing to attend to
-    for (int b = blockIdx.x; b < a.batch; b += gridDim.x) {
-        int row;
-        if (row_tokens(a, b, row) == 0) {
-            for (int i = tid; i < a.n_heads * hd; i += FL_THREADS) a.out[b * a.o_row + i] = __float2half_rn(0.f);
-            if (a.lse)
-                for (int h = tid; h < a.n_heads; h += FL_THREADS) a.lse[(long long)b * a.n_heads + h] = -INFINITY;
+    auto empty_rows = [&] {
+        for (int b = blockIdx.x; b < a.batch; b += gridDim.x) {
+            int row;
+            if (row_tokens(a, b, row) == 0) {
+                for (int i = tid; i < a.n_heads * hd; i += FL_THREADS) a.out[b * a.o_row + i] = __float2half_rn(0.f);
+                if (a.lse)
+                    for (int h = tid; h < a.n_heads; h += FL_THREADS) a.lse[(long long)b * a.n_heads + h] = -INFINITY;
+            }
         }
+    };
+    if (u0 >= u1) {
+        empty_rows();
+        return;
     }
-    if (u0 >= u1) return;
     if (u0 >= before * p.groups && u0 < (before + mine) * p.groups) {      // one thread's run holds the start
         unsigned long long at = before;
         for (int b = b0; b < b1; b++) {
             int row;
-            const int n = units_of(row_tokens(a, b, row));
+            const int len = row_tokens(a, b, row), n = units_of(len);
             if (u0 < (at + n) * p.groups) {
-                start_sh[0] = (unsigned long long)b;
-                start_sh[1] = at;
+                start_sh = at;
+                start_b = b;
+                start_row = row;
+                start_len = len;
                 break;
             }
             at += n;
@@ -246,42 +256,44 @@ __global__ void __launch_bounds__(FL_THREADS, FlashShape<HDP, NT>::CTAS) k_paged
     }
     __syncthreads();
     Cursor cur;                                   // what is computed next
-    cur.b = (int)start_sh[0];
-    cur.len = row_tokens(a, cur.b, cur.row);
+    cur.b = start_b;
+    cur.row = start_row;
+    cur.len = start_len;
     cur.units = units_of(cur.len);
     {
-        const unsigned long long in = u0 - start_sh[1] * p.groups;
-        cur.hg = (int)(in / cur.units);
+        const unsigned long long in = u0 - start_sh * p.groups;
+        cur.hg = in < (1ull << 31) ? (int)((unsigned)in / (unsigned)cur.units) : (int)(in / cur.units);
         cur.i = (int)(in - (unsigned long long)cur.hg * cur.units);
     }
     cur.left = (long long)(u1 - u0);
     Cursor ahead = cur;                           // what is looked up next
 
     // 2: loads. lookup(): the page id of this lane's token (lanes 16.. repeat 0..15); issue(): the tile's rows.
-    int raw = 0, slot = -1, raw_hg = 0;
+    struct Look { int page, slot, kvh; };
     auto lookup = [&]() {
-        slot = -1;
+        Look k{0, -1, 0};
         if (ahead.left > 0) {
             const int tok = ahead.i * FL_UNIT + warp * FL_TILE + (lane & 15);
-            raw_hg = ahead.hg;
+            k.kvh = ahead.hg / p.chunks;
             if (tok < ahead.len) {
                 unsigned pg, s;
                 a.by_page.divmod((unsigned)tok, pg, s);
-                slot = (int)s;
-                raw = a.table[(long long)ahead.row * a.max_pages + pg];
+                k.slot = (int)s;
+                k.page = a.table[(long long)ahead.row * a.max_pages + pg];
             }
             advance(p, ahead);
         }
+        return k;
     };
     constexpr int CPR = HDP / 8;                  // 16-byte chunks a row
     constexpr int ROWS = 32 / CPR;                // rows an instruction
     const int chunk = lane % CPR;
     const bool in_row = chunk * 8 < hd;
     unsigned char* ring = sm + warp * F::STAGES * 2 * F::TILE_BYTES;
-    auto issue = [&](int stage) {
+    auto issue = [&](int stage, const Look& k) {
         long long off = -1;
-        if (slot >= 0) {
-            if ((unsigned)raw < (unsigned)a.n_pages) off = raw * a.page_stride + slot * a.token_stride + (long long)(raw_hg / p.chunks) * a.head_stride;
+        if (k.slot >= 0) {
+            if ((unsigned)k.page < (unsigned)a.n_pages) off = k.page * a.page_stride + k.slot * a.token_stride + k.kvh * a.head_stride;
             else atomicExch(a.status, TL_ERR_INVALID_ARGUMENT);
         }
         const uint32_t mask = __ballot_sync(0xffffffffu, off >= 0) & 0xffffu;
@@ -301,12 +313,16 @@ __global__ void __launch_bounds__(FL_THREADS, FlashShape<HDP, NT>::CTAS) k_paged
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
+    Look ahead_look;
+    {
+        Look first[F::STAGES - 1];                // their lookups are under way together
 #pragma unroll
-    for (int s = 0; s < F::STAGES - 1; s++) {
-        lookup();
-        issue(s);
+        for (int s = 0; s < F::STAGES - 1; s++) first[s] = lookup();
+        ahead_look = lookup();
+#pragma unroll
+        for (int s = 0; s < F::STAGES - 1; s++) issue(s, first[s]);
     }
-    lookup();
+    empty_rows();
 
     // 3: the range, segment by segment (one (sequence, head group) each)
     const int g = lane >> 2, t = lane & 3;        // fragment row and column pair
@@ -315,7 +331,7 @@ __global__ void __launch_bounds__(FL_THREADS, FlashShape<HDP, NT>::CTAS) k_paged
         const int kvh = cur.hg / p.chunks, h0 = kvh * a.group + (cur.hg - kvh * p.chunks) * p.chunk;
         const int heads = min(p.chunk, (kvh + 1) * a.group - h0);
         const long long seg_units = min((long long)(cur.units - cur.i), cur.left);
-        const int seg_b = cur.b, seg_hg = cur.hg, seg_i = cur.i, seg_n = cur.units;
+        const int seg_b = cur.b, seg_i = cur.i, seg_n = cur.units;
         uint32_t q[NT][HDP / 16][2];
 #pragma unroll
         for (int n = 0; n < NT; n++)
@@ -340,8 +356,8 @@ __global__ void __launch_bounds__(FL_THREADS, FlashShape<HDP, NT>::CTAS) k_paged
             const uint32_t mask = masks[warp * F::STAGES + stage];
             {
                 const int next = stage == 0 ? F::STAGES - 1 : stage - 1;       // the stage computed last
-                issue(next);
-                lookup();
+                issue(next, ahead_look);
+                ahead_look = lookup();
             }
             if (mask) {
                 const uint32_t ks_base = smem_addr(ring + stage * 2 * F::TILE_BYTES), vs_base = ks_base + F::TILE_BYTES;
@@ -414,113 +430,125 @@ __global__ void __launch_bounds__(FL_THREADS, FlashShape<HDP, NT>::CTAS) k_paged
             stage = stage + 1 == F::STAGES ? 0 : stage + 1;
             advance(p, cur);
         }
-        // 4: the warps' results become one. Sums of the weights over the eight rows of lanes first.
+        // 4: the warps' results become one. Each leaves its sums in the stage of its ring that was computed last (the others are
+        // being filled), the head's words turned by 8 for each pair of heads, which spreads an accumulator register's stores
+        // over all banks.
+        const int freed = stage == 0 ? F::STAGES - 1 : stage - 1;
+        auto sums = [&](int w) { return reinterpret_cast<float*>(sm + (w * F::STAGES + freed) * 2 * F::TILE_BYTES); };
+        {
+            float* mine_at = sums(warp);
 #pragma unroll
-        for (int n = 0; n < NT; n++)
+            for (int n = 0; n < NT; n++) {
 #pragma unroll
-            for (int j = 0; j < 2; j++) {
-                l[n][j] += __shfl_xor_sync(0xffffffffu, l[n][j], 4);
-                l[n][j] += __shfl_xor_sync(0xffffffffu, l[n][j], 8);
-                l[n][j] += __shfl_xor_sync(0xffffffffu, l[n][j], 16);
-                if (g == 0) stats[warp * F::HEADS + n * 8 + 2 * t + j] = make_float2(m[n][j], l[n][j]);
-            }
-        __syncthreads();
-        float top[NT][2], fac[NT][2];
-#pragma unroll
-        for (int n = 0; n < NT; n++)
-#pragma unroll
-            for (int j = 0; j < 2; j++) {
-                float M = -INFINITY;
-#pragma unroll
-                for (int w = 0; w < FL_WARPS; w++) M = fmaxf(M, stats[w * F::HEADS + n * 8 + 2 * t + j].x);
-                top[n][j] = M == -INFINITY ? 0.f : M;
-                fac[n][j] = exp2f(m[n][j] - top[n][j]);
-            }
-        auto store_slab = [&](int slab, bool add) {
-#pragma unroll
-            for (int n = 0; n < NT; n++)
+                for (int j = 0; j < 2; j++) {
+                    l[n][j] += __shfl_xor_sync(0xffffffffu, l[n][j], 4);
+                    l[n][j] += __shfl_xor_sync(0xffffffffu, l[n][j], 8);
+                    l[n][j] += __shfl_xor_sync(0xffffffffu, l[n][j], 16);
+                    if (g == 0) stats[warp * F::HEADS + n * 8 + 2 * t + j] = make_float2(m[n][j], l[n][j]);
+                }
 #pragma unroll
                 for (int j = 0; j < HDP / 16; j++)
 #pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const int h = n * 8 + 2 * t + (e & 1), d = j * 16 + g + (e >> 1) * 8;
-                        float* at = slabs + slab * (F::SLAB / 4) + h * F::PITCH + d;
-                        const float x = o[n][j][e] * fac[n][e & 1];
-                        *at = add ? *at + x : x;
-                    }
-        };
-        if (warp >= 2) store_slab(warp - 2, false);
-        __syncthreads();
-        if (warp < 2) store_slab(warp, true);
-        __syncthreads();
-        const bool whole = seg_i == 0 && seg_units == seg_n;
-        const int slot_index = 2 * (int)blockIdx.x + (seg_i == 0);
-        float* part = p.partial + (long long)slot_index * p.chunk * (hd + 2);
-        for (int i = tid; i < heads * hd; i += FL_THREADS) {
-            const int h = i / hd, d = i - h * hd;
-            const float x = slabs[h * F::PITCH + d] + slabs[F::SLAB / 4 + h * F::PITCH + d];
-            if (whole) {
-                float M = -INFINITY, L = 0.f;
-#pragma unroll
-                for (int w = 0; w < FL_WARPS; w++) M = fmaxf(M, stats[w * F::HEADS + h].x);
-                const float ref = M == -INFINITY ? 0.f : M;
-#pragma unroll
-                for (int w = 0; w < FL_WARPS; w++) L += stats[w * F::HEADS + h].y * exp2f(stats[w * F::HEADS + h].x - ref);
-                a.out[seg_b * a.o_row + (long long)(h0 + h) * hd + d] = __float2half_rn(L > 0.f ? x / L : 0.f);
-            } else {
-                part[h * (hd + 2) + 2 + d] = x;
+                    for (int e = 0; e < 4; e++) mine_at[(n * 8 + 2 * t + (e & 1)) * HDP + ((j * 16 + g + (e >> 1) * 8) ^ (t * 8))] = o[n][j][e];
             }
         }
-        if (tid < heads) {
+        __syncthreads();
+        const bool whole = seg_i == 0 && seg_units == seg_n;
+        const long long slot_floats = flash_slot_floats(p.chunk, hd);
+        float* part = p.partial + (2ll * blockIdx.x + (seg_i == 0)) * slot_floats;
+        auto finish = [&](int h, int d, float4 x, float M, float L) {     // four elements of a head's result
+            const float inv = L > 0.f ? 1.f / L : 0.f;
+            const __half2 lo = __floats2half2_rn(x.x * inv, x.y * inv), hi = __floats2half2_rn(x.z * inv, x.w * inv);
+            __half* at = a.out + seg_b * a.o_row + (long long)(h0 + h) * hd + d;
+            if (p.out8) {
+                *reinterpret_cast<uint2*>(at) = make_uint2(*reinterpret_cast<const unsigned*>(&lo), *reinterpret_cast<const unsigned*>(&hi));
+            } else {
+                at[0] = __low2half(lo); at[1] = __high2half(lo); at[2] = __low2half(hi); at[3] = __high2half(hi);
+            }
+            if (d == 0 && a.lse) a.lse[(long long)seg_b * a.n_heads + h0 + h] = L > 0.f ? (M + log2f(L)) * 0.69314718055994531f : -INFINITY;
+        };
+        for (int i = tid; i < heads * (HDP / 4); i += FL_THREADS) {
+            const int h = i / (HDP / 4), d = i % (HDP / 4) * 4;
+            if (d >= hd) continue;
+            float2 st[FL_WARPS];
             float M = -INFINITY, L = 0.f;
 #pragma unroll
-            for (int w = 0; w < FL_WARPS; w++) M = fmaxf(M, stats[w * F::HEADS + tid].x);
+            for (int w = 0; w < FL_WARPS; w++) {
+                st[w] = stats[w * F::HEADS + h];
+                M = fmaxf(M, st[w].x);
+            }
             const float ref = M == -INFINITY ? 0.f : M;
+            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-            for (int w = 0; w < FL_WARPS; w++) L += stats[w * F::HEADS + tid].y * exp2f(stats[w * F::HEADS + tid].x - ref);
+            for (int w = 0; w < FL_WARPS; w++) {
+                const float f = exp2f(st[w].x - ref);
+                const float4 y = *reinterpret_cast<const float4*>(sums(w) + h * HDP + (d ^ ((h >> 1 & 3) * 8)));
+                L += st[w].y * f;
+                x.x += y.x * f; x.y += y.y * f; x.z += y.z * f; x.w += y.w * f;
+            }
             if (whole) {
-                if (a.lse) a.lse[(long long)seg_b * a.n_heads + h0 + tid] = L > 0.f ? (M + log2f(L)) * 0.69314718055994531f : -INFINITY;
+                finish(h, d, x, M, L);
             } else {
-                part[tid * (hd + 2)] = M;
-                part[tid * (hd + 2) + 1] = L;
+                *reinterpret_cast<float4*>(part + h * hd + d) = x;
+                if (d == 0) *reinterpret_cast<float2*>(part + p.chunk * hd + 2 * h) = make_float2(M, L);
             }
         }
         if (!whole) {
-            // the ranges that hold a piece of it: CTAs first .. last; the last to arrive joins them
-            const unsigned long long base = (cur.left > 0 ? u1 - cur.left : u1) - seg_units - seg_i;
-            const int first = (int)(base / per), last = (int)((base + seg_n - 1) / per);
-            __threadfence();
+            // the ranges that hold a piece of it: CTAs first .. last; the last to arrive joins them, in their order
+            const unsigned long long base = u1 - cur.left - seg_units - seg_i;
+            int first, pieces;
+            if (U < (1ull << 31)) {
+                first = (int)((unsigned)base / (unsigned)per);
+                pieces = (int)((unsigned)(base + seg_n - 1) / (unsigned)per) - first + 1;
+            } else {
+                first = (int)(base / per);
+                pieces = (int)((base + seg_n - 1) / per) - first + 1;
+            }
             __syncthreads();
             if (tid == 0) {
-                last_sh = atomicAdd(p.counters + first, 1u) == (unsigned)(last - first);
+                __threadfence();
+                last_sh = atomicAdd(p.counters + first, 1u) == (unsigned)(pieces - 1);
                 if (last_sh) p.counters[first] = 0;
+                __threadfence();
             }
             __syncthreads();
             if (last_sh) {
-                __threadfence();
-                const long long step = 2ll * p.chunk * (hd + 2);          // from a CTA's slot to the next one's
-                const float* p0 = p.partial + (2ll * first + 1) * p.chunk * (hd + 2);
-                const float* p1 = p.partial + (2ll * first) * p.chunk * (hd + 2);      // + c * step for the others
-                for (int i = tid; i < heads * hd; i += FL_THREADS) {
-                    const int h = i / hd, d = i - h * hd;
-                    const int at = h * (hd + 2);
-                    float M = __ldcg(p0 + at);
-                    for (int c = 1; c <= last - first; c++) M = fmaxf(M, __ldcg(p1 + c * step + at));
-                    const float ref = M == -INFINITY ? 0.f : M;
-                    float w = exp2f(__ldcg(p0 + at) - ref);
-                    float L = __ldcg(p0 + at + 1) * w, x = __ldcg(p0 + at + 2 + d) * w;
-                    for (int c = 1; c <= last - first; c++) {
-                        const float* q1 = p1 + c * step + at;
-                        w = exp2f(__ldcg(q1) - ref);
-                        L += __ldcg(q1 + 1) * w;
-                        x += __ldcg(q1 + 2 + d) * w;
+                // the first piece is a range's last one (odd slot), the others are their ranges' first ones (even slots)
+                const float* p0 = p.partial + 2ll * first * slot_floats;
+                for (int i = tid; i < heads * (HDP / 4); i += FL_THREADS) {
+                    const int h = i / (HDP / 4), d = i % (HDP / 4) * 4;
+                    if (d >= hd) continue;
+                    float M = -INFINITY, L = 0.f;
+                    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+                    constexpr int AT_ONCE = 4;
+                    for (int c0 = 0; c0 < pieces; c0 += AT_ONCE) {
+                        float2 st[AT_ONCE];
+                        float4 y[AT_ONCE];
+#pragma unroll
+                        for (int c = 0; c < AT_ONCE; c++) {
+                            const float* from = p0 + (2ll * (c0 + c) + (c0 + c == 0)) * slot_floats;
+                            const bool in = c0 + c < pieces;
+                            st[c] = in ? __ldcg(reinterpret_cast<const float2*>(from + p.chunk * hd + 2 * h)) : make_float2(-INFINITY, 0.f);
+                            y[c] = in ? __ldcg(reinterpret_cast<const float4*>(from + h * hd + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
+                        }
+                        float top = M;
+#pragma unroll
+                        for (int c = 0; c < AT_ONCE; c++) top = fmaxf(top, st[c].x);
+                        const float ref = top == -INFINITY ? 0.f : top;
+                        const float old = exp2f(M - ref);
+                        L *= old; x.x *= old; x.y *= old; x.z *= old; x.w *= old;
+                        M = top;
+#pragma unroll
+                        for (int c = 0; c < AT_ONCE; c++) {
+                            const float f = exp2f(st[c].x - ref);
+                            L += st[c].y * f;
+                            x.x += y[c].x * f; x.y += y[c].y * f; x.z += y[c].z * f; x.w += y[c].w * f;
+                        }
                     }
-                    a.out[seg_b * a.o_row + (long long)(h0 + h) * hd + d] = __float2half_rn(L > 0.f ? x / L : 0.f);
-                    if (d == 0 && a.lse) a.lse[(long long)seg_b * a.n_heads + h0 + h] = L > 0.f ? (M + log2f(L)) * 0.69314718055994531f : -INFINITY;
+                    finish(h, d, x, M, L);
                 }
             }
         }
-        (void)seg_hg;
         __syncthreads();
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
@@ -547,7 +575,7 @@ int flash_chunk(int group, int head_dim) {
 
 size_t paged_attn_workspace_bytes(int n_heads, int n_kv_heads, int head_dim) {
     const int ctas = FL_MAX_SMS * (head_dim <= 64 ? FlashShape<64, 1>::CTAS : (head_dim <= 128 ? FlashShape<128, 1>::CTAS : FlashShape<256, 1>::CTAS));
-    return 4096 + 2 * (size_t)ctas * flash_chunk(n_heads / n_kv_heads, head_dim) * (head_dim + 2) * 4;
+    return 4096 + 2 * (size_t)ctas * flash_slot_floats(flash_chunk(n_heads / n_kv_heads, head_dim), head_dim) * 4;
 }
 
 int launch_paged_attn(const PagedView& c, const PagedAttnArgs& a, cudaStream_t st) {
@@ -568,6 +596,7 @@ int launch_paged_attn(const PagedView& c, const PagedAttnArgs& a, cudaStream_t s
     f.chunks = (p.group + f.chunk - 1) / f.chunk;
     f.groups = p.n_kv * f.chunks;
     f.scale_log2 = a.scale * 1.4426950408889634f;
+    f.out8 = (reinterpret_cast<uintptr_t>(a.out) & 7) == 0 && a.o_row % 4 == 0;
     f.counters = static_cast<unsigned int*>(a.work);
     f.partial = reinterpret_cast<float*>(static_cast<char*>(a.work) + 4096);
     if (p.head_dim <= 64) return f.chunk <= 8 ? launch_flash<64, 1>(f, st) : launch_flash<64, 2>(f, st);
