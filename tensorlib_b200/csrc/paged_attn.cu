@@ -110,14 +110,16 @@ __global__ void __launch_bounds__(ANY_WARPS * 32) k_paged_attn_any(AttnLaunch p)
 // (cp.async, zero-filled behind the last token and for ids outside the pool, so nothing unwritten is ever multiplied);
 // page ids are looked up one tile further ahead. Warps meet only at the end of a (sequence, head group).
 //
-// The work of all sequences, counted in units of 64 tokens, is cut into equal contiguous ranges, one a CTA: ragged batches
-// fill the machine whatever their lengths, one long sequence as well as many. A (sequence, head group) that falls into one
+// The work of all sequences, counted in units of 64 tokens and FL_START more for every (sequence, head group), which is about
+// what starting and finishing one costs, is cut into equal contiguous ranges, one a CTA: ragged batches fill the machine
+// whatever their lengths, one long sequence as well as many. A (sequence, head group) that falls into one
 // range is finished there; one that is cut leaves partial results (max, sum, sums of values) in the workspace, and the CTA
 // that comes last joins them, in order of the ranges.
 constexpr int FL_WARPS = 4;
 constexpr int FL_THREADS = FL_WARPS * 32;
 constexpr int FL_TILE = 16;                       // tokens of a warp's tile
 constexpr int FL_UNIT = FL_TILE * FL_WARPS;
+constexpr int FL_START = 2;
 constexpr int FL_MAX_SMS = 160;
 
 struct FlashLaunch {
@@ -130,9 +132,15 @@ struct FlashLaunch {
 
 template <int HDP, int NT>
 struct FlashShape {
-    static constexpr int STAGES = HDP == 64 ? 4 : (HDP == 128 ? 3 : 2);
-    static constexpr int CTAS = HDP == 64 ? 3 : (HDP == 128 ? 2 : 1);     // per SM
-    static constexpr int TILE_BYTES = FL_TILE * HDP * 2;
+    static constexpr int STAGES = HDP <= 96 ? 4 : (HDP == 128 ? 3 : 2);
+    static constexpr int CTAS = HDP == 64 ? 3 : (HDP <= 128 ? 2 : 1);     // per SM
+    // The same 16-byte chunk of eight rows lies in different banks: rows of a multiple of 128 bytes have their chunks turned by
+    // the row (a pitch 16 bytes longer did the same for the reads, but took 320 us for 283 at four long contexts), others
+    // are 16 bytes apart.
+    static constexpr bool TURNED = HDP % 64 == 0;
+    static constexpr int PITCH = TURNED ? HDP * 2 : HDP * 2 + 16;
+    __device__ static __forceinline__ uint32_t at(int row, int chunk) { return row * PITCH + ((TURNED ? chunk ^ (row & 7) : chunk) << 4); }
+    static constexpr int TILE_BYTES = FL_TILE * PITCH;
     static constexpr int RING = FL_WARPS * STAGES * 2 * TILE_BYTES;
     static constexpr int HEADS = 8 * NT;
     static constexpr int SMEM = RING + FL_WARPS * HEADS * 8 + FL_WARPS * STAGES * 4;
@@ -162,17 +170,21 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
     return y;
 }
 
-// a place in the flattened (sequence, head group, unit) space
+// a place in the flattened (sequence, head group, FL_START + unit) space
 struct Cursor {
     int b, row, len, units, hg, i;
-    long long left;                               // units of this CTA's range from here on
+    long long left;                               // of this CTA's range from here on
 };
 
 __device__ __forceinline__ int units_of(int len) { return (len + FL_UNIT - 1) / FL_UNIT; }
 
+__device__ __forceinline__ int cost_of(int len) { return len > 0 ? units_of(len) + FL_START : 0; }
+
 __device__ __forceinline__ void advance(const FlashLaunch& p, Cursor& c) {
     if (--c.left <= 0) return;
     if (++c.i < c.units) return;
+    c.left -= FL_START;
+    if (c.left <= 0) return;
     c.i = 0;
     if (++c.hg < p.groups) return;
     c.hg = 0;
@@ -198,13 +210,13 @@ __global__ void __launch_bounds__(FL_THREADS, FlashShape<HDP, NT>::CTAS) k_paged
     pdl_launch_dependents();
     pdl_wait();
 
-    // 1: this CTA's range. Every CTA adds up the units of all sequences; a thread takes a run of them.
+    // 1: this CTA's range. Every CTA adds up the costs of all sequences; a thread takes a run of them.
     const int per_thread = (a.batch + FL_THREADS - 1) / FL_THREADS;
     const int b0 = min(a.batch, tid * per_thread), b1 = min(a.batch, b0 + per_thread);
     unsigned long long mine = 0;
     for (int b = b0; b < b1; b++) {
         int row;
-        mine += units_of(row_tokens(a, b, row));
+        mine += cost_of(row_tokens(a, b, row));
     }
     unsigned long long upto = mine;
 #pragma unroll
@@ -243,7 +255,7 @@ __global__ void __launch_bounds__(FL_THREADS, FlashShape<HDP, NT>::CTAS) k_paged
         unsigned long long at = before;
         for (int b = b0; b < b1; b++) {
             int row;
-            const int len = row_tokens(a, b, row), n = units_of(len);
+            const int len = row_tokens(a, b, row), n = cost_of(len);
             if (u0 < (at + n) * p.groups) {
                 start_sh = at;
                 start_b = b;
@@ -262,10 +274,15 @@ __global__ void __launch_bounds__(FL_THREADS, FlashShape<HDP, NT>::CTAS) k_paged
     cur.units = units_of(cur.len);
     {
         const unsigned long long in = u0 - start_sh * p.groups;
-        cur.hg = in < (1ull << 31) ? (int)((unsigned)in / (unsigned)cur.units) : (int)(in / cur.units);
-        cur.i = (int)(in - (unsigned long long)cur.hg * cur.units);
+        const int cost = cur.units + FL_START;
+        cur.hg = in < (1ull << 31) ? (int)((unsigned)in / (unsigned)cost) : (int)(in / cost);
+        cur.i = (int)(in - (unsigned long long)cur.hg * cost) - FL_START;
     }
     cur.left = (long long)(u1 - u0);
+    if (cur.i < 0) {
+        cur.left += cur.i;
+        cur.i = 0;
+    }
     Cursor ahead = cur;                           // what is looked up next
 
     // 2: loads. lookup(): the page id of this lane's token (lanes 16.. repeat 0..15); issue(): the tile's rows.
@@ -286,9 +303,6 @@ __global__ void __launch_bounds__(FL_THREADS, FlashShape<HDP, NT>::CTAS) k_paged
         return k;
     };
     constexpr int CPR = HDP / 8;                  // 16-byte chunks a row
-    constexpr int ROWS = 32 / CPR;                // rows an instruction
-    const int chunk = lane % CPR;
-    const bool in_row = chunk * 8 < hd;
     unsigned char* ring = sm + warp * F::STAGES * 2 * F::TILE_BYTES;
     auto issue = [&](int stage, const Look& k) {
         long long off = -1;
@@ -301,24 +315,24 @@ __global__ void __launch_bounds__(FL_THREADS, FlashShape<HDP, NT>::CTAS) k_paged
         if (mask) {
             const uint32_t kd = smem_addr(ring + stage * 2 * F::TILE_BYTES), vd = kd + F::TILE_BYTES;
 #pragma unroll
-            for (int r0 = 0; r0 < FL_TILE; r0 += ROWS) {
-                const int r = r0 + lane / CPR;
+            for (int i0 = 0; i0 < FL_TILE * CPR; i0 += 32) {
+                const int r = (i0 + lane) / CPR, chunk = (i0 + lane) % CPR;
                 const long long o = __shfl_sync(0xffffffffu, off, r);
-                const bool ok = o >= 0 && in_row;
+                const bool ok = o >= 0 && chunk * 8 < hd;
                 const long long at = ok ? o + chunk * 8 : 0;
-                const uint32_t d = r * (HDP * 2) + ((chunk ^ (r & 7)) << 4);
+                const uint32_t d = F::at(r, chunk);
                 cp_async16(kd + d, a.k + at, ok ? 16 : 0);
                 cp_async16(vd + d, a.v + at, ok ? 16 : 0);
             }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    Look ahead_look;
+    Look look;                                    // of the next tile to load
     {
         Look first[F::STAGES - 1];                // their lookups are under way together
 #pragma unroll
         for (int s = 0; s < F::STAGES - 1; s++) first[s] = lookup();
-        ahead_look = lookup();
+        look = lookup();
 #pragma unroll
         for (int s = 0; s < F::STAGES - 1; s++) issue(s, first[s]);
     }
@@ -332,6 +346,7 @@ __global__ void __launch_bounds__(FL_THREADS, FlashShape<HDP, NT>::CTAS) k_paged
         const int heads = min(p.chunk, (kvh + 1) * a.group - h0);
         const long long seg_units = min((long long)(cur.units - cur.i), cur.left);
         const int seg_b = cur.b, seg_i = cur.i, seg_n = cur.units;
+        const unsigned long long base = u1 - cur.left - seg_i;               // where its first unit lies
         uint32_t q[NT][HDP / 16][2];
 #pragma unroll
         for (int n = 0; n < NT; n++)
@@ -356,8 +371,8 @@ __global__ void __launch_bounds__(FL_THREADS, FlashShape<HDP, NT>::CTAS) k_paged
             const uint32_t mask = masks[warp * F::STAGES + stage];
             {
                 const int next = stage == 0 ? F::STAGES - 1 : stage - 1;       // the stage computed last
-                issue(next, ahead_look);
-                ahead_look = lookup();
+                issue(next, look);
+                look = lookup();
             }
             if (mask) {
                 const uint32_t ks_base = smem_addr(ring + stage * 2 * F::TILE_BYTES), vs_base = ks_base + F::TILE_BYTES;
@@ -368,7 +383,7 @@ __global__ void __launch_bounds__(FL_THREADS, FlashShape<HDP, NT>::CTAS) k_paged
 #pragma unroll
                 for (int ks = 0; ks < HDP / 16; ks++) {
                     uint32_t f[4];
-                    ldsm4(f, ks_base + kr * (HDP * 2) + (((2 * ks + (lane >> 4)) ^ (kr & 7)) << 4));
+                    ldsm4(f, ks_base + F::at(kr, 2 * ks + (lane >> 4)));
 #pragma unroll
                     for (int n = 0; n < NT; n++) mma16816(s[n], f, q[n][ks][0], q[n][ks][1]);
                 }
@@ -418,7 +433,7 @@ __global__ void __launch_bounds__(FL_THREADS, FlashShape<HDP, NT>::CTAS) k_paged
 #pragma unroll
                 for (int j = 0; j < HDP / 16; j++) {
                     uint32_t f[4];
-                    ldsm4t(f, vs_base + vr * (HDP * 2) + (((2 * j + vc) ^ (vr & 7)) << 4));
+                    ldsm4t(f, vs_base + F::at(vr, 2 * j + vc));
 #pragma unroll
                     for (int n = 0; n < NT; n++) {
                         mma16816(o[n][j], f, ph[n][0], ph[n][1]);
@@ -495,7 +510,6 @@ __global__ void __launch_bounds__(FL_THREADS, FlashShape<HDP, NT>::CTAS) k_paged
         }
         if (!whole) {
             // the ranges that hold a piece of it: CTAs first .. last; the last to arrive joins them, in their order
-            const unsigned long long base = u1 - cur.left - seg_units - seg_i;
             int first, pieces;
             if (U < (1ull << 31)) {
                 first = (int)((unsigned)base / (unsigned)per);
@@ -600,6 +614,7 @@ int launch_paged_attn(const PagedView& c, const PagedAttnArgs& a, cudaStream_t s
     f.counters = static_cast<unsigned int*>(a.work);
     f.partial = reinterpret_cast<float*>(static_cast<char*>(a.work) + 4096);
     if (p.head_dim <= 64) return f.chunk <= 8 ? launch_flash<64, 1>(f, st) : launch_flash<64, 2>(f, st);
+    if (p.head_dim <= 96) return f.chunk <= 8 ? launch_flash<96, 1>(f, st) : launch_flash<96, 2>(f, st);
     if (p.head_dim <= 128) return f.chunk <= 8 ? launch_flash<128, 1>(f, st) : launch_flash<128, 2>(f, st);
     return launch_flash<256, 1>(f, st);
 }
