@@ -352,7 +352,8 @@ TL_API int tl_rotary_append_f16(const tl_paged_cache* cache, int layer, const tl
 /* Attention of one query per batch entry over all lengths[row] tokens of its row: out_h = sum_t softmax_t(scale q_h.k_t) v_t, query
  * head h reading KV head h / (n_heads / n_kv_heads). q, out: [batch] rows of n_heads * head_dim values, row strides in elements.
  * rows[b]: the row of entry b, -1 for a padding entry (rows == NULL: row b). lse, if not NULL: fp32 [batch, n_heads],
- * log sum_t exp(scale q_h.k_t). An empty row gives zeros and -inf. head_dim <= 256. workspace: tl_paged_attn_workspace bytes (at
+ * log sum_t exp(scale q_h.k_t). An empty row gives zeros and -inf. head_dim <= 256, and batch * n_heads * (max_pages * page_size / 64 + 3)
+ * has to stay below 2^31 (TL_ERR_UNSUPPORTED). workspace: tl_paged_attn_workspace bytes (at
  * most 32 MB), zeroed once before its first use; calls leave it as the next one needs it. */
 TL_API int tl_paged_attn_decode_f16(const tl_paged_cache* cache, int layer, const tl_half* q, tl_half* out, float* lse, const int* rows,
                                     int batch, int n_heads, float scale, long long q_row_stride, long long out_row_stride,

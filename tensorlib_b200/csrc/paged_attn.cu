@@ -120,20 +120,22 @@ constexpr int FL_THREADS = FL_WARPS * 32;
 constexpr int FL_TILE = 16;                       // tokens of a warp's tile
 constexpr int FL_UNIT = FL_TILE * FL_WARPS;
 constexpr int FL_START = 2;
+constexpr int FL_JOIN = 16;                       // pieces joined at a time
 constexpr int FL_MAX_SMS = 160;
 
 struct FlashLaunch {
     AttnLaunch a;
     int chunk, chunks, groups;                    // query heads of a head group, head groups a KV head, head groups in all
+    FastDiv by_grid;
     float scale_log2;
     bool out8;                                    // out can be stored 8 bytes at a time
-    unsigned int* counters; float* partial;       // workspace: [CTAs], [2 CTAs] partial results
+    unsigned int* counters; float* partial;       // workspace: [3 CTAs]; [4 CTAs] partial results
 };
 
 template <int HDP, int NT>
 struct FlashShape {
-    static constexpr int STAGES = HDP <= 96 ? 4 : (HDP == 128 ? 3 : 2);
-    static constexpr int CTAS = HDP == 64 ? 3 : (HDP <= 128 ? 2 : 1);     // per SM
+    static constexpr int STAGES = HDP <= 96 ? 4 : (HDP == 192 ? 2 : 3);
+    static constexpr int CTAS = HDP == 64 ? 3 : (HDP <= 192 ? 2 : 1);     // per SM
     // The same 16-byte chunk of eight rows lies in different banks: rows of a multiple of 128 bytes have their chunks turned by
     // the row (a pitch 16 bytes longer did the same for the reads, but took 320 us for 283 at four long contexts), others
     // are 16 bytes apart.
@@ -170,14 +172,13 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
     return y;
 }
 
-// a place in the flattened (sequence, head group, FL_START + unit) space
+// a place in the flattened (sequence, head group, FL_START + unit) space; a head group is a part of a KV head's query heads
 struct Cursor {
-    int b, row, len, units, hg, i;
-    long long left;                               // of this CTA's range from here on
+    int b, row, len, units, kvh, part, i;
+    int left;                                     // of this CTA's range from here on
 };
 
 __device__ __forceinline__ int units_of(int len) { return (len + FL_UNIT - 1) / FL_UNIT; }
-
 __device__ __forceinline__ int cost_of(int len) { return len > 0 ? units_of(len) + FL_START : 0; }
 
 __device__ __forceinline__ void advance(const FlashLaunch& p, Cursor& c) {
@@ -186,13 +187,25 @@ __device__ __forceinline__ void advance(const FlashLaunch& p, Cursor& c) {
     c.left -= FL_START;
     if (c.left <= 0) return;
     c.i = 0;
-    if (++c.hg < p.groups) return;
-    c.hg = 0;
+    if (++c.part < p.chunks) return;
+    c.part = 0;
+    if (++c.kvh < p.a.n_kv) return;
+    c.kvh = 0;
     do {
         c.b++;
         c.len = row_tokens(p.a, c.b, c.row);
         c.units = units_of(c.len);
     } while (c.units == 0);
+}
+
+// one more arrival of `expected`; true for the last one, which then sees what the others wrote (the caller's CTA has met at a
+// barrier before, so its writes are covered) and leaves the counter at 0
+__device__ __forceinline__ bool last_to_arrive(unsigned int* counter, int expected) {
+    unsigned int before;
+    asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(before) : "l"(counter) : "memory");
+    if (before != (unsigned)(expected - 1)) return false;
+    *counter = 0;
+    return true;
 }
 
 template <int HDP, int NT>
@@ -201,41 +214,44 @@ __global__ void __launch_bounds__(FL_THREADS, FlashShape<HDP, NT>::CTAS) k_paged
     extern __shared__ __align__(128) unsigned char sm[];
     float2* stats = reinterpret_cast<float2*>(sm + F::RING);                                 // [warp][head]: max, sum
     uint32_t* masks = reinterpret_cast<uint32_t*>(sm + F::RING + FL_WARPS * F::HEADS * 8);   // [warp][stage]
-    __shared__ unsigned long long scan_sh[FL_WARPS];
-    __shared__ unsigned long long start_sh;
-    __shared__ int start_b, start_row, start_len;
+    __shared__ int scan_sh[FL_WARPS];
+    __shared__ int start_sh, start_b, start_row, start_len;
     __shared__ int last_sh;
     const AttnLaunch& a = p.a;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, hd = a.head_dim;
     pdl_launch_dependents();
     pdl_wait();
 
-    // 1: this CTA's range. Every CTA adds up the costs of all sequences; a thread takes a run of them.
+    // 1: this CTA's range. Every CTA adds up the costs of all sequences; a thread takes a run of them. (The host has made sure
+    // that the sum fits 31 bits.)
     const int per_thread = (a.batch + FL_THREADS - 1) / FL_THREADS;
     const int b0 = min(a.batch, tid * per_thread), b1 = min(a.batch, b0 + per_thread);
-    unsigned long long mine = 0;
-    for (int b = b0; b < b1; b++) {
+    int row0 = 0, len0 = 0, mine = 0;             // the run's first sequence, the run's cost
+    if (b0 < b1) {
+        len0 = row_tokens(a, b0, row0);
+        mine = cost_of(len0);
+    }
+    for (int b = b0 + 1; b < b1; b++) {
         int row;
         mine += cost_of(row_tokens(a, b, row));
     }
-    unsigned long long upto = mine;
+    int upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const unsigned long long y = __shfl_up_sync(0xffffffffu, upto, o);
+        const int y = __shfl_up_sync(0xffffffffu, upto, o);
         if (lane >= o) upto += y;
     }
     if (lane == 31) scan_sh[warp] = upto;
     __syncthreads();
-    unsigned long long before = upto - mine, total = 0;
+    int before = upto - mine, total = 0;
 #pragma unroll
     for (int w = 0; w < FL_WARPS; w++) {
         if (w < warp) before += scan_sh[w];
         total += scan_sh[w];
     }
-    // (counts of units that fit 32 bits, the ordinary case, are divided there: a 64-bit division takes a tenth of a microsecond)
-    const unsigned long long U = total * p.groups;
-    const unsigned long long per = U < (1ull << 31) ? ((unsigned)U + gridDim.x - 1) / gridDim.x : (U + gridDim.x - 1) / gridDim.x;
-    const unsigned long long u0 = per * blockIdx.x, u1 = u0 + per < U ? u0 + per : U;
+    const int U = total * p.groups;
+    const int per = (int)p.by_grid.div((unsigned)U + gridDim.x - 1);
+    const int u0 = per * (int)blockIdx.x, u1 = min(u0 + per, U);
     // sequences with nothing to attend to
     auto empty_rows = [&] {
         for (int b = blockIdx.x; b < a.batch; b += gridDim.x) {
@@ -252,19 +268,15 @@ __global__ void __launch_bounds__(FL_THREADS, FlashShape<HDP, NT>::CTAS) k_paged
         return;
     }
     if (u0 >= before * p.groups && u0 < (before + mine) * p.groups) {      // one thread's run holds the start
-        unsigned long long at = before;
-        for (int b = b0; b < b1; b++) {
-            int row;
-            const int len = row_tokens(a, b, row), n = cost_of(len);
-            if (u0 < (at + n) * p.groups) {
-                start_sh = at;
-                start_b = b;
-                start_row = row;
-                start_len = len;
-                break;
-            }
-            at += n;
+        int b = b0, at = before;
+        while (u0 >= (at + cost_of(len0)) * p.groups) {
+            at += cost_of(len0);
+            len0 = row_tokens(a, ++b, row0);
         }
+        start_sh = at * p.groups;
+        start_b = b;
+        start_row = row0;
+        start_len = len0;
     }
     __syncthreads();
     Cursor cur;                                   // what is computed next
@@ -273,12 +285,13 @@ __global__ void __launch_bounds__(FL_THREADS, FlashShape<HDP, NT>::CTAS) k_paged
     cur.len = start_len;
     cur.units = units_of(cur.len);
     {
-        const unsigned long long in = u0 - start_sh * p.groups;
-        const int cost = cur.units + FL_START;
-        cur.hg = in < (1ull << 31) ? (int)((unsigned)in / (unsigned)cost) : (int)(in / cost);
-        cur.i = (int)(in - (unsigned long long)cur.hg * cost) - FL_START;
+        const unsigned in = (unsigned)(u0 - start_sh), cost = (unsigned)cur.units + FL_START;
+        const int hg = (int)(in / cost);
+        cur.i = (int)(in - (unsigned)hg * cost) - FL_START;
+        cur.kvh = p.chunks == 1 ? hg : hg / p.chunks;
+        cur.part = hg - cur.kvh * p.chunks;
     }
-    cur.left = (long long)(u1 - u0);
+    cur.left = u1 - u0;
     if (cur.i < 0) {
         cur.left += cur.i;
         cur.i = 0;
@@ -291,7 +304,7 @@ __global__ void __launch_bounds__(FL_THREADS, FlashShape<HDP, NT>::CTAS) k_paged
         Look k{0, -1, 0};
         if (ahead.left > 0) {
             const int tok = ahead.i * FL_UNIT + warp * FL_TILE + (lane & 15);
-            k.kvh = ahead.hg / p.chunks;
+            k.kvh = ahead.kvh;
             if (tok < ahead.len) {
                 unsigned pg, s;
                 a.by_page.divmod((unsigned)tok, pg, s);
@@ -342,11 +355,10 @@ __global__ void __launch_bounds__(FL_THREADS, FlashShape<HDP, NT>::CTAS) k_paged
     const int g = lane >> 2, t = lane & 3;        // fragment row and column pair
     int stage = 0;
     while (cur.left > 0) {
-        const int kvh = cur.hg / p.chunks, h0 = kvh * a.group + (cur.hg - kvh * p.chunks) * p.chunk;
-        const int heads = min(p.chunk, (kvh + 1) * a.group - h0);
-        const long long seg_units = min((long long)(cur.units - cur.i), cur.left);
+        const int h0 = cur.kvh * a.group + cur.part * p.chunk, heads = min(p.chunk, (cur.kvh + 1) * a.group - h0);
+        const int seg_units = min(cur.units - cur.i, cur.left);
         const int seg_b = cur.b, seg_i = cur.i, seg_n = cur.units;
-        const unsigned long long base = u1 - cur.left - seg_i;               // where its first unit lies
+        const int base = u1 - cur.left - seg_i;                              // where its first unit lies
         uint32_t q[NT][HDP / 16][2];
 #pragma unroll
         for (int n = 0; n < NT; n++)
@@ -365,7 +377,7 @@ __global__ void __launch_bounds__(FL_THREADS, FlashShape<HDP, NT>::CTAS) k_paged
 #pragma unroll
             for (int j = 0; j < HDP / 16; j++) o[n][j][0] = o[n][j][1] = o[n][j][2] = o[n][j][3] = 0.f;
         }
-        for (long long u = 0; u < seg_units; u++) {
+        for (int u = 0; u < seg_units; u++) {
             asm volatile("cp.async.wait_group %0;" ::"n"(F::STAGES - 2) : "memory");
             __syncwarp();
             const uint32_t mask = masks[warp * F::STAGES + stage];
@@ -509,39 +521,24 @@ __global__ void __launch_bounds__(FL_THREADS, FlashShape<HDP, NT>::CTAS) k_paged
             }
         }
         if (!whole) {
-            // the ranges that hold a piece of it: CTAs first .. last; the last to arrive joins them, in their order
-            int first, pieces;
-            if (U < (1ull << 31)) {
-                first = (int)((unsigned)base / (unsigned)per);
-                pieces = (int)((unsigned)(base + seg_n - 1) / (unsigned)per) - first + 1;
-            } else {
-                first = (int)(base / per);
-                pieces = (int)((base + seg_n - 1) / per) - first + 1;
-            }
-            __syncthreads();
-            if (tid == 0) {
-                __threadfence();
-                last_sh = atomicAdd(p.counters + first, 1u) == (unsigned)(pieces - 1);
-                if (last_sh) p.counters[first] = 0;
-                __threadfence();
-            }
-            __syncthreads();
-            if (last_sh) {
-                // the first piece is a range's last one (odd slot), the others are their ranges' first ones (even slots)
-                const float* p0 = p.partial + 2ll * first * slot_floats;
+            // The ranges that hold a piece of it: CTAs first .. first + pieces - 1. Up to FL_JOIN consecutive pieces are joined by
+            // the last of them to arrive; where there are more groups than one, the last group to arrive joins the groups'
+            // results the same way, in order.
+            const int first = (int)((unsigned)base / (unsigned)per), pieces = (int)((unsigned)(base + seg_n - 1) / (unsigned)per) - first + 1;
+            auto join = [&](int n, auto&& piece, bool final, float* to) {       // piece(c): partial result c < n
                 for (int i = tid; i < heads * (HDP / 4); i += FL_THREADS) {
                     const int h = i / (HDP / 4), d = i % (HDP / 4) * 4;
                     if (d >= hd) continue;
                     float M = -INFINITY, L = 0.f;
                     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
                     constexpr int AT_ONCE = 4;
-                    for (int c0 = 0; c0 < pieces; c0 += AT_ONCE) {
+                    for (int c0 = 0; c0 < n; c0 += AT_ONCE) {
                         float2 st[AT_ONCE];
                         float4 y[AT_ONCE];
 #pragma unroll
                         for (int c = 0; c < AT_ONCE; c++) {
-                            const float* from = p0 + (2ll * (c0 + c) + (c0 + c == 0)) * slot_floats;
-                            const bool in = c0 + c < pieces;
+                            const bool in = c0 + c < n;
+                            const float* from = piece(in ? c0 + c : 0);
                             st[c] = in ? __ldcg(reinterpret_cast<const float2*>(from + p.chunk * hd + 2 * h)) : make_float2(-INFINITY, 0.f);
                             y[c] = in ? __ldcg(reinterpret_cast<const float4*>(from + h * hd + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
                         }
@@ -559,7 +556,30 @@ __global__ void __launch_bounds__(FL_THREADS, FlashShape<HDP, NT>::CTAS) k_paged
                             x.x += y[c].x * f; x.y += y[c].y * f; x.z += y[c].z * f; x.w += y[c].w * f;
                         }
                     }
-                    finish(h, d, x, M, L);
+                    if (final) {
+                        finish(h, d, x, M, L);
+                    } else {
+                        *reinterpret_cast<float4*>(to + h * hd + d) = x;
+                        if (d == 0) *reinterpret_cast<float2*>(to + p.chunk * hd + 2 * h) = make_float2(M, L);
+                    }
+                }
+            };
+            // the first piece is its range's last segment (odd slot), the others are their ranges' first ones (even slots)
+            auto slot_of = [&](int c) { return 2ll * (first + c) + (c == 0); };
+            const int c = (int)blockIdx.x - first, group = c / FL_JOIN, groups = (pieces + FL_JOIN - 1) / FL_JOIN;
+            const int members = min(FL_JOIN, pieces - group * FL_JOIN);
+            const long long joined0 = 2ll * gridDim.x;                          // groups' results lie behind the pieces
+            __syncthreads();
+            if (tid == 0) last_sh = last_to_arrive(p.counters + slot_of(group * FL_JOIN), members);
+            __syncthreads();
+            if (last_sh) {
+                join(members, [&](int k) { return p.partial + slot_of(group * FL_JOIN + k) * slot_floats; }, groups == 1,
+                     p.partial + (joined0 + slot_of(group * FL_JOIN)) * slot_floats);
+                if (groups > 1) {
+                    __syncthreads();
+                    if (tid == 0) last_sh = last_to_arrive(p.counters + 2 * gridDim.x + first, groups);
+                    __syncthreads();
+                    if (last_sh) join(groups, [&](int k) { return p.partial + (joined0 + slot_of(k * FL_JOIN)) * slot_floats; }, true, nullptr);
                 }
             }
         }
@@ -573,8 +593,10 @@ int launch_flash(const FlashLaunch& p, cudaStream_t st) {
     using F = FlashShape<HDP, NT>;
     static PerDeviceOnce once;
     if (once.needed()) TL_CUDA(cudaFuncSetAttribute(k_paged_attn<HDP, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::SMEM));
+    FlashLaunch q = p;
     const int grid = (sm_count() < FL_MAX_SMS ? sm_count() : FL_MAX_SMS) * F::CTAS;
-    return launch_pdl(k_paged_attn<HDP, NT>, grid, FL_THREADS, F::SMEM, st, true, p);
+    q.by_grid = FastDiv((unsigned)grid);
+    return launch_pdl(k_paged_attn<HDP, NT>, grid, FL_THREADS, F::SMEM, st, true, q);
 }
 
 // query heads of a head group: as few groups as 16 columns allow (8 at 256 elements a head, where 16 would not fit the
@@ -588,8 +610,8 @@ int flash_chunk(int group, int head_dim) {
 }  // namespace
 
 size_t paged_attn_workspace_bytes(int n_heads, int n_kv_heads, int head_dim) {
-    const int ctas = FL_MAX_SMS * (head_dim <= 64 ? FlashShape<64, 1>::CTAS : (head_dim <= 128 ? FlashShape<128, 1>::CTAS : FlashShape<256, 1>::CTAS));
-    return 4096 + 2 * (size_t)ctas * flash_slot_floats(flash_chunk(n_heads / n_kv_heads, head_dim), head_dim) * 4;
+    const int ctas = FL_MAX_SMS * (head_dim <= 64 ? FlashShape<64, 1>::CTAS : (head_dim <= 192 ? FlashShape<192, 1>::CTAS : FlashShape<256, 1>::CTAS));
+    return 8192 + 4 * (size_t)ctas * flash_slot_floats(flash_chunk(n_heads / n_kv_heads, head_dim), head_dim) * 4;
 }
 
 int launch_paged_attn(const PagedView& c, const PagedAttnArgs& a, cudaStream_t st) {
@@ -604,6 +626,10 @@ int launch_paged_attn(const PagedView& c, const PagedAttnArgs& a, cudaStream_t s
     p.status = device_status_word();
     const bool fast = c.aligned16() && (reinterpret_cast<uintptr_t>(a.q) & 3) == 0 && a.q_row % 2 == 0;
     if (!fast) return launch_pdl(k_paged_attn_any, dim3(a.n_heads, a.batch), ANY_WARPS * 32, 0, st, true, p);
+    // the cost of the whole batch has to fit 31 bits
+    const long long cost = ((long long)c.max_pages * c.page_size + FL_UNIT - 1) / FL_UNIT + FL_START;
+    if (cost * a.batch * a.n_heads >= (1ll << 31) - 1024)
+        return set_error(TL_ERR_UNSUPPORTED, "paged_attn_decode: batch * n_heads * (max_pages * page_size / 64 + 3) has to stay below 2^31");
     FlashLaunch f{};
     f.a = p;
     f.chunk = flash_chunk(p.group, p.head_dim);
@@ -612,11 +638,11 @@ int launch_paged_attn(const PagedView& c, const PagedAttnArgs& a, cudaStream_t s
     f.scale_log2 = a.scale * 1.4426950408889634f;
     f.out8 = (reinterpret_cast<uintptr_t>(a.out) & 7) == 0 && a.o_row % 4 == 0;
     f.counters = static_cast<unsigned int*>(a.work);
-    f.partial = reinterpret_cast<float*>(static_cast<char*>(a.work) + 4096);
+    f.partial = reinterpret_cast<float*>(static_cast<char*>(a.work) + 8192);
     if (p.head_dim <= 64) return f.chunk <= 8 ? launch_flash<64, 1>(f, st) : launch_flash<64, 2>(f, st);
     if (p.head_dim <= 96) return f.chunk <= 8 ? launch_flash<96, 1>(f, st) : launch_flash<96, 2>(f, st);
     if (p.head_dim <= 128) return f.chunk <= 8 ? launch_flash<128, 1>(f, st) : launch_flash<128, 2>(f, st);
-    return launch_flash<256, 1>(f, st);
+    return p.head_dim <= 192 ? launch_flash<192, 1>(f, st) : launch_flash<256, 1>(f, st);
 }
 
 }  // namespace tlb
