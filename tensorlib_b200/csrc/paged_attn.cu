@@ -122,6 +122,7 @@ constexpr int FL_UNIT = FL_TILE * FL_WARPS;
 constexpr int FL_START = 2;
 constexpr int FL_JOIN = 16;                       // pieces joined at a time
 constexpr int FL_MAX_SMS = 160;
+constexpr int FL_COUNTER_BYTES = 8192;
 
 struct FlashLaunch {
     AttnLaunch a;
@@ -134,14 +135,17 @@ struct FlashLaunch {
 
 template <int HDP, int NT>
 struct FlashShape {
-    static constexpr int STAGES = HDP <= 96 ? 4 : (HDP == 192 ? 2 : 3);
-    static constexpr int CTAS = HDP == 64 ? 3 : (HDP <= 192 ? 2 : 1);     // per SM
-    // The same 16-byte chunk of eight rows lies in different banks: rows of a multiple of 128 bytes have their chunks turned by
-    // the row (a pitch 16 bytes longer did the same for the reads, but took 320 us for 283 at four long contexts), others
-    // are 16 bytes apart.
-    static constexpr bool TURNED = HDP % 64 == 0;
-    static constexpr int PITCH = TURNED ? HDP * 2 : HDP * 2 + 16;
-    __device__ static __forceinline__ uint32_t at(int row, int chunk) { return row * PITCH + ((TURNED ? chunk ^ (row & 7) : chunk) << 4); }
+    // Stages of a warp's ring and CTAs an SM. More warps beat deeper rings where both keep some 100 KB under way: at 128
+    // elements, 3 x 2 against 2 x 3, 32 sequences of 500..2000 tokens took 31.0 against 32.9 us, 256 of 1..100 21.0 against 25.6.
+    static constexpr int STAGES = HDP <= 96 ? 3 : (HDP == 256 ? 3 : 2);
+    static constexpr int CTAS = HDP == 64 ? 4 : (HDP <= 128 ? 3 : (HDP == 192 ? 2 : 1));
+    // The same 16-byte chunk of eight rows lies in different banks: the chunks are turned by the row, where rows are 192 bytes,
+    // which alternate between halves of the banks, by every second one. (A pitch 16 bytes longer did the same for the reads,
+    // but took 320 us for 283 at four long contexts.)
+    static constexpr int PITCH = HDP * 2;
+    __device__ static __forceinline__ uint32_t at(int row, int chunk) {
+        return row * PITCH + ((chunk ^ (HDP == 96 ? (row >> 1) & 3 : row & 7)) << 4);
+    }
     static constexpr int TILE_BYTES = FL_TILE * PITCH;
     static constexpr int RING = FL_WARPS * STAGES * 2 * TILE_BYTES;
     static constexpr int HEADS = 8 * NT;
@@ -610,8 +614,11 @@ int flash_chunk(int group, int head_dim) {
 }  // namespace
 
 size_t paged_attn_workspace_bytes(int n_heads, int n_kv_heads, int head_dim) {
-    const int ctas = FL_MAX_SMS * (head_dim <= 64 ? FlashShape<64, 1>::CTAS : (head_dim <= 192 ? FlashShape<192, 1>::CTAS : FlashShape<256, 1>::CTAS));
-    return 8192 + 4 * (size_t)ctas * flash_slot_floats(flash_chunk(n_heads / n_kv_heads, head_dim), head_dim) * 4;
+    const int ctas = FL_MAX_SMS * (head_dim <= 64 ? FlashShape<64, 1>::CTAS : (head_dim <= 128 ? FlashShape<128, 1>::CTAS :
+                                   (head_dim <= 192 ? FlashShape<192, 1>::CTAS : FlashShape<256, 1>::CTAS)));
+    static_assert(FlashShape<96, 1>::CTAS == FlashShape<128, 1>::CTAS, "one formula for both");
+    static_assert(3 * FL_MAX_SMS * FlashShape<64, 1>::CTAS * 4 <= FL_COUNTER_BYTES, "counters");
+    return FL_COUNTER_BYTES + 4 * (size_t)ctas * flash_slot_floats(flash_chunk(n_heads / n_kv_heads, head_dim), head_dim) * 4;
 }
 
 int launch_paged_attn(const PagedView& c, const PagedAttnArgs& a, cudaStream_t st) {
@@ -638,7 +645,7 @@ int launch_paged_attn(const PagedView& c, const PagedAttnArgs& a, cudaStream_t s
     f.scale_log2 = a.scale * 1.4426950408889634f;
     f.out8 = (reinterpret_cast<uintptr_t>(a.out) & 7) == 0 && a.o_row % 4 == 0;
     f.counters = static_cast<unsigned int*>(a.work);
-    f.partial = reinterpret_cast<float*>(static_cast<char*>(a.work) + 8192);
+    f.partial = reinterpret_cast<float*>(static_cast<char*>(a.work) + FL_COUNTER_BYTES);
     if (p.head_dim <= 64) return f.chunk <= 8 ? launch_flash<64, 1>(f, st) : launch_flash<64, 2>(f, st);
     if (p.head_dim <= 96) return f.chunk <= 8 ? launch_flash<96, 1>(f, st) : launch_flash<96, 2>(f, st);
     if (p.head_dim <= 128) return f.chunk <= 8 ? launch_flash<128, 1>(f, st) : launch_flash<128, 2>(f, st);
