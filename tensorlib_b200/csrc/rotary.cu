@@ -7,8 +7,11 @@
 // The rotation itself is in 32 bits with one rounding to fp16.
 //
 // Bound: HBM at many tokens (every element is read and written once), launch and one dependent load chain
-// (position -> cos/sin -> store) at one token. One CTA a token: its cos/sin (rot/2 pairs) are computed once and shared by
-// all heads through shared memory.
+// (position -> cos/sin -> store) at one token. What has to be small for that is the number of instructions a vector: a form
+// that found token, head and element of every vector anew issued 190 of them and took 83 us for 16384 tokens of 40 heads of
+// 128, at 83% of the issue slots. So a thread keeps to one vector of the head and steps through (token, head) rows with
+// pointers that only grow; the cos/sin of a CTA's tokens are worked out once, for all heads, in shared memory, while the first
+// vectors arrive.
 #include "serving.cuh"
 
 namespace tlb {
@@ -16,23 +19,162 @@ namespace tlb {
 namespace {
 
 constexpr int ROT_THREADS = 256;
-constexpr int MAX_ROT_PAIRS = 512;
+// CTAs of an SM: what the registers of the rows under way allow. 16384 tokens of 40 heads of 128: 58 us interleaved with five
+// (64 with six, which spill), 58 us in halves with four (65 with five).
+constexpr int rot_ctas(bool half_layout) { return half_layout ? 4 : 5; }
+constexpr int ROT_ROWS = 16;                      // rows of a thread
+constexpr int ROT_MAX_GROUP = 64;                 // tokens of a CTA
+constexpr int ROT_MAX_PAIRS = 1024;               // their pairs in shared memory (one token has at most 512)
+
+// One of the tensors that a call moves: rows (token, head) of head_dim values.
+struct RotPlane {
+    const __half* in; __half* out;
+    long long in_token, in_head, out_token, out_head;      // out_token: only where rows do not go to pages
+    int heads;
+    bool turned, paged;                           // rotated; stored at the token's slot of the page
+    int heads_at_once, tokens_at_once;            // of a CTA
+    FastDiv by_heads_at_once;
+};
 
 struct RotLaunch {
     RotaryArgs a;
-    __half* kc; __half* vc; int* table;           // cache (kc == nullptr: none)
-    long long page_stride, token_stride, head_stride;
-    int n_kv, n_rows, max_pages, n_pages;
-    FastDiv by_page, by_items;
-    int items;                                    // work items of a head
+    RotPlane plane[3];
+    int planes;
+    const int* table;                             // of the cache, if there is one
+    long long page_stride, token_stride;
+    int n_rows, max_pages, n_pages;
+    bool paged;
+    FastDiv by_page, by_items, by_pairs;
+    int items, group, turn_stride;                // items of a head; tokens of a CTA; floats between a token's cos and sin
     int* status;
 };
 
-// VEC = 8: 16-byte items. Interleaved: one vector = four pairs. Half layout: one item = the vectors at i and i + rot/2.
-// VEC = 1: any alignment, one pair or one passed-through element an item.
-template <int VEC>
-__global__ void __launch_bounds__(ROT_THREADS) k_rotary(RotLaunch p) {
-    __shared__ float2 cs[MAX_ROT_PAIRS];
+// cos and sin of pair i at `pos`, times the magnitude
+__device__ __forceinline__ float2 turn_of(const RotaryArgs& a, int pos, int i) {
+    const double turns = (double)pos * (a.freqs[i] * 0.15915494309189533577);
+    const float frac = (float)(turns - rint(turns));
+    float s, c;
+    sincospif(2.f * frac, &s, &c);
+    return make_float2(c * a.magnitude, (a.inverse ? -s : s) * a.magnitude);
+}
+// where token t goes in its page, -1 if its row, position or page is not there
+__device__ __forceinline__ long long slot_of(const RotLaunch& p, int t, int pos) {
+    const int row = p.a.rows ? p.a.rows[t] : t;
+    const unsigned pg = p.by_page.div((unsigned)pos);
+    if (row >= 0 && row < p.n_rows && (int)pg < p.max_pages) {
+        const int page = p.table[(long long)row * p.max_pages + pg];
+        if (page >= 0 && page < p.n_pages) return page * p.page_stride + (long long)((unsigned)pos - pg * p.by_page.d) * p.token_stride;
+    }
+    atomicExch(p.status, TL_ERR_INVALID_ARGUMENT);
+    return -1;
+}
+
+template <int VEC> struct HalfVec;
+template <> struct HalfVec<8> { using T = uint4; };
+template <> struct HalfVec<4> { using T = uint2; };
+template <> struct HalfVec<2> { using T = unsigned; };
+
+// Items of VEC values. Interleaved pairs: an item is a vector, VEC / 2 pairs. Half layout: an item is the vectors at i and
+// i + rot / 2, VEC pairs; behind rot, one vector.
+template <int VEC, bool HALF>
+__global__ void __launch_bounds__(ROT_THREADS, rot_ctas(HALF)) k_rotary(RotLaunch p) {
+    using V = typename HalfVec<VEC>::T;
+    constexpr int PAIRS = HALF ? VEC : VEC / 2;   // of an item
+    extern __shared__ __align__(16) float turns[];             // [group]: cos [stride], sin [stride]
+    __shared__ long long slots[ROT_MAX_GROUP];    // where the token goes in its page, -1: nowhere
+    __shared__ int live[ROT_MAX_GROUP];           // 0: padding
+    pdl_launch_dependents();
+    pdl_wait();
+    const RotaryArgs& a = p.a;
+    const int pairs = a.rot / 2, stride = p.turn_stride, t0 = blockIdx.x * p.group, n_tokens = min(p.group, a.tokens - t0);
+    unsigned r, item;
+    p.by_items.divmod(threadIdx.x, r, item);
+    const bool pair = HALF && (int)item < pairs / VEC, mine = HALF ? pair : (int)item * VEC < a.rot;
+    const int d = !HALF || pair ? (int)item * VEC : a.rot + ((int)item - pairs / VEC) * VEC;
+    // all planes one after the other, or (few tokens) one a CTA
+    const int first = gridDim.y > 1 ? blockIdx.y : 0, end = gridDim.y > 1 ? first + 1 : p.planes;
+    constexpr int U = HALF ? 2 : 4;               // rows under way a thread
+    V x[U], y[U];
+    bool ready = false;
+    for (int w = first; w < end; w++) {
+        const int heads = p.plane[w].heads, at_once = p.plane[w].heads_at_once, tokens_at_once = p.plane[w].tokens_at_once;
+        const bool paged = p.plane[w].paged, turn = p.plane[w].turned && mine;
+        const long long in_step = (long long)at_once * p.plane[w].in_head, out_step = (long long)at_once * p.plane[w].out_head;
+        unsigned tt, h0;
+        p.plane[w].by_heads_at_once.divmod(r, tt, h0);
+        const int left = (int)tt < tokens_at_once ? heads - (int)h0 : 0;       // rows of a token: 0, at_once, .. below this
+        const __half* in_token = p.plane[w].in + (long long)(t0 + (int)tt) * p.plane[w].in_token + h0 * p.plane[w].in_head + d;
+        const long long in_next = tokens_at_once * p.plane[w].in_token;
+        __half* const out0 = p.plane[w].out + h0 * p.plane[w].out_head + d;
+        const long long out_token = p.plane[w].out_token;
+        for (int t = (int)tt;; t += tokens_at_once) {
+            const __half* in = in_token;
+            int h = 0;
+            do {
+#pragma unroll
+                for (int u = 0; u < U; u++)
+                    if (t < n_tokens && h + u * at_once < left) {
+                        x[u] = *reinterpret_cast<const V*>(in + u * in_step);
+                        if (pair) y[u] = *reinterpret_cast<const V*>(in + u * in_step + pairs);
+                    }
+                if (!ready) {                     // the turns and places of the CTA's tokens, while the first rows arrive
+                    for (int j = threadIdx.x; j < n_tokens; j += ROT_THREADS) {
+                        const int pos = a.positions[t0 + j];
+                        live[j] = pos >= 0;
+                        slots[j] = p.paged && pos >= 0 ? slot_of(p, t0 + j, pos) : -1;
+                    }
+                    const int todo = p.plane[first].turned ? n_tokens * pairs : 0;      // (values alone need no turns)
+                    for (int j = threadIdx.x; j < todo; j += ROT_THREADS) {
+                        unsigned k, i;
+                        p.by_pairs.divmod((unsigned)j, k, i);
+                        const float2 c = turn_of(a, a.positions[t0 + (int)k], (int)i);
+                        turns[k * 2 * stride + i] = c.x;
+                        turns[(k * 2 + 1) * stride + i] = c.y;
+                    }
+                    __syncthreads();
+                    ready = true;
+                }
+                if (t >= n_tokens || left <= 0) break;
+                const long long at = paged ? slots[t] : (long long)(t0 + t) * out_token;
+                if (live[t] && at >= 0) {
+                    __half* out = out0 + at + (h == 0 ? 0 : (long long)(h / at_once) * out_step);
+                    const float* c = turns + t * 2 * stride + (HALF ? d : d / 2);
+#pragma unroll
+                    for (int u = 0; u < U; u++) {
+                        if (h + u * at_once >= left) continue;
+                        if (turn) {
+                            __half2* xh = reinterpret_cast<__half2*>(&x[u]);
+                            __half2* yh = reinterpret_cast<__half2*>(&y[u]);
+#pragma unroll
+                            for (int j = 0; j < VEC / 2; j++) {
+                                const float2 f = __half22float2(xh[j]);
+                                if (HALF) {
+                                    const float2 g = __half22float2(yh[j]);
+                                    const float2 co = *reinterpret_cast<const float2*>(c + 2 * j), si = *reinterpret_cast<const float2*>(c + stride + 2 * j);
+                                    xh[j] = __floats2half2_rn(f.x * co.x - g.x * si.x, f.y * co.y - g.y * si.y);
+                                    yh[j] = __floats2half2_rn(f.x * si.x + g.x * co.x, f.y * si.y + g.y * co.y);
+                                } else {
+                                    const float co = c[j], si = c[stride + j];
+                                    xh[j] = __floats2half2_rn(f.x * co - f.y * si, f.x * si + f.y * co);
+                                }
+                            }
+                        }
+                        *reinterpret_cast<V*>(out + u * out_step) = x[u];
+                        if (pair) *reinterpret_cast<V*>(out + u * out_step + pairs) = y[u];
+                    }
+                }
+                in += U * in_step;
+                h += U * at_once;
+            } while (h < left);
+            if (t >= n_tokens || left <= 0) break;
+            in_token += in_next;
+        }
+    }
+}
+
+// Any alignment: one pair or one passed-through element an item, one token a CTA.
+__global__ void __launch_bounds__(ROT_THREADS) k_rotary_any(RotLaunch p) {
+    extern __shared__ float2 cs[];
     __shared__ long long slot_sh;
     pdl_launch_dependents();
     pdl_wait();
@@ -42,86 +184,22 @@ __global__ void __launch_bounds__(ROT_THREADS) k_rotary(RotLaunch p) {
         const int pos = a.positions[t];
         __syncthreads();
         if (pos < 0) continue;                    // padding: nothing is written
-        for (int i = threadIdx.x; i < pairs; i += ROT_THREADS) {
-            const double turns = (double)pos * (a.freqs[i] * 0.15915494309189533577);
-            const float frac = (float)(turns - rint(turns));
-            float s, c;
-            sincospif(2.f * frac, &s, &c);
-            cs[i] = make_float2(c * a.magnitude, (a.inverse ? -s : s) * a.magnitude);
-        }
-        if (threadIdx.x == 0 && p.kc) {
-            const int row = a.rows ? a.rows[t] : t;
-            const unsigned pg = p.by_page.div((unsigned)pos);
-            long long slot = -1;
-            if (row >= 0 && row < p.n_rows && (int)pg < p.max_pages) {
-                const int page = p.table[(long long)row * p.max_pages + pg];
-                if (page >= 0 && page < p.n_pages)
-                    slot = page * p.page_stride + (long long)((unsigned)pos - pg * p.by_page.d) * p.token_stride;
-            }
-            if (slot < 0) atomicExch(p.status, TL_ERR_INVALID_ARGUMENT);
-            slot_sh = slot;
-        }
+        for (int i = threadIdx.x; i < pairs; i += ROT_THREADS) cs[i] = turn_of(a, pos, i);
+        if (threadIdx.x == 0 && p.paged) slot_sh = slot_of(p, t, pos);
         __syncthreads();
-        const long long slot = p.kc ? slot_sh : -1;
-        const int heads = a.n_heads + (slot >= 0 ? 2 * p.n_kv : 0);
-        for (int w = threadIdx.x; w < heads * p.items; w += ROT_THREADS) {
-            unsigned h, i;
-            p.by_items.divmod((unsigned)w, h, i);
-            const __half* in;
-            __half* out;
-            bool rotate = true;
-            if ((int)h < a.n_heads) {
-                in = a.q + t * a.q_token + h * a.q_head;
-                out = a.q_out + t * a.qo_token + h * a.qo_head;
-            } else if ((int)h < a.n_heads + p.n_kv) {
-                in = a.k + t * a.kv_token + (long long)(h - a.n_heads) * a.head_dim;
-                out = p.kc + slot + (long long)(h - a.n_heads) * p.head_stride;
-            } else {
-                in = a.v + t * a.kv_token + (long long)(h - a.n_heads - p.n_kv) * a.head_dim;
-                out = p.vc + slot + (long long)(h - a.n_heads - p.n_kv) * p.head_stride;
-                rotate = false;
-            }
-            if constexpr (VEC == 8) {
-                if (a.half_layout && (int)i < a.rot / 16) {
-                    const int d = (int)i * 8;
-                    const uint4 x = *reinterpret_cast<const uint4*>(in + d), y = *reinterpret_cast<const uint4*>(in + d + pairs);
-                    uint4 xo = x, yo = y;
-                    if (rotate) {
-                        const __half2* xh = reinterpret_cast<const __half2*>(&x);
-                        const __half2* yh = reinterpret_cast<const __half2*>(&y);
-                        __half2* xq = reinterpret_cast<__half2*>(&xo);
-                        __half2* yq = reinterpret_cast<__half2*>(&yo);
-#pragma unroll
-                        for (int j = 0; j < 4; j++) {
-                            const float2 u = __half22float2(xh[j]), v = __half22float2(yh[j]);
-                            const float2 c0 = cs[d + 2 * j], c1 = cs[d + 2 * j + 1];
-                            xq[j] = __floats2half2_rn(u.x * c0.x - v.x * c0.y, u.y * c1.x - v.y * c1.y);
-                            yq[j] = __floats2half2_rn(u.x * c0.y + v.x * c0.x, u.y * c1.y + v.y * c1.x);
-                        }
-                    }
-                    *reinterpret_cast<uint4*>(out + d) = xo;
-                    *reinterpret_cast<uint4*>(out + d + pairs) = yo;
-                } else {
-                    const int d = a.half_layout ? a.rot + ((int)i - a.rot / 16) * 8 : (int)i * 8;
-                    const uint4 x = *reinterpret_cast<const uint4*>(in + d);
-                    uint4 xo = x;
-                    if (rotate && d < a.rot) {
-                        const __half2* xh = reinterpret_cast<const __half2*>(&x);
-                        __half2* xq = reinterpret_cast<__half2*>(&xo);
-#pragma unroll
-                        for (int j = 0; j < 4; j++) {
-                            const float2 u = __half22float2(xh[j]);
-                            const float2 c = cs[d / 2 + j];
-                            xq[j] = __floats2half2_rn(u.x * c.x - u.y * c.y, u.x * c.y + u.y * c.x);
-                        }
-                    }
-                    *reinterpret_cast<uint4*>(out + d) = xo;
-                }
-            } else {
+        const long long slot = p.paged ? slot_sh : -1;
+        for (int w = 0; w < p.planes; w++) {
+            const RotPlane& q = p.plane[w];
+            if (q.paged && slot < 0) continue;
+            for (int k = threadIdx.x; k < q.heads * p.items; k += ROT_THREADS) {
+                unsigned h, i;
+                p.by_items.divmod((unsigned)k, h, i);
+                const __half* in = q.in + t * q.in_token + h * q.in_head;
+                __half* out = q.out + (q.paged ? slot : t * q.out_token) + h * q.out_head;
                 if ((int)i < pairs) {
                     const int d0 = a.half_layout ? (int)i : 2 * (int)i, d1 = a.half_layout ? (int)i + pairs : 2 * (int)i + 1;
                     const __half xh = in[d0], yh = in[d1];
-                    if (rotate) {
+                    if (q.turned) {
                         const float x = __half2float(xh), y = __half2float(yh);
                         const float2 c = cs[i];
                         out[d0] = __float2half_rn(x * c.x - y * c.y);
@@ -139,6 +217,12 @@ __global__ void __launch_bounds__(ROT_THREADS) k_rotary(RotLaunch p) {
     }
 }
 
+template <int VEC>
+int launch_vec(const RotLaunch& p, dim3 grid, size_t smem, cudaStream_t st) {
+    return p.a.half_layout ? launch_pdl(k_rotary<VEC, true>, grid, ROT_THREADS, smem, st, true, p)
+                           : launch_pdl(k_rotary<VEC, false>, grid, ROT_THREADS, smem, st, true, p);
+}
+
 }  // namespace
 
 int launch_rotary(const RotaryArgs& a, const PagedView* cache, cudaStream_t st) {
@@ -146,23 +230,61 @@ int launch_rotary(const RotaryArgs& a, const PagedView* cache, cudaStream_t st) 
     RotLaunch p{};
     p.a = a;
     p.status = device_status_word();
-    auto on16 = [](const void* x) { return (reinterpret_cast<uintptr_t>(x) & 15) == 0; };
-    bool vec = a.head_dim % 8 == 0 && a.rot % 8 == 0 && (!a.half_layout || a.rot % 16 == 0);
     if (a.n_heads > 0)
-        vec = vec && on16(a.q) && on16(a.q_out) && a.q_token % 8 == 0 && a.q_head % 8 == 0 && a.qo_token % 8 == 0 && a.qo_head % 8 == 0;
+        p.plane[p.planes++] = RotPlane{a.q, a.q_out, a.q_token, a.q_head, a.qo_token, a.qo_head, a.n_heads, true, false};
     if (cache) {
-        p.kc = cache->k; p.vc = cache->v; p.table = cache->table;
-        p.page_stride = cache->page_stride; p.token_stride = cache->token_stride; p.head_stride = cache->head_stride;
-        p.n_kv = cache->n_kv_heads; p.n_rows = cache->n_rows; p.max_pages = cache->max_pages; p.n_pages = cache->n_pages;
-        p.by_page = cache->by_page;
-        vec = vec && cache->aligned16() && on16(a.k) && on16(a.v) && a.kv_token % 8 == 0;
+        p.paged = true;
+        p.table = cache->table; p.page_stride = cache->page_stride; p.token_stride = cache->token_stride;
+        p.n_rows = cache->n_rows; p.max_pages = cache->max_pages; p.n_pages = cache->n_pages; p.by_page = cache->by_page;
+        p.plane[p.planes++] = RotPlane{a.k, cache->k, a.kv_token, a.head_dim, 0, cache->head_stride, cache->n_kv_heads, true, true};
+        p.plane[p.planes++] = RotPlane{a.v, cache->v, a.kv_token, a.head_dim, 0, cache->head_stride, cache->n_kv_heads, false, true};
     }
-    if (vec) p.items = a.half_layout ? a.rot / 16 + (a.head_dim - a.rot) / 8 : a.head_dim / 8;
-    else p.items = a.rot / 2 + (a.head_dim - a.rot);
+    // the widest vectors that every row, the rotated part and its halves allow
+    const int pairs = a.rot / 2;
+    auto fits = [&](int vec) {
+        auto on = [&](const void* x) { return reinterpret_cast<uintptr_t>(x) % (2 * vec) == 0; };
+        bool ok = a.head_dim % vec == 0 && (a.half_layout ? pairs : a.rot) % vec == 0;
+        if (cache) ok = ok && cache->page_stride % vec == 0 && cache->token_stride % vec == 0;
+        for (int w = 0; w < p.planes; w++) {
+            const RotPlane& q = p.plane[w];
+            ok = ok && on(q.in) && on(q.out) && q.in_token % vec == 0 && q.in_head % vec == 0 && q.out_token % vec == 0 && q.out_head % vec == 0;
+        }
+        return ok;
+    };
+    int vec = fits(8) ? 8 : (fits(4) ? 4 : (fits(2) ? 2 : 1));
+    if (vec > 1) {
+        p.items = (a.half_layout ? pairs : a.rot) / vec + (a.head_dim - a.rot) / vec;
+        if (p.items > ROT_THREADS) vec = 1;       // a thread keeps to an item of the head
+    }
+    if (vec == 1) {
+        p.items = pairs + (a.head_dim - a.rot);
+        p.by_items = FastDiv((unsigned)p.items);
+        return launch_pdl(k_rotary_any, a.tokens < 148 * 64 ? a.tokens : 148 * 64, ROT_THREADS, (size_t)pairs * 8, st, true, p);
+    }
     p.by_items = FastDiv((unsigned)p.items);
-    const int grid = a.tokens < 148 * 64 ? a.tokens : 148 * 64;
-    return vec ? launch_pdl(k_rotary<8>, grid, ROT_THREADS, 0, st, true, p)
-               : launch_pdl(k_rotary<1>, grid, ROT_THREADS, 0, st, true, p);
+    p.by_pairs = FastDiv((unsigned)(pairs > 0 ? pairs : 1));
+    const int rows = ROT_THREADS / p.items;
+    int heads = 0;
+    for (int w = 0; w < p.planes; w++) {
+        RotPlane& q = p.plane[w];
+        q.heads_at_once = rows < q.heads ? rows : q.heads;
+        q.tokens_at_once = rows / q.heads_at_once;
+        q.by_heads_at_once = FastDiv((unsigned)q.heads_at_once);
+        heads += q.heads;
+    }
+    // Tokens a CTA: enough that setting up a tensor is small against moving its rows (about ROT_ROWS a thread), and so that the
+    // CTAs make whole rounds of those that are resident. Where a token is a CTA, so is each tensor of it.
+    const long long resident = (long long)rot_ctas(a.half_layout != 0) * sm_count();
+    long long most = (long long)ROT_ROWS * rows / heads;
+    if (pairs > 0 && most > ROT_MAX_PAIRS / pairs) most = ROT_MAX_PAIRS / pairs;
+    if (most > ROT_MAX_GROUP) most = ROT_MAX_GROUP;
+    if (most < 1) most = 1;
+    const long long rounds = (a.tokens + most * resident - 1) / (most * resident);
+    p.group = (int)((a.tokens + rounds * resident - 1) / (rounds * resident));
+    p.turn_stride = (pairs + 3) / 4 * 4;
+    const dim3 grid((unsigned)((a.tokens + p.group - 1) / p.group), p.group == 1 ? p.planes : 1);
+    const size_t smem = (size_t)p.group * p.turn_stride * 8;
+    return vec == 8 ? launch_vec<8>(p, grid, smem, st) : (vec == 4 ? launch_vec<4>(p, grid, smem, st) : launch_vec<2>(p, grid, smem, st));
 }
 
 }  // namespace tlb
