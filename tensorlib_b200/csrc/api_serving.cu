@@ -28,6 +28,7 @@ int check_cache(const tl_paged_cache* c, bool pools, const char* who) {
         TL_REQUIRE(c->page_stride > 0 && c->token_stride > 0 && c->head_stride > 0 && (c->n_layers == 1 || c->layer_stride > 0),
                    "%s: cache strides must be positive", who);
         TL_REQUIRE((long long)c->page_size * c->n_kv_heads * c->head_dim < (1ll << 31), "%s: a page of more than 2^31 - 1 values", who);
+        TL_REQUIRE(2ll * c->n_layers * ((long long)c->n_pages + c->n_rows) < (1ll << 31), "%s: more than 2^31 - 1 pages over all layers", who);
     }
     return TL_OK;
 }
@@ -188,7 +189,7 @@ int tl_paged_reserve_f16(const tl_paged_cache* cache, const int* new_tokens, int
 
 int tl_paged_copy_f16(const tl_paged_cache* cache, const int* src, const int* dst, int n, tl_stream stream) {
     TL_PROPAGATE(check_cache(cache, true, "paged_copy"));
-    TL_REQUIRE(n >= 0 && (n == 0 || (src && dst)), "paged_copy: bad arguments");
+    TL_REQUIRE(n >= 0 && (n == 0 || (src && dst)) && 2ll * n * cache->n_layers < (1ll << 31), "paged_copy: bad arguments");
     TL_ON_LIBRARY_DEVICE();
     return launch_paged_copy(PagedView(*cache), src, dst, n, as_stream(stream));
 }

@@ -16,30 +16,38 @@ namespace {
 // columns of ALL rows in shared memory needs no other CTA and no second launch. Entries that stay the same are skipped.
 // The last CTA does the same with the lengths. Counts change by atomic additions of whole numbers: any order, same result.
 constexpr int FORK_THREADS = 256;
+constexpr int FORK_SMEM = 196608;
 
+template <int SLAB>
 __global__ void __launch_bounds__(FORK_THREADS) k_fork(int* table, int* lengths, int* refs, const int* parents, int n_rows,
-                                                       int max_pages, int n_pages, int slab, int* status) {
+                                                       int max_pages, int n_pages, int* status) {
     extern __shared__ int sm[];
     pdl_launch_dependents();
     pdl_wait();
-    const bool is_len = blockIdx.x == gridDim.x - 1;
-    const int c0 = is_len ? 0 : blockIdx.x * slab;
-    const int w = is_len ? 1 : min(slab, max_pages - c0);
-    int* base = is_len ? lengths : table + c0;
-    const long long pitch = is_len ? 1 : max_pages;
-    for (int i = threadIdx.x; i < n_rows * w; i += FORK_THREADS) sm[i] = base[(i / w) * pitch + i % w];
-    __syncthreads();
-    for (int i = threadIdx.x; i < n_rows * w; i += FORK_THREADS) {
-        const int r = i / w, j = i % w;
-        const int parent = parents[r];
-        if (parent >= n_rows || parent < -1) {    // not a row: this one stays as it is
-            atomicExch(status, TL_ERR_INVALID_ARGUMENT);
-            continue;
+    if (blockIdx.x == gridDim.x - 1) {            // the lengths
+        for (int r = threadIdx.x; r < n_rows; r += FORK_THREADS) sm[r] = lengths[r];
+        __syncthreads();
+        for (int r = threadIdx.x; r < n_rows; r += FORK_THREADS) {
+            const int parent = parents[r];
+            if (parent >= n_rows || parent < -1) atomicExch(status, TL_ERR_INVALID_ARGUMENT);
+            else if (parent != r) lengths[r] = parent < 0 ? 0 : sm[parent];
         }
-        const int o = sm[i], n = parent < 0 ? (is_len ? 0 : -1) : sm[parent * w + j];
+        return;
+    }
+    const int c0 = blockIdx.x * SLAB;
+    int* base = table + c0;
+    for (int i = threadIdx.x; i < n_rows * SLAB; i += FORK_THREADS) {
+        const int r = i / SLAB, j = i % SLAB;
+        sm[i] = c0 + j < max_pages ? base[(long long)r * max_pages + j] : -1;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < n_rows * SLAB; i += FORK_THREADS) {
+        const int r = i / SLAB, j = i % SLAB;
+        const int parent = parents[r];
+        if (parent >= n_rows || parent < -1) continue;         // not a row: this one stays as it is
+        const int o = sm[i], n = parent < 0 ? -1 : sm[parent * SLAB + j];
         if (o == n) continue;
-        base[r * pitch + j] = n;
-        if (is_len) continue;
+        base[(long long)r * max_pages + j] = n;
         if (n >= 0 && n < n_pages) atomicAdd(refs + n, 1);
         if (o >= 0 && o < n_pages) atomicSub(refs + o, 1);
         if (n >= n_pages || o >= n_pages || n < -1 || o < -1) atomicExch(status, TL_ERR_INVALID_ARGUMENT);
@@ -72,40 +80,35 @@ PageShape page_shape(const PagedView& c) {
     return s;
 }
 
-template <typename V>
-__device__ __forceinline__ void copy_run(__half* dst, const __half* src, long long n, int tid, int threads) {
-    const V* s = reinterpret_cast<const V*>(src);
-    V* d = reinterpret_cast<V*>(dst);
-    constexpr int U = 8;           // loads in flight a thread
-    long long i = tid;
-    for (; i + (U - 1) * threads < n; i += U * threads) {
+// n vectors by THREADS threads, eight loads under way each
+template <typename V, int THREADS>
+__device__ __forceinline__ void copy_run(__half* dst, const __half* src, int n, int tid) {
+    const V* s = reinterpret_cast<const V*>(src) + tid;
+    V* d = reinterpret_cast<V*>(dst) + tid;
+    constexpr int U = 8;
+    for (int left = n - tid; left > 0; left -= U * THREADS, s += U * THREADS, d += U * THREADS) {
         V x[U];
 #pragma unroll
-        for (int u = 0; u < U; u++) x[u] = s[i + u * threads];
+        for (int u = 0; u < U; u++)
+            if (u * THREADS < left) x[u] = s[u * THREADS];
 #pragma unroll
-        for (int u = 0; u < U; u++) d[i + u * threads] = x[u];
+        for (int u = 0; u < U; u++)
+            if (u * THREADS < left) d[u * THREADS] = x[u];
     }
-    for (; i < n; i += threads) d[i] = s[i];
 }
 
-template <typename V>
-__device__ __forceinline__ void copy_page(const PageShape& s, __half* dst, const __half* src, int n, int tid, int threads) {
+template <typename V, int THREADS>
+__device__ __forceinline__ void copy_page(const PageShape& s, __half* dst, const __half* src, int n, int tid) {
     constexpr int VEC = sizeof(V) / sizeof(__half);
-    if (s.kind == 0) {
-        copy_run<V>(dst, src, (long long)n * s.heads * s.dim / VEC, tid, threads);
-        return;
-    }
-    if (s.kind == 1 && n == s.page_size && s.head_stride == (long long)n * s.dim) {
-        copy_run<V>(dst, src, (long long)n * s.heads * s.dim / VEC, tid, threads);
-        return;
-    }
-    if (s.kind == 1) {
-        for (int h = 0; h < s.heads; h++)
-            copy_run<V>(dst + h * s.head_stride, src + h * s.head_stride, (long long)n * s.dim / VEC, tid, threads);
+    if (s.kind <= 1) {
+        const bool by_head = s.kind == 1 && !(n == s.page_size && s.head_stride == (long long)n * s.dim);
+        const int len = n * s.dim / VEC * (by_head ? 1 : s.heads);
+        for (int run = 0; run < (by_head ? s.heads : 1); run++)
+            copy_run<V, THREADS>(dst + run * s.head_stride, src + run * s.head_stride, len, tid);
         return;
     }
     const unsigned total = (unsigned)n * (s.kind == 2 ? 1 : s.heads) * s.by_row.d;
-    for (unsigned i = tid; i < total; i += threads) {
+    for (unsigned i = tid; i < total; i += THREADS) {
         unsigned run, v, tok, h = 0;
         s.by_row.divmod(i, run, v);
         tok = run;
@@ -117,36 +120,47 @@ __device__ __forceinline__ void copy_page(const PageShape& s, __half* dst, const
 
 constexpr int COPY_THREADS = 256;
 
+// An item is one page of one layer of K or of V; TEAM threads copy it (a CTA, or where pages are small a warp).
 struct CopyArgs {
     __half* k; __half* v;
     long long layer_stride, page_stride;
-    int n_layers, n_pages;
+    int n_layers, n_pages, team;
     PageShape shape;
+    FastDiv by_each;                              // 2 n_layers items a page
     int* status;
 };
 
-__device__ __forceinline__ void copy_item(const CopyArgs& a, int what, int src, int dst, int tokens) {
+template <typename V, int TEAM>
+__device__ __forceinline__ void copy_item(const CopyArgs& a, unsigned what, int src, int dst, int tokens) {
     __half* pool = (what & 1) ? a.v : a.k;
     __half* layer = pool + (long long)(what >> 1) * a.layer_stride;
-    if (a.shape.vec == 8) copy_page<uint4>(a.shape, layer + dst * a.page_stride, layer + src * a.page_stride, tokens, threadIdx.x, COPY_THREADS);
-    else copy_page<__half>(a.shape, layer + dst * a.page_stride, layer + src * a.page_stride, tokens, threadIdx.x, COPY_THREADS);
+    copy_page<V, TEAM>(a.shape, layer + dst * a.page_stride, layer + src * a.page_stride, tokens, threadIdx.x % TEAM);
+}
+// f(page pair, what) for the items of n page pairs, below 2^31 in all
+template <int TEAM, typename Fn>
+__device__ __forceinline__ void each_item(const CopyArgs& a, int n, Fn&& f) {
+    constexpr unsigned TEAMS = COPY_THREADS / TEAM;
+    const unsigned total = (unsigned)n * a.by_each.d;
+    for (unsigned it = blockIdx.x * TEAMS + threadIdx.x / TEAM; it < total; it += gridDim.x * TEAMS) {
+        unsigned m, what;
+        a.by_each.divmod(it, m, what);
+        f((int)m, what);
+    }
 }
 
-// one item = one page of one layer of K or of V
-__global__ void __launch_bounds__(COPY_THREADS) k_copy_pages(CopyArgs a, const int* src, const int* dst, int n) {
+template <typename V, int TEAM>
+__global__ void __launch_bounds__(COPY_THREADS, 4) k_copy_pages(CopyArgs a, const int* src, const int* dst, int n) {
     pdl_launch_dependents();
     pdl_wait();
-    const int each = 2 * a.n_layers;
-    for (long long it = blockIdx.x; it < (long long)n * each; it += gridDim.x) {
-        const int m = (int)(it / each), what = (int)(it - (long long)m * each);
+    each_item<TEAM>(a, n, [&](int m, unsigned what) {
         const int s = src[m], d = dst[m];
-        if (s == d || s == -1) continue;
+        if (s == d || s == -1) return;
         if (s < 0 || d < 0 || s >= a.n_pages || d >= a.n_pages) {
-            if (threadIdx.x == 0) atomicExch(a.status, TL_ERR_INVALID_ARGUMENT);
-            continue;
+            atomicExch(a.status, TL_ERR_INVALID_ARGUMENT);
+            return;
         }
-        copy_item(a, what, s, d, a.shape.page_size);
-    }
+        copy_item<V, TEAM>(a, what, s, d, a.shape.page_size);
+    });
 }
 
 // ---- making room ---------------------------------------------------------------------------------------------------
@@ -180,78 +194,124 @@ __device__ __forceinline__ unsigned long long block_scan(unsigned long long v, u
     return before + x - v;
 }
 
-__global__ void __launch_bounds__(RES_THREADS) k_reserve(PagedView c, const int* new_tokens, int* result, ReserveWork wk, int* status) {
+__global__ void __launch_bounds__(RES_THREADS, 1) k_reserve(PagedView c, const int* new_tokens, int* result, ReserveWork wk, int* status) {
     __shared__ unsigned long long sums[RES_THREADS / 32];
     __shared__ int bad_sh;
     pdl_launch_dependents();
     pdl_wait();
     const int tid = threadIdx.x;
+    // Rows r0 .. r1 are this thread's; of the first one, where nearly always there is no other, everything stays in registers.
     const int per = (c.n_rows + RES_THREADS - 1) / RES_THREADS;
     const int r0 = min(c.n_rows, tid * per), r1 = min(c.n_rows, r0 + per);
+    constexpr int WRITES = 1 << 30, COPY = 1 << 29;
+    struct Row { int len, add, pages, slot, last, flag; };     // pages that it holds, slots used of the last one, its id
+    auto read = [&](int r) {
+        Row x;
+        x.len = c.lengths[r];
+        x.add = new_tokens[r];
+        if (x.len < 0) x.len = -1;
+        const unsigned whole = x.len < 0 ? 0u : c.by_page.div((unsigned)x.len);
+        x.slot = x.len < 0 ? 0 : (int)((unsigned)x.len - whole * c.by_page.d);
+        x.pages = (int)whole + (x.slot != 0);
+        x.last = -1;
+        x.flag = 0;
+        return x;
+    };
+    auto again = [&](int r) {                     // a row beyond the first, with what was found out about it
+        Row x = read(r);
+        x.flag = wk.need[r];
+        if (x.flag & WRITES) x.last = __ldcg(c.table + (long long)r * c.max_pages + x.pages - 1);
+        return x;
+    };
+    Row mine{};
+    if (r0 < r1) mine = read(r0);
+    // the free pages among the first 4 RES_THREADS ones, as they are before any count changes
+    unsigned free4 = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const int pg = tid * 4 + i;
+        if (pg < c.n_pages && __ldcg(c.refs + pg) == 0) free4 |= 1u << i;
+    }
     if (tid == 0) bad_sh = 0;
     __syncthreads();
-    auto last_page = [&](int r, int len) { return __ldcg(c.table + (long long)r * c.max_pages + len / c.page_size); };
     // 1: every row that writes into a page that is there lets go of it
-    constexpr int NONE = 0, WRITES = 1 << 30, COPY = 1 << 29;
-    for (int r = r0; r < r1; r++) {
-        const int len = c.lengths[r], add = new_tokens[r];
-        int flag = NONE;
-        if (len < 0 || add < 0 || (long long)len + add > (long long)c.max_pages * c.page_size) {
-            atomicMax(&bad_sh, add < 0 || len < 0 ? 2 : 1);
-        } else if (add > 0 && len % c.page_size != 0) {
-            const int page = last_page(r, len);
-            if (page < 0 || page >= c.n_pages) atomicMax(&bad_sh, 2);
-            else {
-                if (atomicSub(c.refs + page, 1) <= 0) atomicMax(&bad_sh, 2);
-                flag = WRITES;
-            }
-        }
-        wk.need[r] = flag;
+    auto let_go = [&](int r, Row& x) {
+        if (x.len < 0 || x.add < 0) { atomicMax(&bad_sh, 2); return; }
+        if ((long long)x.len + x.add > (long long)c.max_pages * c.page_size) { atomicMax(&bad_sh, 1); return; }
+        if (x.add == 0 || x.slot == 0) return;
+        x.last = __ldcg(c.table + (long long)r * c.max_pages + x.pages - 1);
+        if (x.last < 0 || x.last >= c.n_pages) { atomicMax(&bad_sh, 2); return; }
+        if (atomicSub(c.refs + x.last, 1) <= 0) atomicMax(&bad_sh, 2);
+        x.flag = WRITES;
+    };
+    if (r0 < r1) let_go(r0, mine);
+    for (int r = r0 + 1; r < r1; r++) {
+        Row x = read(r);
+        let_go(r, x);
+        wk.need[r] = x.flag;
     }
     __syncthreads();
     // 2: a page that nobody holds any more goes to the highest of the rows that let go of it: its count becomes -(row + 1)
-    for (int r = r0; r < r1; r++)
-        if (wk.need[r] & WRITES) {
-            int* ref = c.refs + last_page(r, c.lengths[r]);
-            if (__ldcg(ref) <= 0) atomicMin(ref, -(r + 1));
-        }
+    auto claim = [&](int r, const Row& x) {
+        if ((x.flag & WRITES) && __ldcg(c.refs + x.last) <= 0) atomicMin(c.refs + x.last, -(r + 1));
+    };
+    if (r0 < r1) claim(r0, mine);
+    for (int r = r0 + 1; r < r1; r++) claim(r, again(r));
     __syncthreads();
-    unsigned long long mine = 0;                  // copies in the upper half, pages in the lower
-    for (int r = r0; r < r1; r++) {
-        const int len = c.lengths[r], add = new_tokens[r];
-        int flag = wk.need[r];
-        if (flag & WRITES) {
-            if (__ldcg(c.refs + last_page(r, len)) != -(r + 1)) {
-                flag |= COPY;
-                mine += (1ull << 32) + 1;
-            }
-            wk.need[r] = flag;
+    unsigned long long wants = 0;                 // copies in the upper half, pages in the lower
+    auto count = [&](int r, Row& x) {
+        if ((x.flag & WRITES) && __ldcg(c.refs + x.last) != -(r + 1)) {
+            x.flag |= COPY;
+            wants += (1ull << 32) + 1;
         }
-        if (add > 0 && len >= 0)
-            mine += (unsigned)(((long long)len + add + c.page_size - 1) / c.page_size - ((long long)len + c.page_size - 1) / c.page_size);
+        if (x.add > 0 && x.len >= 0 && (long long)x.len + x.add <= (long long)c.max_pages * c.page_size)
+            wants += (unsigned)((int)c.by_page.div((unsigned)(x.len + x.add - 1)) + 1 - x.pages);
+    };
+    if (r0 < r1) count(r0, mine);
+    for (int r = r0 + 1; r < r1; r++) {
+        Row x = again(r);
+        count(r, x);
+        wk.need[r] = x.flag;
     }
-    __syncthreads();
-    // 3: the keepers' counts are 1 again
-    for (int r = r0; r < r1; r++)
-        if ((wk.need[r] & (WRITES | COPY)) == WRITES) atomicExch(c.refs + last_page(r, c.lengths[r]), 1);
+    // 3: the keepers' counts are 1 again (after the barrier in the sum: everyone has looked)
     unsigned long long total;
-    const unsigned long long before = block_scan(mine, sums, total);
+    const unsigned long long before = block_scan(wants, sums, total);
     const int pages_wanted = (int)(total & 0xffffffffu);
+    auto keep = [&](const Row& x) {
+        if ((x.flag & (WRITES | COPY)) == WRITES) atomicExch(c.refs + x.last, 1);
+    };
+    if (r0 < r1) keep(mine);
+    for (int r = r0 + 1; r < r1; r++) keep(again(r));
     __syncthreads();
     // 4: the lowest free pages, ascending
+    const int bad = bad_sh;
     int found = 0;
-    for (int p0 = 0; p0 < c.n_pages && found < pages_wanted && bad_sh == 0; p0 += RES_THREADS) {
-        const int p = p0 + tid;
-        const bool is_free = p < c.n_pages && __ldcg(c.refs + p) == 0;
+    for (int p0 = 0; p0 < c.n_pages && found < pages_wanted && bad == 0; p0 += 4 * RES_THREADS) {
+        unsigned mask = free4;
+        if (p0 > 0) {
+            mask = 0;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int pg = p0 + tid * 4 + i;
+                if (pg < c.n_pages && __ldcg(c.refs + pg) == 0) mask |= 1u << i;
+            }
+        }
         unsigned long long here;
-        const int at = found + (int)block_scan(is_free, sums, here);
-        if (is_free && at < pages_wanted) wk.freed[at] = p;
+        int at = found + (int)block_scan((unsigned long long)__popc(mask), sums, here);
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (mask >> i & 1u) {
+                if (at < pages_wanted) wk.freed[at] = p0 + tid * 4 + i;
+                at++;
+            }
         found += (int)here;
     }
-    const int bad = bad_sh;
     if (bad || found < pages_wanted) {            // refused: the counts as they were, nothing else has changed
-        for (int r = r0; r < r1; r++)
-            if (wk.need[r] & COPY) atomicAdd(c.refs + last_page(r, c.lengths[r]), 1);
+        if (r0 < r1 && (mine.flag & COPY)) atomicAdd(c.refs + mine.last, 1);
+        for (int r = r0 + 1; r < r1; r++) {
+            const Row x = again(r);
+            if (x.flag & COPY) atomicAdd(c.refs + x.last, 1);
+        }
         if (tid == 0) {
             *result = bad == 2 ? TL_ERR_INVALID_ARGUMENT : TL_ERR_OUT_OF_MEMORY;
             *wk.n_copies = 0;
@@ -262,24 +322,25 @@ __global__ void __launch_bounds__(RES_THREADS) k_reserve(PagedView c, const int*
     __syncthreads();
     // 5: hand them out, rows in order: a row's copy first, then its new pages
     int at = (int)(before & 0xffffffffu), copy_at = (int)(before >> 32);
-    for (int r = r0; r < r1; r++) {
-        const int len = c.lengths[r], add = new_tokens[r];
-        if (add <= 0) continue;
+    auto hand_out = [&](int r, const Row& x) {
+        if (x.add <= 0) return;
         int* row = c.table + (long long)r * c.max_pages;
-        if (wk.need[r] & COPY) {
+        if (x.flag & COPY) {
             const int dst = __ldcg(wk.freed + at++);
-            wk.copies[copy_at++] = CowItem{row[len / c.page_size], dst, len % c.page_size, 0};
-            row[len / c.page_size] = dst;
+            wk.copies[copy_at++] = CowItem{x.last, dst, x.slot, 0};
+            row[x.pages - 1] = dst;
             c.refs[dst] = 1;
         }
-        const int p1 = (int)(((long long)len + add + c.page_size - 1) / c.page_size);
-        for (int p = (int)(((long long)len + c.page_size - 1) / c.page_size); p < p1; p++) {
+        const int end = (int)c.by_page.div((unsigned)(x.len + x.add - 1)) + 1;
+        for (int pg = x.pages; pg < end; pg++) {
             const int dst = __ldcg(wk.freed + at++);
-            row[p] = dst;
+            row[pg] = dst;
             c.refs[dst] = 1;
         }
-        c.lengths[r] = len + add;
-    }
+        c.lengths[r] = x.len + x.add;
+    };
+    if (r0 < r1) hand_out(r0, mine);
+    for (int r = r0 + 1; r < r1; r++) hand_out(r, again(r));
     if (tid == 0) {
         *result = TL_OK;
         *wk.n_copies = (int)(total >> 32);
@@ -287,16 +348,14 @@ __global__ void __launch_bounds__(RES_THREADS) k_reserve(PagedView c, const int*
 }
 
 // the filled tokens of the shared pages that k_reserve gave a copy
-__global__ void __launch_bounds__(COPY_THREADS) k_copy_shared(CopyArgs a, ReserveWork wk) {
+template <typename V, int TEAM>
+__global__ void __launch_bounds__(COPY_THREADS, 4) k_copy_shared(CopyArgs a, ReserveWork wk) {
     pdl_launch_dependents();
     pdl_wait();
-    const int each = 2 * a.n_layers;
-    const long long n = (long long)*wk.n_copies * each;
-    for (long long it = blockIdx.x; it < n; it += gridDim.x) {
-        const int m = (int)(it / each), what = (int)(it - (long long)m * each);
+    each_item<TEAM>(a, *wk.n_copies, [&](int m, unsigned what) {
         const CowItem c = wk.copies[m];
-        copy_item(a, what, c.src, c.dst, c.tokens);
-    }
+        copy_item<V, TEAM>(a, what, c.src, c.dst, c.tokens);
+    });
 }
 
 // ---- moving the live pages together --------------------------------------------------------------------------------
@@ -376,7 +435,8 @@ __global__ void __launch_bounds__(CMP_THREADS) k_compact_plan(const int* refs, i
     }
 }
 
-__global__ void __launch_bounds__(COPY_THREADS) k_compact_move(CopyArgs a, PagedView c, int* moved_to, const int* live_out, CompactWork wk) {
+template <typename V, int TEAM>
+__global__ void __launch_bounds__(COPY_THREADS, 4) k_compact_move(CopyArgs a, PagedView c, int* moved_to, const int* live_out, CompactWork wk) {
     pdl_launch_dependents();
     pdl_wait();
     const int M = *wk.moves, L = *live_out;
@@ -384,17 +444,13 @@ __global__ void __launch_bounds__(COPY_THREADS) k_compact_move(CopyArgs a, Paged
     const long long gtid = (long long)blockIdx.x * COPY_THREADS + threadIdx.x, gsize = (long long)gridDim.x * COPY_THREADS;
     for (long long i = gtid; i < (long long)c.n_rows * c.max_pages; i += gsize) {
         const int e = c.table[i];
-        if (e >= L && e < c.n_pages && c.refs[e] >= 0) {
+        if (e >= L && e < c.n_pages) {
             const int k = wk.rank[e];
             if (k >= 0 && k < M && wk.src[k] == e) c.table[i] = wk.dst[k];
         }
     }
     for (long long i = gtid; i < M; i += gsize) moved_to[wk.src[i]] = wk.dst[i];
-    const int each = 2 * a.n_layers;
-    for (long long it = blockIdx.x; it < (long long)M * each; it += gridDim.x) {
-        const int m = (int)(it / each), what = (int)(it - (long long)m * each);
-        copy_item(a, what, wk.src[m], wk.dst[m], a.shape.page_size);
-    }
+    each_item<TEAM>(a, M, [&](int m, unsigned what) { copy_item<V, TEAM>(a, what, wk.src[m], wk.dst[m], a.shape.page_size); });
 }
 
 // the counts follow their pages
@@ -408,10 +464,10 @@ __global__ void __launch_bounds__(CMP_THREADS) k_compact_refs(int* refs, Compact
 }
 
 // ---- rows of contiguous state --------------------------------------------------------------------------------------
-constexpr int GATHER_VECS = 4096;                 // vectors an item
+constexpr int GATHER_VECS = 2048;                 // vectors an item
 
 template <typename V>
-__global__ void __launch_bounds__(COPY_THREADS) k_gather_rows(const __half* src, __half* dst, const int* parents, int outer, int rows,
+__global__ void __launch_bounds__(COPY_THREADS, 4) k_gather_rows(const __half* src, __half* dst, const int* parents, int outer, int rows,
                                                               long long used, long long so, long long sr, long long dso, long long dsr,
                                                               int pieces, int* status) {
     pdl_launch_dependents();
@@ -431,31 +487,42 @@ __global__ void __launch_bounds__(COPY_THREADS) k_gather_rows(const __half* src,
         const __half* s = src + o * so + parent * sr;
         __half* d = dst + o * dso + r * dsr;
         const long long v0 = (long long)piece * GATHER_VECS;
-        copy_run<V>(d + v0 * VEC, s + v0 * VEC, min((long long)GATHER_VECS, vecs - v0), threadIdx.x, COPY_THREADS);
+        copy_run<V, COPY_THREADS>(d + v0 * VEC, s + v0 * VEC, (int)min((long long)GATHER_VECS, vecs - v0), threadIdx.x);
         if (piece == pieces - 1)
             for (long long i = vecs * VEC + threadIdx.x; i < used; i += COPY_THREADS) d[i] = s[i];
     }
 }
 
 CopyArgs copy_args(const PagedView& c) {
-    return CopyArgs{c.k, c.v, c.layer_stride, c.page_stride, c.n_layers, c.n_pages, page_shape(c), device_status_word()};
+    CopyArgs a{c.k, c.v, c.layer_stride, c.page_stride, c.n_layers, c.n_pages, COPY_THREADS, page_shape(c), FastDiv(2u * c.n_layers), device_status_word()};
+    if ((long long)c.page_size * c.n_kv_heads * c.head_dim / a.shape.vec <= 2 * COPY_THREADS) a.team = 32;
+    return a;
 }
+// the kernel of a copy for vectors of 16 or 2 bytes and a CTA or a warp an item
+#define TL_LAUNCH_COPY(KERNEL, ...)                                                                                      \
+    (a.shape.vec == 8 ? (a.team == 32 ? launch_pdl(KERNEL<uint4, 32>, __VA_ARGS__) : launch_pdl(KERNEL<uint4, COPY_THREADS>, __VA_ARGS__))   \
+                      : (a.team == 32 ? launch_pdl(KERNEL<__half, 32>, __VA_ARGS__) : launch_pdl(KERNEL<__half, COPY_THREADS>, __VA_ARGS__)))
+// CTAs of a copy: one an item where that is at all possible. Fewer that loop over items keep too little under way: rows of 1.4 MB
+// took 224 us with eight CTAs an SM, 200 with 64, 191 with one an item; pages of 32 KB 360, 343 and 338.
 unsigned copy_grid(long long items) {
-    const long long most = (long long)sm_count() * 8;
+    const long long most = (long long)sm_count() * 256;
     return (unsigned)(items < 1 ? 1 : (items < most ? items : most));
 }
+unsigned page_grid(const CopyArgs& a, long long pages) { return copy_grid((pages * 2 * a.n_layers * a.team + COPY_THREADS - 1) / COPY_THREADS); }
 }  // namespace
 
-int launch_paged_fork(const PagedView& c, const int* parents, cudaStream_t st) {
-    int slab = 8;                                 // 32 bytes of a row; fewer columns where many rows fill shared memory
-    while (slab > 1 && (long long)c.n_rows * slab * 4 > 196608) slab /= 2;
-    const size_t smem = (size_t)c.n_rows * slab * 4;
-    if (smem > 196608) return set_error(TL_ERR_UNSUPPORTED, "paged_fork: more than 49152 rows");
+template <int SLAB>
+static int launch_fork(const PagedView& c, const int* parents, cudaStream_t st) {
     static PerDeviceOnce once;
-    if (once.needed()) TL_CUDA(cudaFuncSetAttribute(k_fork, cudaFuncAttributeMaxDynamicSharedMemorySize, 196608));
-    const int grid = (c.max_pages + slab - 1) / slab + 1;
-    return launch_pdl(k_fork, grid, FORK_THREADS, smem, st, true, c.table, c.lengths, c.refs, parents, c.n_rows, c.max_pages, c.n_pages,
-                      slab, device_status_word());
+    if (once.needed()) TL_CUDA(cudaFuncSetAttribute(k_fork<SLAB>, cudaFuncAttributeMaxDynamicSharedMemorySize, FORK_SMEM));
+    return launch_pdl(k_fork<SLAB>, (unsigned)((c.max_pages + SLAB - 1) / SLAB + 1), FORK_THREADS, (size_t)c.n_rows * SLAB * 4, st, true, c.table,
+                      c.lengths, c.refs, parents, c.n_rows, c.max_pages, c.n_pages, device_status_word());
+}
+int launch_paged_fork(const PagedView& c, const int* parents, cudaStream_t st) {
+    // 32 bytes of a row at a time; less where many rows fill shared memory
+    if ((long long)c.n_rows * 32 <= FORK_SMEM) return launch_fork<8>(c, parents, st);
+    if ((long long)c.n_rows * 4 <= FORK_SMEM) return launch_fork<1>(c, parents, st);
+    return set_error(TL_ERR_UNSUPPORTED, "paged_fork: more than 49152 rows");
 }
 
 // reserve: 64 bytes of counters, CowItem[n_rows], int need[n_rows], int freed[n_pages];
@@ -470,12 +537,14 @@ int launch_paged_reserve(const PagedView& c, const int* new_tokens, int* result,
     wk.need = reinterpret_cast<int*>(w + 64 + sizeof(CowItem) * (size_t)c.n_rows);
     wk.freed = wk.need + c.n_rows;
     TL_PROPAGATE(launch_pdl(k_reserve, 1, RES_THREADS, 0, st, true, c, new_tokens, result, wk, device_status_word()));
-    return launch_pdl(k_copy_shared, copy_grid((long long)c.n_rows * 2 * c.n_layers), COPY_THREADS, 0, st, true, copy_args(c), wk);
+    const CopyArgs a = copy_args(c);
+    return TL_LAUNCH_COPY(k_copy_shared, page_grid(a, c.n_rows), COPY_THREADS, 0, st, true, a, wk);
 }
 
 int launch_paged_copy(const PagedView& c, const int* src, const int* dst, int n, cudaStream_t st) {
     if (n == 0) return TL_OK;
-    return launch_pdl(k_copy_pages, copy_grid((long long)n * 2 * c.n_layers), COPY_THREADS, 0, st, true, copy_args(c), src, dst, n);
+    const CopyArgs a = copy_args(c);
+    return TL_LAUNCH_COPY(k_copy_pages, page_grid(a, n), COPY_THREADS, 0, st, true, a, src, dst, n);
 }
 
 int launch_paged_compact(const PagedView& c, int* moved_to, int* live, void* work, cudaStream_t st) {
@@ -488,8 +557,8 @@ int launch_paged_compact(const PagedView& c, int* moved_to, int* live, void* wor
     wk.dst = wk.src + c.n_pages;
     TL_PROPAGATE(launch_pdl(k_compact_count, blocks, CMP_THREADS, 0, st, true, c.refs, c.n_pages, wk));
     TL_PROPAGATE(launch_pdl(k_compact_plan, blocks, CMP_THREADS, 0, st, true, c.refs, c.n_pages, moved_to, live, wk));
-    const long long most = (long long)(c.n_pages / 2) * 2 * c.n_layers;
-    TL_PROPAGATE(launch_pdl(k_compact_move, copy_grid(most), COPY_THREADS, 0, st, true, copy_args(c), c, moved_to, live, wk));
+    const CopyArgs a = copy_args(c);              // (no more pages can move than half of them)
+    TL_PROPAGATE(TL_LAUNCH_COPY(k_compact_move, page_grid(a, c.n_pages / 2 + 1), COPY_THREADS, 0, st, true, a, c, moved_to, live, wk));
     return launch_pdl(k_compact_refs, (unsigned)ceil_div((size_t)c.n_pages / 2 + 1, CMP_THREADS) < 64u ? (unsigned)ceil_div((size_t)c.n_pages / 2 + 1, CMP_THREADS) : 64u,
                       CMP_THREADS, 0, st, true, c.refs, wk);
 }
