@@ -172,7 +172,7 @@ __global__ void __launch_bounds__(SEL_THREADS, 4) k_beam_select(SelLaunch p) {
         constexpr float L2E = 1.4426950408889634f;
         uint4* aside = reinterpret_cast<uint4*>(dyn);            // [W * SEL_THREADS + SEL_ASIDE]: a window's vectors always fit
         unsigned* aside_at = reinterpret_cast<unsigned*>(aside + W * SEL_THREADS + SEL_ASIDE);
-        unsigned* list = aside_at + W * SEL_THREADS + SEL_ASIDE; // [SEL_LONG + 8 * SEL_BATCH]
+        unsigned* list = aside_at + W * SEL_THREADS + SEL_ASIDE; // [SEL_LONG + 8 * SEL_ASIDE]
         const int first = split * p.chunk, n = min(p.chunk, a.vocab - first);
         const __half* x = a.logits + row * a.pitch + first;
         const int skew = (int)((reinterpret_cast<uintptr_t>(x) & 15) >> 1);
@@ -217,6 +217,7 @@ __global__ void __launch_bounds__(SEL_THREADS, 4) k_beam_select(SelLaunch p) {
                         if (e0 + r < (unsigned)n && o >= border) list[atomicAdd(&listed_sh, 1)] = o << 16 | (0xffffu - (e0 + r));
                     }
                 }
+                if ((i0 + SEL_BATCH) % SEL_ASIDE != 0 && i0 + SEL_BATCH < have) continue;      // the list holds that many more
                 __syncthreads();
                 const int listed = listed_sh;
                 __syncthreads();
@@ -417,13 +418,13 @@ __global__ void __launch_bounds__(SEL_THREADS, 4) k_beam_select(SelLaunch p) {
             if (rank < a.k) out[rank] = key;
         }
     }
-    // 6: the last CTA of the entry joins (the barrier before the fence makes it cover all threads' results)
+    // 6: the last CTA of the entry joins (the barrier makes the release cover all threads' results)
     __syncthreads();
     if (tid == 0) {
-        __threadfence();
-        last_sh = atomicAdd(p.counters + entry, 1u) == (unsigned)(a.beams * p.splits - 1);
+        unsigned seen;
+        asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(seen) : "l"(p.counters + entry) : "memory");
+        last_sh = seen == (unsigned)(a.beams * p.splits - 1);
         if (last_sh) p.counters[entry] = 0;
-        __threadfence();
         count_sh = 0;
     }
     __syncthreads();
@@ -447,8 +448,8 @@ __global__ void __launch_bounds__(SEL_THREADS, 4) k_beam_select(SelLaunch p) {
         if (lane == 0) lse[w] = M > -INFINITY ? (double)M + log(S) : 0.0;
     }
     __syncthreads();
-    // the heads of the lists (as many of each as make k candidates): their k-th bounds the result from below
-    const int heads = (a.k + lists - 1) / lists, some = heads * lists;
+    // the heads of the lists (as many of each as make 4 k candidates): their k-th bounds the result from below, closely
+    const int heads = min(a.k, (4 * a.k + lists - 1) / lists), some = heads * lists;
     for (int i = tid; i < total; i += SEL_THREADS) {
         const int l = i / a.k, j = i - l * a.k, w = l / p.splits, s = l - w * p.splits, r = entry * a.beams + w;
         const double score = beam_score(a.scores[r]);
@@ -542,7 +543,7 @@ int sel_chunk(int vocab, int splits) { return ((vocab + splits - 1) / splits + 7
 template <int W>
 int launch_sel(const SelLaunch& p, cudaStream_t st) {
     const size_t total = (size_t)p.a.beams * p.splits * p.a.k, join = total * 24 + (size_t)p.a.beams * 8;
-    const size_t list = (size_t)(SEL_THREADS * W + SEL_ASIDE) * 20 + (SEL_LONG + 8 * SEL_BATCH) * 4, smem = list > join ? list : join;
+    const size_t list = (size_t)(SEL_THREADS * W + SEL_ASIDE) * 20 + (SEL_LONG + 8 * SEL_ASIDE) * 4, smem = list > join ? list : join;
     static PerDeviceOnce once;
     if (once.needed()) TL_CUDA(cudaFuncSetAttribute(k_beam_select<W>, cudaFuncAttributeMaxDynamicSharedMemorySize, SEL_MAX_MERGE * 24 + 128 * 8));
     return launch_pdl(k_beam_select<W>, p.a.batch * p.a.beams * p.splits, SEL_THREADS, smem, st, true, p);
