@@ -72,7 +72,8 @@ __global__ void __launch_bounds__(ANY_WARPS * 32) k_paged_attn_any(AttnLaunch p)
         }
         s = warp_sum(s);
         const float mn = fmaxf(m, s);
-        const float keep = mn == -INFINITY ? 1.f : expf(m - mn), e = mn == -INFINITY ? 0.f : expf(s - mn);
+        const float ref = mn == -INFINITY ? 0.f : mn;
+        const float keep = expf(m - ref), e = expf(s - ref);
         l = l * keep + e;
         m = mn;
 #pragma unroll
@@ -93,9 +94,9 @@ __global__ void __launch_bounds__(ANY_WARPS * 32) k_paged_attn_any(AttnLaunch p)
     for (int d = threadIdx.x; d < hd; d += ANY_WARPS * 32) {
         float a = 0.f;
         for (int w = 0; w < ANY_WARPS; w++) a += sm_acc[w][d] * expf(sm_m[w] - ref);
-        p.out[b * p.o_row + (long long)h * hd + d] = __float2half_rn(L > 0.f ? a / L : 0.f);
+        p.out[b * p.o_row + (long long)h * hd + d] = __float2half_rn(L == 0.f ? 0.f : a / L);
     }
-    if (threadIdx.x == 0 && p.lse) p.lse[(long long)b * p.n_heads + h] = L > 0.f ? M + logf(L) : -INFINITY;
+    if (threadIdx.x == 0 && p.lse) p.lse[(long long)b * p.n_heads + h] = L == 0.f ? -INFINITY : M + logf(L);
 }
 
 
@@ -488,7 +489,7 @@ __global__ void __launch_bounds__(FL_THREADS, FlashShape<HDP, NT>::CTAS) k_paged
         const long long slot_floats = flash_slot_floats(p.chunk, hd);
         float* part = p.partial + (2ll * blockIdx.x + (seg_i == 0)) * slot_floats;
         auto finish = [&](int h, int d, float4 x, float M, float L) {     // four elements of a head's result
-            const float inv = L > 0.f ? 1.f / L : 0.f;
+            const float inv = L == 0.f ? 0.f : 1.f / L;                      // (a NaN stays one)
             const __half2 lo = __floats2half2_rn(x.x * inv, x.y * inv), hi = __floats2half2_rn(x.z * inv, x.w * inv);
             __half* at = a.out + seg_b * a.o_row + (long long)(h0 + h) * hd + d;
             if (p.out8) {
@@ -496,7 +497,7 @@ __global__ void __launch_bounds__(FL_THREADS, FlashShape<HDP, NT>::CTAS) k_paged
             } else {
                 at[0] = __low2half(lo); at[1] = __high2half(lo); at[2] = __low2half(hi); at[3] = __high2half(hi);
             }
-            if (d == 0 && a.lse) a.lse[(long long)seg_b * a.n_heads + h0 + h] = L > 0.f ? (M + log2f(L)) * 0.69314718055994531f : -INFINITY;
+            if (d == 0 && a.lse) a.lse[(long long)seg_b * a.n_heads + h0 + h] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.69314718055994531f;
         };
         for (int i = tid; i < heads * (HDP / 4); i += FL_THREADS) {
             const int h = i / (HDP / 4), d = i % (HDP / 4) * 4;

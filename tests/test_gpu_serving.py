@@ -271,6 +271,24 @@ def test_attention_never_follows_bad_ids(tl, hd):
     assert tl.device_status() == 0
 
 
+@pytest.mark.parametrize("hd", [64, 7])
+def test_attention_shows_a_nan_where_there_is_one(tl, hd):
+    """A NaN in a stored key or value reaches the results of its row's heads, and no other's."""
+    r = np.random.default_rng(17)
+    lens = [100, 100, 100]
+    c, k, v, table, refs = filled_cache(tl, r, 1, 16, 2, hd, lens, garbage=False)
+    k[0, table[1, 2], 5, 1, 3] = np.nan
+    v[0, table[2, 6], 3, 0, 2] = np.nan
+    c = tl.PagedCache(1, k.shape[1], 16, 2, hd, 3, table.shape[1], k=k, v=v)
+    c.set_state(table, lens, refs)
+    q = normal(r, 3, 4, hd)
+    out, lse = c.attend(0, q)
+    assert np.isnan(out[1, 2:]).all() and np.isnan(lse[1, 2:]).all()
+    assert np.isnan(out[2, :2, 2]).all() and not np.isnan(np.delete(out[2, :2], 2, 1)).any() and not np.isnan(lse[2]).any()
+    assert not np.isnan(out[0]).any() and not np.isnan(out[1, :2]).any() and not np.isnan(out[2, 2:]).any()
+    check_attention(tl, c, k[0], v[0], table, lens, 16, q[:1], rows=[0], got=(out[:1], lse[:1]))
+
+
 def test_attention_with_padded_rows_of_q_and_out_and_no_lse(tl):
     r = np.random.default_rng(15)
     lens, heads, hd = [70, 3, 0], 8, 64
