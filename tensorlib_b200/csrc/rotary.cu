@@ -3,8 +3,9 @@
 // they are, straight into their pages: one pass over q, k and v.
 //
 // The angle: position * freqs[i] / (2 pi) in 64 bits, reduced to the nearest turn there, so that position 10^6 loses
-// nothing; the fraction (at most half a turn) is exact to 2^-24 of a turn in 32 bits, and sincospif takes it from there.
-// The rotation itself is in 32 bits with one rounding to fp16.
+// nothing; the fraction (at most half a turn) is exact to 2^-24 of a turn in 32 bits. Within half a turn the hardware's sine and
+// cosine are good to 2^-20.5, a seven-hundredth of the rounding of the result to fp16. The rotation itself is in 32 bits with
+// that one rounding.
 //
 // Bound: HBM at many tokens (every element is read and written once), launch and one dependent load chain
 // (position -> cos/sin -> store) at one token. What has to be small for that is the number of instructions a vector: a form
@@ -12,6 +13,8 @@
 // 128, at 83% of the issue slots. So a thread keeps to one vector of the head and steps through (token, head) rows with
 // pointers that only grow; the cos/sin of a CTA's tokens are worked out once, for all heads, in shared memory, while the first
 // vectors arrive.
+#include <type_traits>
+
 #include "serving.cuh"
 
 namespace tlb {
@@ -19,10 +22,10 @@ namespace tlb {
 namespace {
 
 constexpr int ROT_THREADS = 256;
-// CTAs of an SM: what the registers of the rows under way allow. 16384 tokens of 40 heads of 128: 58 us interleaved with five
-// (64 with six, which spill), 58 us in halves with four (65 with five).
+// CTAs of an SM: what the registers of the rows under way allow. 16384 tokens of 40 heads of 128: interleaved 59 us with five (64
+// with four), in halves 59 us with four (65 with five).
 constexpr int rot_ctas(bool half_layout) { return half_layout ? 4 : 5; }
-constexpr int ROT_ROWS = 16;                      // rows of a thread
+constexpr int ROT_ROWS = 32;                      // rows of a thread
 constexpr int ROT_MAX_GROUP = 64;                 // tokens of a CTA
 constexpr int ROT_MAX_PAIRS = 1024;               // their pairs in shared memory (one token has at most 512)
 
@@ -52,9 +55,8 @@ struct RotLaunch {
 // cos and sin of pair i at `pos`, times the magnitude
 __device__ __forceinline__ float2 turn_of(const RotaryArgs& a, int pos, int i) {
     const double turns = (double)pos * (a.freqs[i] * 0.15915494309189533577);
-    const float frac = (float)(turns - rint(turns));
-    float s, c;
-    sincospif(2.f * frac, &s, &c);
+    const float angle = (float)(turns - rint(turns)) * 6.2831853071795865f;
+    const float s = __sinf(angle), c = __cosf(angle);
     return make_float2(c * a.magnitude, (a.inverse ? -s : s) * a.magnitude);
 }
 // where token t goes in its page, -1 if its row, position or page is not there
@@ -69,20 +71,52 @@ __device__ __forceinline__ long long slot_of(const RotLaunch& p, int t, int pos)
     return -1;
 }
 
+template <int N> struct FloatVec;
+template <> struct FloatVec<4> { using T = float4; };
+template <> struct FloatVec<2> { using T = float2; };
+template <> struct FloatVec<1> { using T = float; };
 template <int VEC> struct HalfVec;
 template <> struct HalfVec<8> { using T = uint4; };
 template <> struct HalfVec<4> { using T = uint2; };
 template <> struct HalfVec<2> { using T = unsigned; };
+
+// x (and y, the vector half a rotated part further) turned by the cos and sin of its pairs, which lie at c and c + stride
+template <int VEC, bool HALF, typename V>
+__device__ __forceinline__ void turn_item(V& x, V& y, const float* c, int stride) {
+    constexpr int PAIRS = HALF ? VEC : VEC / 2, W = PAIRS < 4 ? PAIRS : 4;
+    using F = typename FloatVec<W>::T;            // W pairs by one load each
+    __half2* xh = reinterpret_cast<__half2*>(&x);
+    __half2* yh = reinterpret_cast<__half2*>(&y);
+#pragma unroll
+    for (int j0 = 0; j0 < PAIRS; j0 += W) {
+        const F cv = *reinterpret_cast<const F*>(c + j0), sv = *reinterpret_cast<const F*>(c + stride + j0);
+        const float* co = reinterpret_cast<const float*>(&cv);
+        const float* si = reinterpret_cast<const float*>(&sv);
+        if constexpr (HALF) {
+#pragma unroll
+            for (int j = 0; j < W; j += 2) {
+                __half2 &xv = xh[(j0 + j) / 2], &yv = yh[(j0 + j) / 2];
+                const float2 f = __half22float2(xv), g = __half22float2(yv);
+                xv = __floats2half2_rn(f.x * co[j] - g.x * si[j], f.y * co[j + 1] - g.y * si[j + 1]);
+                yv = __floats2half2_rn(f.x * si[j] + g.x * co[j], f.y * si[j + 1] + g.y * co[j + 1]);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < W; j++) {
+                const float2 f = __half22float2(xh[j0 + j]);
+                xh[j0 + j] = __floats2half2_rn(f.x * co[j] - f.y * si[j], f.x * si[j] + f.y * co[j]);
+            }
+        }
+    }
+}
 
 // Items of VEC values. Interleaved pairs: an item is a vector, VEC / 2 pairs. Half layout: an item is the vectors at i and
 // i + rot / 2, VEC pairs; behind rot, one vector.
 template <int VEC, bool HALF>
 __global__ void __launch_bounds__(ROT_THREADS, rot_ctas(HALF)) k_rotary(RotLaunch p) {
     using V = typename HalfVec<VEC>::T;
-    constexpr int PAIRS = HALF ? VEC : VEC / 2;   // of an item
     extern __shared__ __align__(16) float turns[];             // [group]: cos [stride], sin [stride]
-    __shared__ long long slots[ROT_MAX_GROUP];    // where the token goes in its page, -1: nowhere
-    __shared__ int live[ROT_MAX_GROUP];           // 0: padding
+    __shared__ long long places[2][ROT_MAX_GROUP];             // where the token goes: its row of q, its slot in the page; -1: nowhere
     pdl_launch_dependents();
     pdl_wait();
     const RotaryArgs& a = p.a;
@@ -93,7 +127,7 @@ __global__ void __launch_bounds__(ROT_THREADS, rot_ctas(HALF)) k_rotary(RotLaunc
     const int d = !HALF || pair ? (int)item * VEC : a.rot + ((int)item - pairs / VEC) * VEC;
     // all planes one after the other, or (few tokens) one a CTA
     const int first = gridDim.y > 1 ? blockIdx.y : 0, end = gridDim.y > 1 ? first + 1 : p.planes;
-    constexpr int U = HALF ? 2 : 4;               // rows under way a thread
+    constexpr int U = HALF ? 2 : 3;               // rows under way a thread
     V x[U], y[U];
     bool ready = false;
     for (int w = first; w < end; w++) {
@@ -104,71 +138,59 @@ __global__ void __launch_bounds__(ROT_THREADS, rot_ctas(HALF)) k_rotary(RotLaunc
         p.plane[w].by_heads_at_once.divmod(r, tt, h0);
         const int left = (int)tt < tokens_at_once ? heads - (int)h0 : 0;       // rows of a token: 0, at_once, .. below this
         const __half* in_token = p.plane[w].in + (long long)(t0 + (int)tt) * p.plane[w].in_token + h0 * p.plane[w].in_head + d;
-        const long long in_next = tokens_at_once * p.plane[w].in_token;
         __half* const out0 = p.plane[w].out + h0 * p.plane[w].out_head + d;
-        const long long out_token = p.plane[w].out_token;
-        for (int t = (int)tt;; t += tokens_at_once) {
-            const __half* in = in_token;
-            int h = 0;
-            do {
+        // a thread's rows under way: heads of one token, or, where all its heads are moved at once, tokens
+        auto move = [&](auto by_token_c) {
+            constexpr bool by_token = decltype(by_token_c)::value;
+            const int more_tokens = by_token ? tokens_at_once : 0, t_step = by_token ? U * tokens_at_once : tokens_at_once;
+            const long long in_more = by_token ? tokens_at_once * p.plane[w].in_token : in_step, out_more = by_token ? 0 : out_step;
+            const long long in_next = t_step * p.plane[w].in_token;
+            for (int t = (int)tt;; t += t_step, in_token += in_next) {
+                const __half* in = in_token;
+                int h = 0;
+                do {
 #pragma unroll
-                for (int u = 0; u < U; u++)
-                    if (t < n_tokens && h + u * at_once < left) {
-                        x[u] = *reinterpret_cast<const V*>(in + u * in_step);
-                        if (pair) y[u] = *reinterpret_cast<const V*>(in + u * in_step + pairs);
+                    for (int u = 0; u < U; u++)
+                        if (t + u * more_tokens < n_tokens && (by_token ? left > 0 : h + u * at_once < left)) {
+                            x[u] = *reinterpret_cast<const V*>(in + u * in_more);
+                            if (pair) y[u] = *reinterpret_cast<const V*>(in + u * in_more + pairs);
+                        }
+                    if (!ready) {                 // the turns and places of the CTA's tokens, while the first rows arrive
+                        for (int j = threadIdx.x; j < n_tokens; j += ROT_THREADS) {
+                            const int pos = a.positions[t0 + j];          // below 0: padding
+                            places[0][j] = pos >= 0 ? (t0 + j) * p.plane[0].out_token : -1;
+                            places[1][j] = p.paged && pos >= 0 ? slot_of(p, t0 + j, pos) : -1;
+                        }
+                        const int todo = p.plane[first].turned ? n_tokens * pairs : 0;      // (values alone need no turns)
+                        for (int j = threadIdx.x; j < todo; j += ROT_THREADS) {
+                            unsigned k, i;
+                            p.by_pairs.divmod((unsigned)j, k, i);
+                            const float2 c = turn_of(a, a.positions[t0 + (int)k], (int)i);
+                            turns[k * 2 * stride + i] = c.x;
+                            turns[(k * 2 + 1) * stride + i] = c.y;
+                        }
+                        __syncthreads();
+                        ready = true;
                     }
-                if (!ready) {                     // the turns and places of the CTA's tokens, while the first rows arrive
-                    for (int j = threadIdx.x; j < n_tokens; j += ROT_THREADS) {
-                        const int pos = a.positions[t0 + j];
-                        live[j] = pos >= 0;
-                        slots[j] = p.paged && pos >= 0 ? slot_of(p, t0 + j, pos) : -1;
-                    }
-                    const int todo = p.plane[first].turned ? n_tokens * pairs : 0;      // (values alone need no turns)
-                    for (int j = threadIdx.x; j < todo; j += ROT_THREADS) {
-                        unsigned k, i;
-                        p.by_pairs.divmod((unsigned)j, k, i);
-                        const float2 c = turn_of(a, a.positions[t0 + (int)k], (int)i);
-                        turns[k * 2 * stride + i] = c.x;
-                        turns[(k * 2 + 1) * stride + i] = c.y;
-                    }
-                    __syncthreads();
-                    ready = true;
-                }
-                if (t >= n_tokens || left <= 0) break;
-                const long long at = paged ? slots[t] : (long long)(t0 + t) * out_token;
-                if (live[t] && at >= 0) {
-                    __half* out = out0 + at + (h == 0 ? 0 : (long long)(h / at_once) * out_step);
-                    const float* c = turns + t * 2 * stride + (HALF ? d : d / 2);
+                    if (t >= n_tokens || left <= 0) return;
+                    __half* out = out0 + (h == 0 ? 0 : (long long)(h / at_once) * out_step);
 #pragma unroll
                     for (int u = 0; u < U; u++) {
-                        if (h + u * at_once >= left) continue;
-                        if (turn) {
-                            __half2* xh = reinterpret_cast<__half2*>(&x[u]);
-                            __half2* yh = reinterpret_cast<__half2*>(&y[u]);
-#pragma unroll
-                            for (int j = 0; j < VEC / 2; j++) {
-                                const float2 f = __half22float2(xh[j]);
-                                if (HALF) {
-                                    const float2 g = __half22float2(yh[j]);
-                                    const float2 co = *reinterpret_cast<const float2*>(c + 2 * j), si = *reinterpret_cast<const float2*>(c + stride + 2 * j);
-                                    xh[j] = __floats2half2_rn(f.x * co.x - g.x * si.x, f.y * co.y - g.y * si.y);
-                                    yh[j] = __floats2half2_rn(f.x * si.x + g.x * co.x, f.y * si.y + g.y * co.y);
-                                } else {
-                                    const float co = c[j], si = c[stride + j];
-                                    xh[j] = __floats2half2_rn(f.x * co - f.y * si, f.x * si + f.y * co);
-                                }
-                            }
-                        }
-                        *reinterpret_cast<V*>(out + u * out_step) = x[u];
-                        if (pair) *reinterpret_cast<V*>(out + u * out_step + pairs) = y[u];
+                        const int tu = t + u * more_tokens;
+                        if (tu >= n_tokens || (!by_token && h + u * at_once >= left)) continue;
+                        const long long at = places[paged][tu];
+                        if (at < 0) continue;
+                        if (turn) turn_item<VEC, HALF>(x[u], y[u], turns + tu * 2 * stride + (HALF ? d : d / 2), stride);
+                        *reinterpret_cast<V*>(out + at + u * out_more) = x[u];
+                        if (pair) *reinterpret_cast<V*>(out + at + u * out_more + pairs) = y[u];
                     }
-                }
-                in += U * in_step;
-                h += U * at_once;
-            } while (h < left);
-            if (t >= n_tokens || left <= 0) break;
-            in_token += in_next;
-        }
+                    in += U * in_step;
+                    h += U * at_once;
+                } while (!by_token && h < left);
+            }
+        };
+        if (at_once == heads) move(std::true_type{});
+        else move(std::false_type{});
     }
 }
 
