@@ -344,7 +344,8 @@ TL_API int tl_paged_workspace(int n_rows, int n_pages, size_t* bytes);
 /* The way into the cache for new tokens, one launch: q rotated into q_out (n_heads heads; 0: none; q_out == q with equal strides is
  * allowed), k rotated and v as it is stored at positions[t] of row rows[t] (rows == NULL: row t). Heads of a token are
  * contiguous in q, k and v, so that they can be parts of one fused projection; token strides in elements. rot_dim, half_layout,
- * freqs, magnitude and padding as for tl_rotary_f16; rot_dim = 0 only stores. Room must have been made (tl_paged_reserve_f16). */
+ * freqs, magnitude and padding as for tl_rotary_f16; rot_dim = 0 only stores. Room must have been made (tl_paged_reserve_f16), and no
+ * two tokens of a call may go to the same place. */
 TL_API int tl_rotary_append_f16(const tl_paged_cache* cache, int layer, const tl_half* q, tl_half* q_out, const tl_half* k,
                                 const tl_half* v, const int* rows, const int* positions, const double* freqs, float magnitude,
                                 int tokens, int n_heads, int rot_dim, int half_layout, long long q_token_stride,

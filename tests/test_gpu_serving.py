@@ -207,7 +207,8 @@ def test_attention_over_pages(tl, hd, kv, group, page, by_head):
 
 @pytest.mark.parametrize("B,low,high,kv,group,hd,page", [(1, 1, 1, 32, 1, 128, 16), (1, 333, 333, 32, 1, 128, 16), (1, 20011, 20011, 1, 8, 128, 16),
                                                          (1, 9000, 9000, 8, 4, 64, 64), (3, 1, 7000, 2, 4, 128, 24), (200, 1, 90, 2, 2, 64, 16),
-                                                         (65, 30, 500, 4, 3, 80, 32), (300, 0, 3, 1, 1, 128, 16)])
+                                                         (65, 30, 500, 4, 3, 80, 32), (300, 0, 3, 1, 1, 128, 16),
+                                                         (1, 30000, 30000, 1, 16, 64, 16), (2, 6000, 9000, 1, 12, 256, 32), (1, 15000, 15000, 2, 3, 192, 8)])
 def test_attention_split_over_the_length(tl, B, low, high, kv, group, hd, page):
     r = np.random.default_rng([B, high, kv])
     lens = r.integers(low, high + 1, B).tolist()
