@@ -22,10 +22,10 @@ namespace tlb {
 namespace {
 
 constexpr int ROT_THREADS = 256;
-// CTAs of an SM: what the registers of the rows under way allow. 16384 tokens of 40 heads of 128: interleaved 59 us with five (64
+// CTAs of an SM: what the registers of the rows under way allow. 16384 tokens of 40 heads of 128: interleaved 58 us with five (64
 // with four), in halves 59 us with four (65 with five).
 constexpr int rot_ctas(bool half_layout) { return half_layout ? 4 : 5; }
-constexpr int ROT_ROWS = 32;                      // rows of a thread
+constexpr int ROT_ROWS = 16;                      // rows of a thread; twice that where three tensors are set up
 constexpr int ROT_MAX_GROUP = 64;                 // tokens of a CTA
 constexpr int ROT_MAX_PAIRS = 1024;               // their pairs in shared memory (one token has at most 512)
 
@@ -112,7 +112,10 @@ __device__ __forceinline__ void turn_item(V& x, V& y, const float* c, int stride
 
 // Items of VEC values. Interleaved pairs: an item is a vector, VEC / 2 pairs. Half layout: an item is the vectors at i and
 // i + rot / 2, VEC pairs; behind rot, one vector.
-template <int VEC, bool HALF>
+// BY: how the rows that a thread has under way follow one another: ROT_BY_HEAD within a token, ROT_BY_TOKEN (all heads of a token
+// are moved at once) from token to token, ROT_EITHER as each tensor wants it, which takes more registers.
+enum { ROT_BY_HEAD, ROT_BY_TOKEN, ROT_EITHER };
+template <int VEC, bool HALF, int BY>
 __global__ void __launch_bounds__(ROT_THREADS, rot_ctas(HALF)) k_rotary(RotLaunch p) {
     using V = typename HalfVec<VEC>::T;
     extern __shared__ __align__(16) float turns[];             // [group]: cos [stride], sin [stride]
@@ -127,7 +130,7 @@ __global__ void __launch_bounds__(ROT_THREADS, rot_ctas(HALF)) k_rotary(RotLaunc
     const int d = !HALF || pair ? (int)item * VEC : a.rot + ((int)item - pairs / VEC) * VEC;
     // all planes one after the other, or (few tokens) one a CTA
     const int first = gridDim.y > 1 ? blockIdx.y : 0, end = gridDim.y > 1 ? first + 1 : p.planes;
-    constexpr int U = HALF ? 2 : 3;               // rows under way a thread
+    constexpr int U = HALF ? 2 : (BY == ROT_EITHER ? 3 : 4);    // rows under way a thread
     V x[U], y[U];
     bool ready = false;
     for (int w = first; w < end; w++) {
@@ -189,7 +192,9 @@ __global__ void __launch_bounds__(ROT_THREADS, rot_ctas(HALF)) k_rotary(RotLaunc
                 } while (!by_token && h < left);
             }
         };
-        if (at_once == heads) move(std::true_type{});
+        if constexpr (BY == ROT_BY_HEAD) move(std::false_type{});
+        else if constexpr (BY == ROT_BY_TOKEN) move(std::true_type{});
+        else if (at_once == heads) move(std::true_type{});
         else move(std::false_type{});
     }
 }
@@ -239,10 +244,17 @@ __global__ void __launch_bounds__(ROT_THREADS) k_rotary_any(RotLaunch p) {
     }
 }
 
+template <int VEC, bool HALF>
+int launch_by(const RotLaunch& p, dim3 grid, size_t smem, cudaStream_t st) {
+    int by_token = 0;
+    for (int w = 0; w < p.planes; w++) by_token += p.plane[w].heads_at_once == p.plane[w].heads;
+    return by_token == 0 ? launch_pdl(k_rotary<VEC, HALF, ROT_BY_HEAD>, grid, ROT_THREADS, smem, st, true, p)
+         : by_token == p.planes ? launch_pdl(k_rotary<VEC, HALF, ROT_BY_TOKEN>, grid, ROT_THREADS, smem, st, true, p)
+                                : launch_pdl(k_rotary<VEC, HALF, ROT_EITHER>, grid, ROT_THREADS, smem, st, true, p);
+}
 template <int VEC>
 int launch_vec(const RotLaunch& p, dim3 grid, size_t smem, cudaStream_t st) {
-    return p.a.half_layout ? launch_pdl(k_rotary<VEC, true>, grid, ROT_THREADS, smem, st, true, p)
-                           : launch_pdl(k_rotary<VEC, false>, grid, ROT_THREADS, smem, st, true, p);
+    return p.a.half_layout ? launch_by<VEC, true>(p, grid, smem, st) : launch_by<VEC, false>(p, grid, smem, st);
 }
 
 }  // namespace
@@ -297,7 +309,7 @@ int launch_rotary(const RotaryArgs& a, const PagedView* cache, cudaStream_t st) 
     // Tokens a CTA: enough that setting up a tensor is small against moving its rows (about ROT_ROWS a thread), and so that the
     // CTAs make whole rounds of those that are resident. Where a token is a CTA, so is each tensor of it.
     const long long resident = (long long)rot_ctas(a.half_layout != 0) * sm_count();
-    long long most = (long long)ROT_ROWS * rows / heads;
+    long long most = (long long)ROT_ROWS * (p.planes > 1 ? 2 : 1) * rows / heads;
     if (pairs > 0 && most > ROT_MAX_PAIRS / pairs) most = ROT_MAX_PAIRS / pairs;
     if (most > ROT_MAX_GROUP) most = ROT_MAX_GROUP;
     if (most < 1) most = 1;
