@@ -366,7 +366,8 @@ TL_API int tl_paged_attn_workspace(int n_heads, int n_kv_heads, int head_dim, si
  * the k best in descending order, ties to the lowest w, then the lowest j: out_scores [batch, k] fp32, out_parents [batch, k] the row
  * batch_entry * beams + w (as tl_paged_fork and tl_beam_reorder_f16 take it), out_tokens [batch, k]. Values are compared in 64 bits.
  * finished (may be NULL): a beam with finished[row] != 0 has one candidate, pad_token, at its score; its logits are not used. A score
- * of -inf makes a dead beam; NaN logits count as -inf and +inf as 65504, NaN scores as -inf. beams, k <= 128. workspace:
+ * of -inf makes a dead beam; NaN logits count as -inf and +inf as 65504, NaN scores as -inf. beams, k <= 128. out_scores may be
+ * scores where k == beams. workspace:
  * tl_beam_select_workspace bytes, zeroed once before its first use. */
 TL_API int tl_beam_select_f16(const tl_half* logits, long long row_stride, const float* scores, const unsigned char* finished,
                               int pad_token, int batch, int beams, int vocab, int k, float* out_scores, int* out_parents,

@@ -86,6 +86,7 @@ int tl_rotary_f16(const tl_half* in, tl_half* out, const int* positions, const d
         return TL_OK;
     }
     TL_REQUIRE(in && out && positions && (freqs || rot_dim == 0), "rotary: null pointer");
+    TL_REQUIRE(in_token_stride >= 0 && in_head_stride >= 0 && out_token_stride >= 0 && out_head_stride >= 0, "rotary: negative stride");
     TL_REQUIRE(in != out || (in_token_stride == out_token_stride && in_head_stride == out_head_stride),
                "rotary: in place needs the same strides on both sides");
     TL_ON_LIBRARY_DEVICE();
@@ -114,6 +115,7 @@ int tl_rotary_append_f16(const tl_paged_cache* cache, int layer, const tl_half* 
     }
     TL_REQUIRE(k && v && positions && (freqs || rot_dim == 0) && (n_heads == 0 || (q && q_out)), "rotary_append: null pointer");
     TL_REQUIRE(rows || tokens <= cache->n_rows, "rotary_append: more tokens than rows without a row list");
+    TL_REQUIRE(q_token_stride >= 0 && q_out_token_stride >= 0 && kv_token_stride >= 0, "rotary_append: negative stride");
     TL_REQUIRE(n_heads == 0 || q != q_out || q_token_stride == q_out_token_stride, "rotary_append: in place needs the same strides on both sides");
     TL_ON_LIBRARY_DEVICE();
     RotaryArgs a{};
@@ -147,6 +149,7 @@ int tl_paged_attn_decode_f16(const tl_paged_cache* cache, int layer, const tl_ha
         return TL_OK;
     }
     TL_REQUIRE(q && out && cache->lengths, "paged_attn_decode: null pointer");
+    TL_REQUIRE(q_row_stride >= 0 && out_row_stride >= 0, "paged_attn_decode: negative stride");
     TL_REQUIRE(rows || batch <= cache->n_rows, "paged_attn_decode: more queries than rows without a row list");
     TL_REQUIRE(workspace && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0, "paged_attn_decode: the workspace must be 16-byte aligned");
     const size_t need = paged_attn_workspace_bytes(n_heads, cache->n_kv_heads, cache->head_dim);
@@ -246,6 +249,7 @@ int tl_beam_reorder_f16(const tl_half* src, tl_half* dst, const int* parents, in
     }
     TL_REQUIRE(src && dst && parents && src != dst, "beam_reorder: null pointer, or in place");
     TL_REQUIRE(src_row_stride >= used && dst_row_stride >= used, "beam_reorder: row stride smaller than the row");
+    TL_REQUIRE(src_outer_stride >= 0 && dst_outer_stride >= 0, "beam_reorder: negative stride");
     TL_REQUIRE(used < (1ll << 40) && (long long)outer * rows < (1ll << 31), "beam_reorder: too large");
     TL_ON_LIBRARY_DEVICE();
     return launch_gather_rows(H(src), H(dst), parents, outer, rows, used, src_outer_stride, src_row_stride, dst_outer_stride, dst_row_stride,

@@ -15,15 +15,18 @@ __device__ __forceinline__ float beam_logit(__half h) {
 }
 __device__ __forceinline__ double beam_score(float s) { return s != s ? -INFINITY : (double)fminf(s, 3.402823466e38f); }
 
-// Plain form for any shape: one CTA a batch entry; lse of its rows, then k rounds of an arg-maximum over what comes after
+// Plain form for what one CTA cannot join or 32 chunks cannot hold (many beams times many results, vocabularies beyond 2 million;
+// four beams of 32000, which the kernel below takes 8 us for: 865 us): one CTA a batch entry; lse of its rows, then k rounds of an arg-maximum over what comes after
 // the last one chosen.
 __global__ void __launch_bounds__(BEAM_THREADS) k_beam_any(BeamArgs a) {
-    extern __shared__ double lse[];               // [beams]
+    extern __shared__ double lse[];               // [beams], and the scores [beams]: out_scores may be their place
     __shared__ double red[BEAM_THREADS / 32];
     __shared__ long long red_i[BEAM_THREADS / 32];
     pdl_launch_dependents();
     pdl_wait();
     const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    double* score = lse + a.beams;
+    for (int w = tid; w < a.beams; w += BEAM_THREADS) score[w] = beam_score(a.scores[b * a.beams + w]);
     for (int w = 0; w < a.beams; w++) {
         const __half* x = a.logits + (long long)(b * a.beams + w) * a.pitch;
         float m = -INFINITY;
@@ -56,7 +59,7 @@ __global__ void __launch_bounds__(BEAM_THREADS) k_beam_any(BeamArgs a) {
         long long best_i = n;
         for (long long i = tid; i < n; i += BEAM_THREADS) {
             const int w = (int)(i / a.vocab), j = (int)(i - (long long)w * a.vocab), row = b * a.beams + w;
-            const double sc = beam_score(a.scores[row]);
+            const double sc = score[w];
             double v;
             if (a.finished && a.finished[row]) v = j == a.pad ? sc : -INFINITY;
             else v = sc + ((double)beam_logit(a.logits[(long long)row * a.pitch + j]) - lse[w]);
@@ -94,7 +97,10 @@ __global__ void __launch_bounds__(BEAM_THREADS) k_beam_any(BeamArgs a) {
 // between and cut back to the k best. The last CTA of a batch entry joins: the rows' log-sums, the candidates' values in 64
 // bits, and a border and ranks over the sorted lists.
 //
-// Bound: HBM with many rows (each logit is read once); with few rows the chain load -> maximum -> sum -> list -> join.
+// Bound: with many rows instructions, some 19 for a warp's 32 logits, before HBM (each logit is read once); with few rows the chain
+// load -> border -> list -> arrival -> log-sum -> ranks. Measured on a B200: 512 rows of 32000 logits, 16 of eight beams each,
+// 21 us (floor 4.7; 3.6 of them the join), four rows 8.3 us. Rows in several chunks took 30 us, for the part of a chunk that does
+// not shrink with it.
 constexpr int SEL_THREADS = 256;
 constexpr int SEL_ASIDE = 256;                    // vectors set aside that wait for the end; more are taken apart
 constexpr int SEL_BATCH = SEL_THREADS / 2;        // vectors taken apart at a time, two threads each
@@ -563,7 +569,7 @@ int launch_beam_select(const BeamArgs& a, cudaStream_t st) {
     p.a = a;
     p.splits = sel_splits(a.batch, a.beams, a.vocab, a.k);
     if (p.splits == 0 || (long long)a.batch * a.beams * p.splits >= (1ll << 31))
-        return launch_pdl(k_beam_any, a.batch, BEAM_THREADS, (size_t)a.beams * 8, st, true, a);
+        return launch_pdl(k_beam_any, a.batch, BEAM_THREADS, (size_t)a.beams * 16, st, true, a);
     p.chunk = sel_chunk(a.vocab, p.splits);
     p.groups = 8;
     while (p.groups < a.k) p.groups *= 2;

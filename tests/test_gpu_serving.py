@@ -495,6 +495,22 @@ def test_beam_selection_first_step_and_nothing_left(tl):
     assert np.array_equal(tl.beam_select(z, [0.0], 1, 9)[2][0], np.arange(9))              # -0 equals +0
 
 
+@pytest.mark.parametrize("batch,beams,vocab", [(5, 4, 3001), (3, 128, 200)])
+def test_beam_selection_writes_the_scores_in_place(tl, batch, beams, vocab):
+    """Both kernels: the second shape has more candidates than one CTA joins."""
+    x, s, fin = beam_case(batch, beams, vocab, 2)
+    with np.errstate(all="ignore"):
+        want = so.beam_select(x, s, beams, beams, fin, 0)
+    assert want[3] > 1e-6
+    lib, need = tl.load(), C.c_size_t(0)
+    tl.check(lib.tl_beam_select_workspace(batch, beams, vocab, beams, C.byref(need)), "ws")
+    w = tl.DeviceBuffer.from_numpy(np.zeros(max(16, need.value), np.uint8))
+    dx, ds, df, dp, dt = (tl.DeviceBuffer.from_numpy(a) for a in (x, s, fin, np.zeros(batch * beams, np.int32), np.zeros(batch * beams, np.int32)))
+    tl.check(lib.tl_beam_select_f16(dx.ptr, vocab, ds.ptr, df.ptr, 0, batch, beams, vocab, beams, ds.ptr, dp.ptr, dt.ptr, w.ptr, w.nbytes, None), "select")
+    assert np.array_equal(dp.to_numpy(np.int32, (batch, beams)), want[1]) and np.array_equal(dt.to_numpy(np.int32, (batch, beams)), want[2])
+    close(ds.to_numpy(np.float32, (batch, beams)), want[0], np.abs(want[0]) * 2.0 ** -24 + 2.0 ** -21)
+
+
 @pytest.mark.parametrize("stride,off", [(1004, 0), (1001, 0), (1008, 3)])
 def test_beam_selection_with_row_strides(tl, stride, off):
     """Rows that start at any 2-byte boundary; what lies behind a row is not read as a candidate."""

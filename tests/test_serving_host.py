@@ -98,7 +98,7 @@ def test_rotary_refuses():
         return lib.tl_rotary_f16(a["i"], a["o"], a["pos"], a["f"], 1.0, a["t"], a["h"], a["d"], a["rot"], a["half"], 0, a["its"], a["ihs"],
                                  a["ots"], a["ohs"], None)
     for bad in (dict(t=-1), dict(h=0), dict(d=0), dict(rot=129), dict(rot=127), dict(rot=130), dict(d=2048, rot=1026), dict(half=2), dict(i=None),
-                dict(o=None), dict(pos=None), dict(f=None), dict(ots=2048), dict(h=1 << 20, d=1 << 12)):
+                dict(o=None), dict(pos=None), dict(f=None), dict(ots=2048), dict(its=-1), dict(ihs=-8), dict(o=2 * P, ots=-1024), dict(o=2 * P, ohs=-1), dict(h=1 << 20, d=1 << 12)):
         refused(call(**bad))
     c = cache()
     for layer, rest in ((2, (None, P, P, 1.0, 1, 8, 128, 0)), (-1, (None, P, P, 1.0, 1, 8, 128, 0)), (0, (None, P, P, 1.0, 5, 8, 128, 0)),
@@ -107,6 +107,8 @@ def test_rotary_refuses():
         refused(lib.tl_rotary_append_f16(c, layer, P, P, P, P, *rest, 1024, 1024, 1024, None))
     refused(lib.tl_rotary_append_f16(c, 0, None, P, P, P, None, P, P, 1.0, 1, 8, 128, 0, 1024, 1024, 1024, None))
     refused(lib.tl_rotary_append_f16(c, 0, P, P, P, P, None, P, P, 1.0, 1, 8, 128, 0, 1024, 2048, 1024, None))
+    for strides in ((-1024, -1024, 1024), (1024, 1024, -1024)):
+        refused(lib.tl_rotary_append_f16(c, 0, P, P, P, P, None, P, P, 1.0, 1, 8, 128, 0, *strides, None))
 
 
 def test_attention_refuses():
@@ -119,6 +121,8 @@ def test_attention_refuses():
                 dict(scale=math.nan), dict(w=None), dict(w=P + 4), dict(c=cache(lengths=None)), dict(batch=65536, c=cache(n_rows=1 << 20))):
         refused(call(**bad))
     refused(call(c=cache(head_dim=264)), status=4)
+    for strides in ((-1024, 1024), (1024, -1024)):
+        refused(lib.tl_paged_attn_decode_f16(cache(), 0, P, P, None, None, 2, 8, 1.0, *strides, P, ws, None))
     need = C.c_size_t(0)
     for heads, kv, d in ((32, 32, 128), (64, 1, 256), (7, 7, 8), (128, 128, 256)):
         assert lib.tl_paged_attn_workspace(heads, kv, d, C.byref(need)) == 0 and need.value <= 32 << 20
@@ -143,7 +147,7 @@ def test_beam_calls_refuse():
     if need.value:
         refused(call(n=need.value - 1))
     for a in ((None, P, P, 1, 2, 8, 8, 8, 8, 8), (P, None, P, 1, 2, 8, 8, 8, 8, 8), (P, 2 * P, None, 1, 2, 8, 8, 8, 8, 8), (P, P, P, 1, 2, 8, 8, 8, 8, 8),
-              (P, 2 * P, P, -1, 2, 8, 8, 8, 8, 8), (P, 2 * P, P, 1, 2, 9, 8, 8, 16, 16), (P, 2 * P, P, 1, 2, 9, 16, 16, 8, 8)):
+              (P, 2 * P, P, -1, 2, 8, 8, 8, 8, 8), (P, 2 * P, P, 1, 2, 8, -8, 8, 8, 8), (P, 2 * P, P, 1, 2, 8, 8, 8, -8, 8), (P, 2 * P, P, 1, 2, 9, 8, 8, 16, 16), (P, 2 * P, P, 1, 2, 9, 16, 16, 8, 8)):
         refused(lib.tl_beam_reorder_f16(*a, None))
 
 
