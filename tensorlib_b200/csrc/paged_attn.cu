@@ -129,7 +129,7 @@ constexpr int FL_JOIN = 16;                       // pieces joined at a time
 constexpr int FL_MAX_SMS = 160;
 constexpr int FL_COUNTER_BYTES = 8192;
 
-struct FlashLaunch {
+struct TiledLaunch {
     AttnLaunch a;
     int chunk, chunks, groups;                    // query heads of a head group, head groups a KV head, head groups in all
     FastDiv by_grid;
@@ -139,7 +139,7 @@ struct FlashLaunch {
 };
 
 template <int HDP, int NT>
-struct FlashShape {
+struct TiledShape {
     // Stages of a warp's ring and CTAs an SM. More warps beat deeper rings where both keep some 100 KB under way: at 128
     // elements, 3 x 2 against 2 x 3, 32 sequences of 500..2000 tokens took 31.0 against 32.9 us, 256 of 1..100 21.0 against 25.6.
     static constexpr int STAGES = HDP <= 96 ? 3 : (HDP == 256 ? 3 : 2);
@@ -159,7 +159,7 @@ struct FlashShape {
 };
 
 // a partial result: [chunk][head_dim] sums, [chunk] (max, sum of weights), 16-byte aligned
-__host__ __device__ __forceinline__ long long flash_slot_floats(int chunk, int head_dim) { return ((long long)chunk * (head_dim + 2) + 3) / 4 * 4; }
+__host__ __device__ __forceinline__ long long tiled_slot_floats(int chunk, int head_dim) { return ((long long)chunk * (head_dim + 2) + 3) / 4 * 4; }
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
@@ -190,7 +190,7 @@ struct Cursor {
 __device__ __forceinline__ int units_of(int len) { return (len + FL_UNIT - 1) / FL_UNIT; }
 __device__ __forceinline__ int cost_of(int len) { return len > 0 ? units_of(len) + FL_START : 0; }
 
-__device__ __forceinline__ void advance(const FlashLaunch& p, Cursor& c) {
+__device__ __forceinline__ void advance(const TiledLaunch& p, Cursor& c) {
     if (--c.left <= 0) return;
     if (++c.i < c.units) return;
     c.left -= FL_START;
@@ -218,8 +218,8 @@ __device__ __forceinline__ bool last_to_arrive(unsigned int* counter, int expect
 }
 
 template <int HDP, int NT>
-__global__ void __launch_bounds__(FL_THREADS, FlashShape<HDP, NT>::CTAS) k_paged_attn(FlashLaunch p) {
-    using F = FlashShape<HDP, NT>;
+__global__ void __launch_bounds__(FL_THREADS, TiledShape<HDP, NT>::CTAS) k_paged_attn(TiledLaunch p) {
+    using F = TiledShape<HDP, NT>;
     extern __shared__ __align__(128) unsigned char sm[];
     float2* stats = reinterpret_cast<float2*>(sm + F::RING);                                 // [warp][head]: max, sum
     uint32_t* masks = reinterpret_cast<uint32_t*>(sm + F::RING + FL_WARPS * F::HEADS * 8);   // [warp][stage]
@@ -490,7 +490,7 @@ __global__ void __launch_bounds__(FL_THREADS, FlashShape<HDP, NT>::CTAS) k_paged
         }
         __syncthreads();
         const bool whole = seg_i == 0 && seg_units == seg_n;
-        const long long slot_floats = flash_slot_floats(p.chunk, hd);
+        const long long slot_floats = tiled_slot_floats(p.chunk, hd);
         float* part = p.partial + (2ll * blockIdx.x + (seg_i == 0)) * slot_floats;
         auto finish = [&](int h, int d, float4 x, float M, float L) {     // four elements of a head's result
             const float inv = L == 0.f ? 0.f : 1.f / L;                      // (a NaN stays one)
@@ -598,11 +598,11 @@ __global__ void __launch_bounds__(FL_THREADS, FlashShape<HDP, NT>::CTAS) k_paged
 }
 
 template <int HDP, int NT>
-int launch_flash(const FlashLaunch& p, cudaStream_t st) {
-    using F = FlashShape<HDP, NT>;
+int launch_tiled(const TiledLaunch& p, cudaStream_t st) {
+    using F = TiledShape<HDP, NT>;
     static PerDeviceOnce once;
     if (once.needed()) TL_CUDA(cudaFuncSetAttribute(k_paged_attn<HDP, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::SMEM));
-    FlashLaunch q = p;
+    TiledLaunch q = p;
     const int grid = (sm_count() < FL_MAX_SMS ? sm_count() : FL_MAX_SMS) * F::CTAS;
     q.by_grid = FastDiv((unsigned)grid);
     return launch_pdl(k_paged_attn<HDP, NT>, grid, FL_THREADS, F::SMEM, st, true, q);
@@ -610,7 +610,7 @@ int launch_flash(const FlashLaunch& p, cudaStream_t st) {
 
 // query heads of a head group: as few groups as 16 columns allow (8 at 256 elements a head, where 16 would not fit the
 // registers), of even size
-int flash_chunk(int group, int head_dim) {
+int tiled_chunk(int group, int head_dim) {
     const int most = head_dim > 128 ? 8 : 16;
     const int chunks = (group + most - 1) / most;
     return (group + chunks - 1) / chunks;
@@ -619,11 +619,11 @@ int flash_chunk(int group, int head_dim) {
 }  // namespace
 
 size_t paged_attn_workspace_bytes(int n_heads, int n_kv_heads, int head_dim) {
-    const int ctas = FL_MAX_SMS * (head_dim <= 64 ? FlashShape<64, 1>::CTAS : (head_dim <= 128 ? FlashShape<128, 1>::CTAS :
-                                   (head_dim <= 192 ? FlashShape<192, 1>::CTAS : FlashShape<256, 1>::CTAS)));
-    static_assert(FlashShape<96, 1>::CTAS == FlashShape<128, 1>::CTAS, "one formula for both");
-    static_assert(3 * FL_MAX_SMS * FlashShape<64, 1>::CTAS * 4 <= FL_COUNTER_BYTES, "counters");
-    return FL_COUNTER_BYTES + 4 * (size_t)ctas * flash_slot_floats(flash_chunk(n_heads / n_kv_heads, head_dim), head_dim) * 4;
+    const int ctas = FL_MAX_SMS * (head_dim <= 64 ? TiledShape<64, 1>::CTAS : (head_dim <= 128 ? TiledShape<128, 1>::CTAS :
+                                   (head_dim <= 192 ? TiledShape<192, 1>::CTAS : TiledShape<256, 1>::CTAS)));
+    static_assert(TiledShape<96, 1>::CTAS == TiledShape<128, 1>::CTAS, "one formula for both");
+    static_assert(3 * FL_MAX_SMS * TiledShape<64, 1>::CTAS * 4 <= FL_COUNTER_BYTES, "counters");
+    return FL_COUNTER_BYTES + 4 * (size_t)ctas * tiled_slot_floats(tiled_chunk(n_heads / n_kv_heads, head_dim), head_dim) * 4;
 }
 
 int launch_paged_attn(const PagedView& c, const PagedAttnArgs& a, cudaStream_t st) {
@@ -642,19 +642,19 @@ int launch_paged_attn(const PagedView& c, const PagedAttnArgs& a, cudaStream_t s
     const long long cost = ((long long)c.max_pages * c.page_size + FL_UNIT - 1) / FL_UNIT + FL_START;
     if (cost * a.batch * a.n_heads >= (1ll << 31) - 1024)
         return set_error(TL_ERR_UNSUPPORTED, "paged_attn_decode: batch * n_heads * (max_pages * page_size / 64 + 3) has to stay below 2^31");
-    FlashLaunch f{};
+    TiledLaunch f{};
     f.a = p;
-    f.chunk = flash_chunk(p.group, p.head_dim);
+    f.chunk = tiled_chunk(p.group, p.head_dim);
     f.chunks = (p.group + f.chunk - 1) / f.chunk;
     f.groups = p.n_kv * f.chunks;
     f.scale_log2 = a.scale * 1.4426950408889634f;
     f.out8 = (reinterpret_cast<uintptr_t>(a.out) & 7) == 0 && a.o_row % 4 == 0;
     f.counters = static_cast<unsigned int*>(a.work);
     f.partial = reinterpret_cast<float*>(static_cast<char*>(a.work) + FL_COUNTER_BYTES);
-    if (p.head_dim <= 64) return f.chunk <= 8 ? launch_flash<64, 1>(f, st) : launch_flash<64, 2>(f, st);
-    if (p.head_dim <= 96) return f.chunk <= 8 ? launch_flash<96, 1>(f, st) : launch_flash<96, 2>(f, st);
-    if (p.head_dim <= 128) return f.chunk <= 8 ? launch_flash<128, 1>(f, st) : launch_flash<128, 2>(f, st);
-    return p.head_dim <= 192 ? launch_flash<192, 1>(f, st) : launch_flash<256, 1>(f, st);
+    if (p.head_dim <= 64) return f.chunk <= 8 ? launch_tiled<64, 1>(f, st) : launch_tiled<64, 2>(f, st);
+    if (p.head_dim <= 96) return f.chunk <= 8 ? launch_tiled<96, 1>(f, st) : launch_tiled<96, 2>(f, st);
+    if (p.head_dim <= 128) return f.chunk <= 8 ? launch_tiled<128, 1>(f, st) : launch_tiled<128, 2>(f, st);
+    return p.head_dim <= 192 ? launch_tiled<192, 1>(f, st) : launch_tiled<256, 1>(f, st);
 }
 
 }  // namespace tlb
