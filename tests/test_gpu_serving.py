@@ -602,6 +602,89 @@ def test_a_beam_search_over_pages_matches_one_over_copied_sequences(tl):
     assert tl.device_status() == 0
 
 
+def test_a_whole_step_replayed_from_a_graph(tl):
+    """Fork, reserve, append, attend, select and compact captured once and replayed: the books move on with every replay."""
+    torch = pytest.importorskip("torch")
+    r = np.random.default_rng(52)
+    lib = tl.load()
+    rows, page, kv, heads, hd, width, pages = 6, 4, 2, 4, 32, 8, 60
+    c, pg = tl.PagedCache(1, pages, page, kv, hd, rows, width), so.Pages(pages, page, rows, width)
+    k, v = c.pools()
+    assert c.reserve([3, 0, 5, 0, 1, 0]) == pg.reserve([3, 0, 5, 0, 1, 0])[0] == 0
+    parents, ones = np.array([0, 0, 2, 2, 4, 4], np.int32), np.ones(rows, np.int32)
+    need, bneed, aneed = C.c_size_t(0), C.c_size_t(0), C.c_size_t(0)
+    tl.check(lib.tl_paged_workspace(rows, pages, C.byref(need)), "ws")
+    tl.check(lib.tl_beam_select_workspace(3, 2, 90, 2, C.byref(bneed)), "ws")
+    tl.check(lib.tl_paged_attn_workspace(heads, kv, hd, C.byref(aneed)), "ws")
+    cuda = lambda a: torch.from_numpy(np.ascontiguousarray(a)).cuda()  # noqa: E731
+    t = dict(par=cuda(parents), one=cuda(ones), pos=cuda(np.zeros(rows, np.int32)), res=cuda(np.zeros(4, np.int32)), moved=cuda(np.zeros(pages, np.int32)),
+             q=cuda(normal(r, rows, heads, hd)), k=cuda(normal(r, rows, kv, hd)), v=cuda(normal(r, rows, kv, hd)), x=cuda(normal(r, rows, 90, std=2)),
+             s=torch.zeros(rows, device="cuda"), f=cuda(tl.rotary_frequencies(hd)[0]), o=torch.zeros(rows, heads, hd, dtype=torch.float16, device="cuda"),
+             qo=torch.zeros(rows, heads, hd, dtype=torch.float16, device="cuda"), sc=torch.zeros(3, 2, device="cuda"),
+             ip=torch.zeros(3, 2, dtype=torch.int32, device="cuda"), it=torch.zeros(3, 2, dtype=torch.int32, device="cuda"),
+             w=torch.zeros(need.value, dtype=torch.uint8, device="cuda"), bw=torch.zeros(max(16, bneed.value), dtype=torch.uint8, device="cuda"),
+             aw=torch.zeros(max(16, aneed.value), dtype=torch.uint8, device="cuda"))
+    p = {n: a.data_ptr() for n, a in t.items()}
+    cc = C.byref(c.c)
+    lengths = torch.zeros(rows, dtype=torch.int32, device="cuda")
+
+    def step(st):
+        tl.check(lib.tl_paged_fork(cc, p["par"], st), "fork")
+        tl.check(lib.tl_paged_reserve_f16(cc, p["one"], p["res"], p["w"], t["w"].numel(), st), "reserve")
+        tl.check(lib.tl_memcpy_d2d(lengths.data_ptr(), c._lengths.ptr, 4 * rows, st), "lengths")
+        torch.sub(lengths, t["one"], out=t["pos"])                    # the new token's position
+        tl.check(lib.tl_rotary_append_f16(cc, 0, p["q"], p["qo"], p["k"], p["v"], None, p["pos"], p["f"], 1.0, rows, heads, hd, 1, heads * hd, heads * hd,
+                                          kv * hd, st), "append")
+        tl.check(lib.tl_paged_attn_decode_f16(cc, 0, p["qo"], p["o"], None, None, rows, heads, hd ** -0.5, heads * hd, heads * hd, p["aw"], t["aw"].numel(), st), "attn")
+        tl.check(lib.tl_beam_select_f16(p["x"], 90, p["s"], None, 0, 3, 2, 90, 2, p["sc"], p["ip"], p["it"], p["bw"], t["bw"].numel(), st), "select")
+        tl.check(lib.tl_paged_compact_f16(cc, p["moved"], p["res"] + 4, p["w"], t["w"].numel(), st), "compact")
+
+    torch.cuda.synchronize()
+    g, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(g, stream=stream):
+        step(torch.cuda.current_stream().cuda_stream)
+    nk, nv, q = (t[n].cpu().numpy() for n in ("k", "v", "q"))
+    f = tl.rotary_frequencies(hd)[0]
+    for rep in range(5):
+        g.replay()
+        torch.cuda.synchronize()
+        pg.fork(parents)
+        status, copies = pg.reserve(ones)
+        assert status == 0 and t["res"].cpu().numpy()[0] == 0
+        for s, d, n in copies:
+            k[:, d, :n], v[:, d, :n] = k[:, s, :n], v[:, s, :n]
+        pos = pg.lengths - 1
+        wk, tk = so.rotary(nk, pos, f, 1.0, True)
+        for i in range(rows):
+            at = (0, pg.table[i, pos[i] // page], pos[i] % page)
+            k[at], v[at] = wk[i].astype(np.float16), nv[i]
+        wq, tq = so.rotary(q, pos, f, 1.0, True)
+        close(t["qo"].cpu().numpy(), wq, tq)
+        before = pg.table.copy()
+        moved, live, moves = pg.compact()
+        kk, vv = k.copy(), v.copy()
+        for s, d in moves:
+            k[:, d], v[:, d] = k[:, s], v[:, s]
+        same_books(c, pg)
+        assert np.array_equal(t["moved"].cpu().numpy(), moved) and t["res"].cpu().numpy()[1] == live
+        gk, gv = c.pools()
+        for i in range(rows):                     # what the rows hold: values bit for bit, keys to their rounding
+            n = pg.lengths[i]
+            assert np.array_equal(row_tokens(gv[0], pg.table[i], n, page), row_tokens(v[0], pg.table[i], n, page))
+            d = row_tokens(gk[0], pg.table[i], n, page).astype(np.float64) - row_tokens(k[0], pg.table[i], n, page).astype(np.float64)
+            assert (np.abs(d) <= 2 * so.EPS16 * np.abs(row_tokens(k[0], pg.table[i], n, page).astype(np.float64)) + 2.0 ** -18).all()
+        k[0], v[0] = gk[0], gv[0]
+        for i in range(rows):
+            keys, vals = row_tokens(k[0], pg.table[i], pg.lengths[i], page), row_tokens(v[0], pg.table[i], pg.lengths[i], page)
+            for h in range(heads):
+                o, l, to, _ = so.attend(t["qo"].cpu().numpy()[i, h], keys[:, h // 2], vals[:, h // 2], hd ** -0.5)
+                close(t["o"].cpu().numpy()[i, h], o, to, (rep, i, h))
+        want = so.beam_select(t["x"].cpu().numpy(), np.zeros(rows), 2, 2)
+        assert np.array_equal(t["it"].cpu().numpy(), want[2]) and np.array_equal(t["ip"].cpu().numpy(), want[1])
+    del g
+    assert tl.device_status() == 0
+
+
 def test_on_two_streams_and_from_a_graph(tl):
     """The calls enqueue on the stream that they are given; captured once, replayed on changed inputs."""
     torch = pytest.importorskip("torch")
