@@ -355,7 +355,7 @@ TL_API int tl_rotary_append_f16(const tl_paged_cache* cache, int layer, const tl
  * rows[b]: the row of entry b, -1 for a padding entry (rows == NULL: row b). lse, if not NULL: fp32 [batch, n_heads],
  * log sum_t exp(scale q_h.k_t). An empty row gives zeros and -inf. head_dim <= 256, and batch * n_heads * (max_pages * page_size / 64 + 3)
  * has to stay below 2^31 (TL_ERR_UNSUPPORTED). workspace: tl_paged_attn_workspace bytes (at
- * most 32 MB), zeroed once before its first use; calls leave it as the next one needs it. */
+ * most 32 MB), zeroed once before its first use; calls leave it as the next one needs it, whatever that one's sizes. */
 TL_API int tl_paged_attn_decode_f16(const tl_paged_cache* cache, int layer, const tl_half* q, tl_half* out, float* lse, const int* rows,
                                     int batch, int n_heads, float scale, long long q_row_stride, long long out_row_stride,
                                     void* workspace, size_t workspace_bytes, tl_stream stream);
@@ -368,7 +368,7 @@ TL_API int tl_paged_attn_workspace(int n_heads, int n_kv_heads, int head_dim, si
  * finished (may be NULL): a beam with finished[row] != 0 has one candidate, pad_token, at its score; its logits are not used. A score
  * of -inf makes a dead beam; NaN logits count as -inf and +inf as 65504, NaN scores as -inf. beams, k <= 128. out_scores may be
  * scores where k == beams. workspace:
- * tl_beam_select_workspace bytes, zeroed once before its first use. */
+ * tl_beam_select_workspace bytes, zeroed once before its first use; it serves calls of any sizes that ask for no more. */
 TL_API int tl_beam_select_f16(const tl_half* logits, long long row_stride, const float* scores, const unsigned char* finished,
                               int pad_token, int batch, int beams, int vocab, int k, float* out_scores, int* out_parents,
                               int* out_tokens, void* workspace, size_t workspace_bytes, tl_stream stream);

@@ -108,6 +108,8 @@ constexpr int SEL_LONG = 1024;                    // a list of values longer tha
 constexpr int SEL_MAX_SPLITS = 32;                // a lane each in the join
 constexpr int SEL_MAX_CHUNK = 65536;              // indices in a chunk have 16 bits
 constexpr int SEL_MAX_MERGE = 8192;               // candidates that one CTA joins
+constexpr int SEL_ENTRIES = 4096;                 // batch entries of a launch: their counters have a place of their own in the workspace,
+                                                  // so that calls of other sizes never find results where they expect a counter at 0
 
 struct SelStat { double sum; float max; float pad; };
 
@@ -115,7 +117,8 @@ struct SelLaunch {
     BeamArgs a;
     int splits, chunk;                            // chunks of a row, logits of a chunk (a multiple of 8)
     int groups;                                   // the power of two from 8 to 128 at or above k
-    unsigned int* counters; SelStat* stats; unsigned int* keys;     // [batch], [row][split], [row][split][k]
+    int row0;                                     // row of the whole call that this launch begins with
+    unsigned int* counters; SelStat* stats; unsigned int* keys;     // [SEL_ENTRIES], [row][split], [row][split][k]
 };
 
 // order of fp16 values as 16-bit integers; 0 stands below every value
@@ -527,7 +530,7 @@ __global__ void __launch_bounds__(SEL_THREADS, 4) k_beam_select(SelLaunch p) {
             const long long at = (long long)entry * a.k + rank;
             const unsigned w = x / (unsigned)a.vocab;
             a.out_scores[at] = (float)ord64_value(o);
-            a.out_parents[at] = entry * a.beams + (int)w;
+            a.out_parents[at] = p.row0 + entry * a.beams + (int)w;
             a.out_tokens[at] = (int)(x - w * (unsigned)a.vocab);
         }
     }
@@ -559,8 +562,8 @@ int launch_sel(const SelLaunch& p, cudaStream_t st) {
 
 size_t beam_workspace_bytes(int batch, int beams, int vocab, int k) {
     const int splits = sel_splits(batch > 0 ? batch : 1, beams, vocab, k);
-    const size_t rows = (size_t)batch * beams;
-    return ((size_t)batch * 4 + 15) / 16 * 16 + rows * splits * (sizeof(SelStat) + 4 * (size_t)k);
+    const size_t rows = (size_t)(batch < SEL_ENTRIES ? batch : SEL_ENTRIES) * beams;
+    return SEL_ENTRIES * 4 + rows * splits * (sizeof(SelStat) + 4 * (size_t)k);
 }
 
 int launch_beam_select(const BeamArgs& a, cudaStream_t st) {
@@ -568,18 +571,30 @@ int launch_beam_select(const BeamArgs& a, cudaStream_t st) {
     SelLaunch p{};
     p.a = a;
     p.splits = sel_splits(a.batch, a.beams, a.vocab, a.k);
-    if (p.splits == 0 || (long long)a.batch * a.beams * p.splits >= (1ll << 31))
+    if (p.splits == 0)
         return launch_pdl(k_beam_any, a.batch, BEAM_THREADS, (size_t)a.beams * 16, st, true, a);
     p.chunk = sel_chunk(a.vocab, p.splits);
     p.groups = 8;
     while (p.groups < a.k) p.groups *= 2;
     char* w = static_cast<char*>(a.work);
-    const size_t lists = (size_t)a.batch * a.beams * p.splits;
+    const int most = a.batch < SEL_ENTRIES ? a.batch : SEL_ENTRIES;
     p.counters = reinterpret_cast<unsigned int*>(w);
-    p.stats = reinterpret_cast<SelStat*>(w + ((size_t)a.batch * 4 + 15) / 16 * 16);
-    p.keys = reinterpret_cast<unsigned int*>(p.stats + lists);
-    // one vector a thread where that covers the chunk: the shortest chain; else four, loaded ahead
-    return p.chunk <= SEL_THREADS * 8 ? launch_sel<1>(p, st) : launch_sel<4>(p, st);
+    p.stats = reinterpret_cast<SelStat*>(w + SEL_ENTRIES * 4);
+    p.keys = reinterpret_cast<unsigned int*>(p.stats + (size_t)most * a.beams * p.splits);
+    for (int e0 = 0; e0 < a.batch; e0 += most) {  // launches behind one another share the workspace
+        p.row0 = e0 * a.beams;
+        p.a.batch = a.batch - e0 < most ? a.batch - e0 : most;
+        p.a.logits = a.logits + (long long)p.row0 * a.pitch;
+        p.a.scores = a.scores + p.row0;
+        p.a.finished = a.finished ? a.finished + p.row0 : nullptr;
+        p.a.out_scores = a.out_scores + (long long)e0 * a.k;
+        p.a.out_parents = a.out_parents + (long long)e0 * a.k;
+        p.a.out_tokens = a.out_tokens + (long long)e0 * a.k;
+        // one vector a thread where that covers the chunk: the shortest chain; else four, loaded ahead
+        TL_PROPAGATE(p.chunk <= SEL_THREADS * 8 ? launch_sel<1>(p, st) : launch_sel<4>(p, st));
+        if (a.batch - e0 <= most) break;          // (e0 may not pass 2^31 - 1)
+    }
+    return TL_OK;
 }
 
 }  // namespace tlb

@@ -531,6 +531,33 @@ def test_beam_selection_with_row_strides(tl, stride, off):
     assert np.array_equal(outs[1].to_numpy(np.int32, (2, k)), want[1]) and np.array_equal(outs[2].to_numpy(np.int32, (2, k)), want[2])
 
 
+def test_beam_selection_of_other_sizes_in_the_same_workspace(tl):
+    """Zeroed once, then calls of any sizes: what one leaves behind is no counter of the next. More entries than one launch takes as well."""
+    shapes = [(2, 4, 5000, 4), (300, 3, 40, 3), (2, 4, 5000, 4), (4100, 2, 17, 5), (1, 8, 30000, 128), (9001, 1, 9, 9), (64, 8, 600, 16)]
+    lib, need = tl.load(), C.c_size_t(0)
+    size = 16
+    for batch, beams, vocab, k in shapes:
+        tl.check(lib.tl_beam_select_workspace(batch, beams, vocab, k, C.byref(need)), "ws")
+        size = max(size, need.value)
+    w = tl.DeviceBuffer.from_numpy(np.zeros(size, np.uint8))
+    for n, (batch, beams, vocab, k) in enumerate(shapes):
+        r = np.random.default_rng([33, n])
+        x, s = normal(r, batch * beams, vocab, std=3), -r.random(batch * beams).astype(np.float32)
+        fin = (r.random(batch * beams) < 0.2).astype(np.uint8)
+        dx, ds, df = (tl.DeviceBuffer.from_numpy(a) for a in (x, s, fin))
+        out = [tl.DeviceBuffer.from_numpy(np.full(batch * k, -7, np.int32)) for _ in range(3)]
+        tl.check(lib.tl_beam_select_f16(dx.ptr, vocab, ds.ptr, df.ptr, 1, batch, beams, vocab, k, *(o.ptr for o in out), w.ptr, w.nbytes, None), "select")
+        values = so.beam_values(x, s, fin, 1).reshape(batch, beams * vocab)
+        parents, tokens = (o.to_numpy(np.int32, (batch, k)) for o in out[1:])
+        at = (parents - np.arange(batch)[:, None] * beams).astype(np.int64) * vocab + tokens
+        assert at.min() >= 0 and at.max() < beams * vocab and all(len(set(a)) == k for a in at), n
+        # values nearer to one another than the logs of the sums are good to may change places
+        got, want = np.take_along_axis(values, at, 1), -np.sort(-values, axis=1)[:, :k]
+        with np.errstate(invalid="ignore"):
+            assert ((got == want) | (np.abs(got - want) <= 2.0 ** -20)).all(), n
+        close(out[0].to_numpy(np.float32, (batch, k)), got, np.abs(got) * 2.0 ** -24 + 2.0 ** -21, n)
+
+
 @pytest.mark.parametrize("outer,rows,pitch,used", [(1, 1, 8, 8), (2, 5, 24, 17), (3, 4, 70000, 69993), (2, 7, 33, 33), (4, 64, 4096, 1000)])
 def test_beam_reorder(tl, outer, rows, pitch, used):
     r = np.random.default_rng([outer, rows, pitch])
