@@ -22,6 +22,7 @@ int check_cache(const tl_paged_cache* c, bool pools, const char* who) {
     TL_REQUIRE(c->n_layers > 0 && c->n_pages > 0 && c->page_size > 0 && c->n_kv_heads > 0 && c->head_dim > 0 && c->n_rows > 0 &&
                    c->max_pages > 0, "%s: cache sizes must be positive", who);
     TL_REQUIRE((long long)c->max_pages * c->page_size <= (1ll << 31) - 128, "%s: a row of more than 2^31 - 128 tokens", who);
+    TL_REQUIRE(c->n_rows < (1 << 28), "%s: 2^28 rows or more", who);
     TL_REQUIRE(c->page_table, "%s: null page table", who);
     if (pools) {
         TL_REQUIRE(c->k_pages && c->v_pages, "%s: null page pool", who);

@@ -205,6 +205,9 @@ __global__ void __launch_bounds__(RES_THREADS, 1) k_reserve(PagedView c, const i
     const int per = (c.n_rows + RES_THREADS - 1) / RES_THREADS;
     const int r0 = min(c.n_rows, tid * per), r1 = min(c.n_rows, r0 + per);
     constexpr int WRITES = 1 << 30, COPY = 1 << 29;
+    // copies and pages are summed in one number: a table of 2^36 entries is more than any memory, and there are fewer than 2^28 rows
+    constexpr int COPIES = 36;
+    constexpr unsigned long long PAGES = (1ull << COPIES) - 1;
     struct Row { int len, add, pages, slot, last, flag; };     // pages that it holds, slots used of the last one, its id
     auto read = [&](int r) {
         Row x;
@@ -259,11 +262,11 @@ __global__ void __launch_bounds__(RES_THREADS, 1) k_reserve(PagedView c, const i
     if (r0 < r1) claim(r0, mine);
     for (int r = r0 + 1; r < r1; r++) claim(r, again(r));
     __syncthreads();
-    unsigned long long wants = 0;                 // copies in the upper half, pages in the lower
+    unsigned long long wants = 0;                 // copies from bit COPIES up, pages below
     auto count = [&](int r, Row& x) {
         if ((x.flag & WRITES) && __ldcg(c.refs + x.last) != -(r + 1)) {
             x.flag |= COPY;
-            wants += (1ull << 32) + 1;
+            wants += (1ull << COPIES) + 1;
         }
         if (x.add > 0 && x.len >= 0 && (long long)x.len + x.add <= (long long)c.max_pages * c.page_size)
             wants += (unsigned)((int)c.by_page.div((unsigned)(x.len + x.add - 1)) + 1 - x.pages);
@@ -277,7 +280,7 @@ __global__ void __launch_bounds__(RES_THREADS, 1) k_reserve(PagedView c, const i
     // 3: the keepers' counts are 1 again (after the barrier in the sum: everyone has looked)
     unsigned long long total;
     const unsigned long long before = block_scan(wants, sums, total);
-    const int pages_wanted = (int)(total & 0xffffffffu);
+    const long long pages_wanted = (long long)(total & PAGES);
     auto keep = [&](const Row& x) {
         if ((x.flag & (WRITES | COPY)) == WRITES) atomicExch(c.refs + x.last, 1);
     };
@@ -322,7 +325,7 @@ __global__ void __launch_bounds__(RES_THREADS, 1) k_reserve(PagedView c, const i
     }
     __syncthreads();
     // 5: hand them out, rows in order: a row's copy first, then its new pages
-    int at = (int)(before & 0xffffffffu), copy_at = (int)(before >> 32);
+    int at = (int)(before & PAGES), copy_at = (int)(before >> COPIES);         // there are that many pages: it fits
     auto hand_out = [&](int r, const Row& x) {
         if (x.add <= 0) return;
         int* row = c.table + (long long)r * c.max_pages;
@@ -344,7 +347,7 @@ __global__ void __launch_bounds__(RES_THREADS, 1) k_reserve(PagedView c, const i
     for (int r = r0 + 1; r < r1; r++) hand_out(r, again(r));
     if (tid == 0) {
         *result = TL_OK;
-        *wk.n_copies = (int)(total >> 32);
+        *wk.n_copies = (int)(total >> COPIES);
     }
 }
 

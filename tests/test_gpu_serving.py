@@ -415,6 +415,27 @@ def test_pages_refuse_without_changing_anything(tl):
     assert tl.device_status() == 1
 
 
+def test_pages_wanted_beyond_32_bits_are_refused(tl):
+    """4096 rows that ask for 2^20 pages each, of a table of 16 GB: 2^32 in all, which 32 bits hold as 0."""
+    rows, width = 4096, 1 << 20
+    c = tl.PagedCache(1, 64, 1, 1, 8, rows, 4)
+    lib, big = tl.load(), tl.DeviceBuffer(4 * rows * width)
+    tl.check(lib.tl_memset(big.ptr, 0xff, big.nbytes, None), "memset")
+    c.c.page_table, c.c.max_pages = big.ptr, width
+    for new in (np.full(rows, width), np.r_[np.full(rows - 1, width), 5]):
+        assert c.reserve(new) == 5
+        assert (c._lengths.to_numpy(np.int32, (rows,)) == 0).all() and (c._refs.to_numpy(np.int32, (64,)) == 0).all()
+    new = np.zeros(rows)
+    new[[0, rows - 1]] = [3, 60]
+    assert c.reserve(new) == 0
+    head, tail = np.empty(4, np.int32), np.empty(61, np.int32)
+    tl.check(lib.tl_memcpy_d2h(tl._np_ptr(head), big.ptr, head.nbytes, None), "d2h")
+    tl.check(lib.tl_memcpy_d2h(tl._np_ptr(tail), big.ptr + 4 * (rows - 1) * width, tail.nbytes, None), "d2h")
+    tl.synchronize()
+    assert head.tolist() == [0, 1, 2, -1] and tail.tolist() == list(range(3, 63)) + [-1]
+    assert tl.device_status() == 0
+
+
 @pytest.mark.parametrize("shape,by_head", [((2, 30, 16, 4, 64), False), ((3, 12, 5, 3, 7), False), ((1, 40, 8, 2, 24), True)])
 def test_page_copies(tl, shape, by_head):
     r = np.random.default_rng(21)
