@@ -501,6 +501,14 @@ def cast(x: np.ndarray, to) -> np.ndarray:
 ROPE_SCALINGS = {"unscaled": 0, "linear": 1, "base": 2, "parts": 3, "ramp": 4}
 
 
+def _shaped(a, dtype, shape, what: str) -> np.ndarray:
+    """a as a contiguous array of that shape; a kernel trusts the sizes that it is told. fp16 operands are not converted."""
+    a = np.asarray(a)
+    if a.shape != tuple(shape) or (dtype == np.float16 and a.dtype != dtype):
+        raise ValueError(f"{what}: {a.dtype}{list(a.shape)}, expected {np.dtype(dtype)}{list(shape)}")
+    return np.ascontiguousarray(a, dtype=dtype)
+
+
 def rotary_frequencies(rot_dim: int, base: float = 10000.0, scaling: str = "unscaled", factor: float = 1.0,
                        trained_len: float = 0.0, low: float = 0.0, high: float = 0.0):
     """Host only: (radians a position for each pair as float64, magnitude) for tl_rotary_f16."""
@@ -515,7 +523,9 @@ def rotary(x: np.ndarray, positions, freqs: np.ndarray, magnitude: float = 1.0, 
     """x [tokens, heads, head_dim] with the first 2 * len(freqs) elements of each head turned by their token's position
     (tl_rotary_f16). Tokens at negative positions keep what `out` (default zeros) held."""
     T, Hh, hd = x.shape
-    pos = np.ascontiguousarray(positions, dtype=np.int32)
+    x, pos = _shaped(x, np.float16, x.shape, "rotary x"), _shaped(positions, np.int32, (T,), "rotary positions")
+    if out is not None:
+        out = _shaped(out, np.float16, x.shape, "rotary out")
     dx, dp, df = DeviceBuffer.from_numpy(x), DeviceBuffer.from_numpy(pos), DeviceBuffer.from_numpy(np.asarray(freqs, np.float64))
     do = dx if in_place else DeviceBuffer.from_numpy(np.zeros_like(x) if out is None else out)
     check(load().tl_rotary_f16(dx.ptr, do.ptr, dp.ptr, df.ptr, magnitude, T, Hh, hd, 2 * len(freqs), int(half_layout), int(inverse),
@@ -531,7 +541,8 @@ class PagedCache:
                  by_head: bool = False, k: np.ndarray | None = None, v: np.ndarray | None = None):
         self.shape, self.by_head = (n_layers, n_pages, page_size, n_kv_heads, head_dim), by_head
         zeros = np.zeros(self.shape, np.float16)
-        self._k, self._v = (DeviceBuffer.from_numpy(self._stored(zeros if a is None else a)) for a in (k, v))
+        self._k, self._v = (DeviceBuffer.from_numpy(self._stored(zeros if a is None else _shaped(a, np.float16, self.shape, "page pool")))
+                            for a in (k, v))
         self._table = DeviceBuffer.from_numpy(np.full((n_rows, max_pages), -1, np.int32))
         self._lengths, self._refs = (DeviceBuffer.from_numpy(np.zeros(n, np.int32)) for n in (n_rows, n_pages))
         page = page_size * n_kv_heads * head_dim
@@ -552,8 +563,9 @@ class PagedCache:
         return tuple(a.swapaxes(2, 3) if self.by_head else a for a in got)
 
     def set_state(self, table, lengths, refs) -> None:
-        for buf, a in ((self._table, table), (self._lengths, lengths), (self._refs, refs)):
-            a = np.ascontiguousarray(a, dtype=np.int32)
+        n, w = self.c.n_rows, self.c.max_pages
+        state = [_shaped(a, np.int32, s, "cache state") for a, s in ((table, (n, w)), (lengths, (n,)), (refs, (self.c.n_pages,)))]
+        for buf, a in zip((self._table, self._lengths, self._refs), state):
             check(load().tl_memcpy_h2d(buf.ptr, _np_ptr(a), a.nbytes, None), "tl_memcpy_h2d")
             synchronize()
 
@@ -563,19 +575,20 @@ class PagedCache:
                 self._refs.to_numpy(np.int32, (self.c.n_pages,)))
 
     def fork(self, parents) -> None:
-        d = DeviceBuffer.from_numpy(np.ascontiguousarray(parents, dtype=np.int32))
+        d = DeviceBuffer.from_numpy(_shaped(parents, np.int32, (self.c.n_rows,), "parents"))
         check(load().tl_paged_fork(C.byref(self.c), d.ptr, None), "tl_paged_fork")
         synchronize()
 
     def reserve(self, new_tokens) -> int:
         """The status that the device found: 0, or why no row has changed."""
-        d = DeviceBuffer.from_numpy(np.ascontiguousarray(new_tokens, dtype=np.int32))
+        d = DeviceBuffer.from_numpy(_shaped(new_tokens, np.int32, (self.c.n_rows,), "new tokens"))
         check(load().tl_paged_reserve_f16(C.byref(self.c), d.ptr, self._result.ptr, self._work.ptr, self._work.nbytes, None),
               "tl_paged_reserve_f16")
         return int(self._result.to_numpy(np.int32, (1,))[0])
 
     def copy(self, src, dst) -> None:
-        s, d = (DeviceBuffer.from_numpy(np.ascontiguousarray(a, dtype=np.int32)) for a in (src, dst))
+        pages = [_shaped(a, np.int32, (len(src),), "pages") for a in (src, dst)]
+        s, d = (DeviceBuffer.from_numpy(a) for a in pages)
         check(load().tl_paged_copy_f16(C.byref(self.c), s.ptr, d.ptr, len(src), None), "tl_paged_copy_f16")
         synchronize()
 
@@ -591,11 +604,14 @@ class PagedCache:
         T = k.shape[0]
         heads = 0 if q is None else q.shape[1]
         kv, hd = self.shape[3], self.shape[4]
+        k, v = (_shaped(a, np.float16, (T, kv, hd), "keys and values") for a in (k, v))
+        q = None if q is None else _shaped(q, np.float16, (T, heads, hd), "queries")
+        positions, rows = _shaped(positions, np.int32, (T,), "positions"), None if rows is None else _shaped(rows, np.int32, (T,), "rows")
         dk, dv = DeviceBuffer.from_numpy(k), DeviceBuffer.from_numpy(v)
         dq = None if q is None else DeviceBuffer.from_numpy(q)
         do = None if q is None else DeviceBuffer.from_numpy(np.zeros_like(q))
-        dp = DeviceBuffer.from_numpy(np.ascontiguousarray(positions, dtype=np.int32))
-        dr = None if rows is None else DeviceBuffer.from_numpy(np.ascontiguousarray(rows, dtype=np.int32))
+        dp = DeviceBuffer.from_numpy(positions)
+        dr = None if rows is None else DeviceBuffer.from_numpy(rows)
         df = None if freqs is None else DeviceBuffer.from_numpy(np.asarray(freqs, np.float64))
         ptr = lambda b: b.ptr if b is not None else None  # noqa: E731
         check(load().tl_rotary_append_f16(C.byref(self.c), layer, ptr(dq), ptr(do), dk.ptr, dv.ptr, ptr(dr), dp.ptr, ptr(df), magnitude, T,
@@ -607,13 +623,14 @@ class PagedCache:
     def attend(self, layer: int, q: np.ndarray, scale: float | None = None, rows=None):
         """tl_paged_attn_decode_f16: q [batch, heads, head_dim] -> (out, lse)."""
         B, Hh, hd = q.shape
+        q, rows = _shaped(q, np.float16, (B, Hh, self.shape[4]), "queries"), None if rows is None else _shaped(rows, np.int32, (B,), "rows")
         if self._attn_work is None or self._attn_work[0] != Hh:
             need = _sz(0)
             check(load().tl_paged_attn_workspace(Hh, self.shape[3], hd, C.byref(need)), "tl_paged_attn_workspace")
             self._attn_work = (Hh, DeviceBuffer.from_numpy(np.zeros(max(need.value, 16), np.uint8)))
         w = self._attn_work[1]
         dq, do, dl = DeviceBuffer.from_numpy(q), DeviceBuffer(max(2 * q.size, 2)), DeviceBuffer(max(4 * B * Hh, 4))
-        dr = None if rows is None else DeviceBuffer.from_numpy(np.ascontiguousarray(rows, dtype=np.int32))
+        dr = None if rows is None else DeviceBuffer.from_numpy(rows)
         check(load().tl_paged_attn_decode_f16(C.byref(self.c), layer, dq.ptr, do.ptr, dl.ptr, dr.ptr if dr is not None else None, B, Hh,
                                               hd ** -0.5 if scale is None else scale, Hh * hd, Hh * hd, w.ptr, w.nbytes, None),
               "tl_paged_attn_decode_f16")
@@ -623,12 +640,15 @@ class PagedCache:
 def beam_select(logits: np.ndarray, scores, beams: int, k: int, finished=None, pad_token: int = 0):
     """logits [batch * beams, vocab] fp16, scores [batch * beams]: (scores, parent rows, tokens), each [batch, k]."""
     rows, vocab = logits.shape
-    batch = rows // beams
+    batch = rows // beams if beams > 0 else 0
+    logits = _shaped(logits, np.float16, (batch * beams, vocab), "logits of whole entries")
+    scores = _shaped(scores, np.float32, (rows,), "scores")
+    finished = None if finished is None else _shaped(finished, np.uint8, (rows,), "finished")
     need = _sz(0)
     check(load().tl_beam_select_workspace(batch, beams, vocab, k, C.byref(need)), "tl_beam_select_workspace")
     w = DeviceBuffer.from_numpy(np.zeros(max(need.value, 16), np.uint8))
-    dl, ds = DeviceBuffer.from_numpy(logits), DeviceBuffer.from_numpy(np.ascontiguousarray(scores, dtype=np.float32))
-    df = None if finished is None else DeviceBuffer.from_numpy(np.ascontiguousarray(finished, dtype=np.uint8))
+    dl, ds = DeviceBuffer.from_numpy(logits), DeviceBuffer.from_numpy(scores)
+    df = None if finished is None else DeviceBuffer.from_numpy(finished)
     out = [DeviceBuffer(max(4 * batch * k, 4)) for _ in range(3)]
     check(load().tl_beam_select_f16(dl.ptr, vocab, ds.ptr, df.ptr if df is not None else None, pad_token, batch, beams, vocab, k, out[0].ptr,
                                     out[1].ptr, out[2].ptr, w.ptr, w.nbytes, None), "tl_beam_select_f16")
@@ -638,8 +658,9 @@ def beam_select(logits: np.ndarray, scores, beams: int, k: int, finished=None, p
 def beam_reorder(src: np.ndarray, dst: np.ndarray, parents, used: int) -> np.ndarray:
     """dst [outer, rows, pitch] with the first `used` values of each row from row parents[r] of src; returned."""
     outer, rows, pitch = src.shape
-    ds, dd = DeviceBuffer.from_numpy(src), DeviceBuffer.from_numpy(dst)
-    dp = DeviceBuffer.from_numpy(np.ascontiguousarray(parents, dtype=np.int32))
+    src, dst = _shaped(src, np.float16, src.shape, "src"), _shaped(dst, np.float16, (outer, rows, dst.shape[-1]), "dst")
+    parents = _shaped(parents, np.int32, (rows,), "parents")
+    ds, dd, dp = (DeviceBuffer.from_numpy(a) for a in (src, dst, parents))
     check(load().tl_beam_reorder_f16(ds.ptr, dd.ptr, dp.ptr, outer, rows, used, rows * pitch, pitch, rows * dst.shape[2], dst.shape[2], None),
           "tl_beam_reorder_f16")
     return dd.to_numpy(np.float16, dst.shape)

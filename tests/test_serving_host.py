@@ -111,6 +111,29 @@ def test_rotary_refuses():
         refused(lib.tl_rotary_append_f16(c, 0, P, P, P, P, None, P, P, 1.0, 1, 8, 128, 0, *strides, None))
 
 
+def test_helpers_refuse_arrays_of_other_sizes():
+    """Before anything is allocated: the kernels read as much as the sizes say."""
+    h = lambda *s: np.zeros(s, np.float16)  # noqa: E731
+    c = tl.PagedCache.__new__(tl.PagedCache)      # no device here: only what the checks look at
+    c.shape, c.by_head, c._attn_work, c._table, c._lengths, c._refs = (1, 4, 8, 2, 16), False, None, None, None, None
+    c.c = cache(n_layers=1, n_pages=4, page_size=8, n_kv_heads=2, head_dim=16, n_rows=3, max_pages=2)._obj
+    f = tl.rotary_frequencies(16)[0]
+    for call in (lambda: tl.rotary(h(3, 2, 16), [0, 1], f), lambda: tl.rotary(h(3, 2, 16).astype(np.float32), [0, 1, 2], f),
+                 lambda: tl.rotary(h(3, 2, 16), [0, 1, 2], f, out=h(3, 2, 8)),
+                 lambda: tl.PagedCache(1, 4, 8, 2, 16, 3, 2, k=h(1, 4, 8, 2, 8)),
+                 lambda: c.set_state(np.zeros((3, 3)), np.zeros(3), np.zeros(4)),
+                 lambda: c.fork([0, 1]), lambda: c.reserve([1, 1, 1, 1]), lambda: c.copy([0, 1], [2]),
+                 lambda: c.append(0, None, h(3, 2, 16), h(2, 2, 16), [0, 0, 0]), lambda: c.append(0, None, h(3, 1, 16), h(3, 1, 16), [0, 0, 0]),
+                 lambda: c.append(0, h(2, 4, 16), h(3, 2, 16), h(3, 2, 16), [0, 0, 0]),
+                 lambda: c.append(0, None, h(3, 2, 16), h(3, 2, 16), [0, 0]),
+                 lambda: c.append(0, None, h(3, 2, 16), h(3, 2, 16), [0, 0, 0], rows=[1, 2]),
+                 lambda: c.attend(0, h(3, 4, 8)), lambda: c.attend(0, h(3, 4, 16), rows=[0, 1]), lambda: tl.beam_select(h(5, 9), np.zeros(5), 2, 2), lambda: tl.beam_select(h(4, 9), np.zeros(3), 2, 2),
+                 lambda: tl.beam_select(h(4, 9), np.zeros(4), 0, 2), lambda: tl.beam_select(h(4, 9), np.zeros(4), 2, 2, finished=[0, 1]),
+                 lambda: tl.beam_reorder(h(1, 3, 8), h(1, 2, 8), [0, 0, 0], 8), lambda: tl.beam_reorder(h(1, 3, 8), h(1, 3, 8), [0, 0], 8)):
+        with pytest.raises(ValueError):
+            call()
+
+
 def test_attention_refuses():
     lib = tl.load()
     ws = 1 << 25
