@@ -104,7 +104,10 @@ __global__ void __launch_bounds__(ANY_WARPS * 32) k_paged_attn_any(AttnLaunch p)
 // For rows of head_dim values that start on 16 bytes. Per KV head the `group` query heads are the columns of the products
 //   S^T [16 tokens x 8 heads] = K_tile Q^T,   O^T [dims x 8 heads] += V_tile^T P^T        (mma.m16n8k16, fp32 sums)
 // so that eight heads cost what one does. P^T leaves the accumulators of the first product through a transposing register
-// move and enters the second as its B operand; it is split into two fp16 parts, which keeps the weights to 2^-22.
+// move and enters the second as its B operand, split into two fp16 parts. A weight is exp(s - running maximum) times 2^FL_LIFT, the
+// largest power of two that fp16 holds, in the sums of weights and of values alike: the factor cancels, and the log-sum takes it
+// off. The parts then keep a weight to 2^-22 of itself or 2^-40 of the largest, whichever is more. (Without the factor that is 2^-25 of
+// the largest, and what thousands of tokens some 17 nats below one other add to the values was lost or off by a quarter.)
 //
 // HBM bound: K and V are read once, and a tile of 16 tokens costs some 250 warp instructions against the 360 cycles that an
 // SM's share of the memory needs for its 8 KB. Each warp streams its own tiles through a private ring of shared memory
@@ -125,6 +128,7 @@ constexpr int FL_THREADS = FL_WARPS * 32;
 constexpr int FL_TILE = 16;                       // tokens of a warp's tile
 constexpr int FL_UNIT = FL_TILE * FL_WARPS;
 constexpr int FL_START = 2;
+constexpr float FL_LIFT = 15.f;
 constexpr int FL_JOIN = 16;                       // pieces joined at a time
 constexpr int FL_MAX_SMS = 160;
 constexpr int FL_COUNTER_BYTES = 8192;
@@ -426,8 +430,8 @@ __global__ void __launch_bounds__(FL_THREADS, TiledShape<HDP, NT>::CTAS) k_paged
                         keep[n][j] = exp2f(m[n][j] - ref);
                         moved |= mn != m[n][j];
                         m[n][j] = mn;
-                        s[n][j] = exp2f(x0 - ref);
-                        s[n][j + 2] = exp2f(x1 - ref);
+                        s[n][j] = exp2f(x0 - ref + FL_LIFT);
+                        s[n][j + 2] = exp2f(x1 - ref + FL_LIFT);
                         l[n][j] = l[n][j] * keep[n][j] + (s[n][j] + s[n][j + 2]);
                     }
 #pragma unroll
@@ -501,7 +505,7 @@ __global__ void __launch_bounds__(FL_THREADS, TiledShape<HDP, NT>::CTAS) k_paged
             } else {
                 at[0] = __low2half(lo); at[1] = __high2half(lo); at[2] = __low2half(hi); at[3] = __high2half(hi);
             }
-            if (d == 0 && a.lse) a.lse[(long long)seg_b * a.n_heads + h0 + h] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.69314718055994531f;
+            if (d == 0 && a.lse) a.lse[(long long)seg_b * a.n_heads + h0 + h] = L == 0.f ? -INFINITY : (M + (log2f(L) - FL_LIFT)) * 0.69314718055994531f;
         };
         for (int i = tid; i < heads * (HDP / 4); i += FL_THREADS) {
             const int h = i / (HDP / 4), d = i % (HDP / 4) * 4;

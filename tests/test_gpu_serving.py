@@ -235,6 +235,28 @@ def test_attention_of_large_scores_and_values(tl):
         check_attention(tl, c, k[0], v[0], table, [777, 64], page, q)
 
 
+@pytest.mark.parametrize("n,at,gap,hd,group,page", [(4096, 0, 17.5, 128, 4, 16), (4096, 2000, 16.25, 64, 1, 16), (131072, 0, 17.5, 128, 8, 16),
+                                                    (131072, 65536, 16.25, 128, 1, 64), (20011, 0, 18.0, 256, 3, 32), (20011, 77, 17.0, 96, 12, 16),
+                                                    (3000, 0, 17.5, 65, 2, 16)])
+def test_attention_keeps_weights_far_below_the_largest(tl, n, at, gap, hd, group, page):
+    """One key `gap` nats above all others, whose value is 0 where theirs are 1: what comes out is the sum of the small weights.
+    The scores are exact sums; scaling by log2 e costs 2^-23 of up to 26 twice; a weight is held to 2^-40 of the largest; the sums of
+    products and of weights add at most n / 16 times with 2^-24 each; then one rounding."""
+    r = np.random.default_rng([n, hd])
+    c, k, v, table, refs = filled_cache(tl, r, 1, page, 1, hd, [n], garbage=False)
+    k[:], v[:] = 0, 1
+    k[0, table[0, at // page], at % page, 0, :64] = gap / 64
+    v[0, table[0, at // page], at % page] = 0
+    c = tl.PagedCache(1, k.shape[1], page, 1, hd, 1, table.shape[1], k=k, v=v)
+    c.set_state(table, [n], refs)
+    out, lse = c.attend(0, np.ones((1, group, hd), np.float16), 1.0)
+    rest = (n - 1) * np.exp(-gap)
+    want = np.full((1, group, hd), rest / (1 + rest))
+    close(out, want, want * (so.EPS16 + 2.0 ** -17 + 2.0 ** -40 * np.exp(gap) + n / 8 * 2.0 ** -24) + so.TINY16)
+    assert (np.abs(lse - (gap + np.log1p(rest))) <= 2.0 ** -17 + n / 16 * 2.0 ** -24).all()
+    assert tl.device_status() == 0
+
+
 def test_attention_takes_a_row_list_with_padding(tl):
     r = np.random.default_rng(13)
     lens = [40, 7, 0, 300]
