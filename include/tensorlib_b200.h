@@ -327,7 +327,7 @@ TL_API int tl_paged_fork(const tl_paged_cache* cache, const int* parents, tl_str
  * lengths[r] grows by new_tokens[r]. Where a row's next token falls into a partly filled page that other rows still name, the row
  * first gets a copy of it (the filled slots, K and V of every layer; the last of the rows that write keeps the page if no other
  * row names it). *result (device memory) = TL_OK; or TL_ERR_OUT_OF_MEMORY if the free pages or max_pages do not suffice, or
- * TL_ERR_INVALID_ARGUMENT if a length, a count or an entry that it has to follow cannot be: then no row has changed. Workspace as
+ * TL_ERR_INVALID_ARGUMENT if a length, a count or an entry that it has to follow cannot be: then no row and no count has changed. Workspace as
  * tl_paged_workspace says. */
 TL_API int tl_paged_reserve_f16(const tl_paged_cache* cache, const int* new_tokens, int* result, void* workspace,
                                 size_t workspace_bytes, tl_stream stream);

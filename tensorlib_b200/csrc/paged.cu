@@ -255,6 +255,19 @@ __global__ void __launch_bounds__(RES_THREADS, 1) k_reserve(PagedView c, const i
         wk.need[r] = x.flag;
     }
     __syncthreads();
+    if (bad_sh) {                                 // refused: before a count is used as a claim, so that taking back restores each
+        auto take_back = [&](const Row& x) {
+            if (x.flag & WRITES) atomicAdd(c.refs + x.last, 1);
+        };
+        if (r0 < r1) take_back(mine);
+        for (int r = r0 + 1; r < r1; r++) take_back(again(r));
+        if (tid == 0) {
+            *result = bad_sh == 2 ? TL_ERR_INVALID_ARGUMENT : TL_ERR_OUT_OF_MEMORY;
+            *wk.n_copies = 0;
+            if (bad_sh == 2) atomicExch(status, TL_ERR_INVALID_ARGUMENT);
+        }
+        return;
+    }
     // 2: a page that nobody holds any more goes to the highest of the rows that let go of it: its count becomes -(row + 1)
     auto claim = [&](int r, const Row& x) {
         if ((x.flag & WRITES) && __ldcg(c.refs + x.last) <= 0) atomicMin(c.refs + x.last, -(r + 1));
@@ -268,8 +281,7 @@ __global__ void __launch_bounds__(RES_THREADS, 1) k_reserve(PagedView c, const i
             x.flag |= COPY;
             wants += (1ull << COPIES) + 1;
         }
-        if (x.add > 0 && x.len >= 0 && (long long)x.len + x.add <= (long long)c.max_pages * c.page_size)
-            wants += (unsigned)((int)c.by_page.div((unsigned)(x.len + x.add - 1)) + 1 - x.pages);
+        if (x.add > 0) wants += (unsigned)((int)c.by_page.div((unsigned)(x.len + x.add - 1)) + 1 - x.pages);
     };
     if (r0 < r1) count(r0, mine);
     for (int r = r0 + 1; r < r1; r++) {
@@ -288,9 +300,8 @@ __global__ void __launch_bounds__(RES_THREADS, 1) k_reserve(PagedView c, const i
     for (int r = r0 + 1; r < r1; r++) keep(again(r));
     __syncthreads();
     // 4: the lowest free pages, ascending
-    const int bad = bad_sh;
     int found = 0;
-    for (int p0 = 0; p0 < c.n_pages && found < pages_wanted && bad == 0; p0 += 4 * RES_THREADS) {
+    for (int p0 = 0; p0 < c.n_pages && found < pages_wanted; p0 += 4 * RES_THREADS) {
         unsigned mask = free4;
         if (p0 > 0) {
             mask = 0;
@@ -310,16 +321,15 @@ __global__ void __launch_bounds__(RES_THREADS, 1) k_reserve(PagedView c, const i
             }
         found += (int)here;
     }
-    if (bad || found < pages_wanted) {            // refused: the counts as they were, nothing else has changed
+    if (found < pages_wanted) {                   // refused: the counts are as they were, nothing else has changed
         if (r0 < r1 && (mine.flag & COPY)) atomicAdd(c.refs + mine.last, 1);
         for (int r = r0 + 1; r < r1; r++) {
             const Row x = again(r);
             if (x.flag & COPY) atomicAdd(c.refs + x.last, 1);
         }
         if (tid == 0) {
-            *result = bad == 2 ? TL_ERR_INVALID_ARGUMENT : TL_ERR_OUT_OF_MEMORY;
+            *result = TL_ERR_OUT_OF_MEMORY;
             *wk.n_copies = 0;
-            if (bad == 2) atomicExch(status, TL_ERR_INVALID_ARGUMENT);
         }
         return;
     }

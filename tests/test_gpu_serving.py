@@ -437,6 +437,22 @@ def test_pages_refuse_without_changing_anything(tl):
     assert tl.device_status() == 1
 
 
+def test_pages_refused_for_their_counts_keep_them(tl):
+    """A count below the number of rows that let go of the page: refused, and every count as it was."""
+    for rows, page, lens, counts, new in ((3, 4, [2, 0, 0], [0], [1, 0, 0]), (3, 4, [2, 2, 0], [1], [1, 1, 0]), (4, 4, [2, 2, 2, 0], [-3], [1, 1, 1, 2]),
+                                          (1500, 8, [3] * 1500, [1498], [1] * 1500), (1500, 8, [3] * 1500, [0], [1] * 1499 + [0])):
+        c = tl.PagedCache(1, 6, page, 1, 8, rows, 3)
+        table, refs = np.full((rows, 3), -1, np.int32), np.zeros(6, np.int32)
+        table[np.array(lens) > 0, 0] = 2
+        refs[2] = counts[0]
+        table[rows - 1, 0], refs[4] = 4, 1                # a sound page beside it
+        lens = lens[:-1] + [1]
+        c.set_state(table, lens, refs)
+        assert c.reserve(new) == 1 and tl.device_status() == 1
+        for got, want in zip(c.state(), (table, lens, refs)):
+            assert np.array_equal(got, want), (rows, got, want)
+
+
 def test_pages_wanted_beyond_32_bits_are_refused(tl):
     """4096 rows that ask for 2^20 pages each, of a table of 16 GB: 2^32 in all, which 32 bits hold as 0."""
     rows, width = 4096, 1 << 20
