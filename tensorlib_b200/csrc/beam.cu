@@ -161,6 +161,50 @@ __device__ __forceinline__ bool dead_row(const BeamArgs& a, int row) {
     return !(s > -INFINITY);
 }
 
+// The k best of one row by (value, lowest token), into its lists' places in the join: k passes over the row by the whole CTA. For rows
+// whose score is so large that distinct logits may have the same value in 64 bits, so that the k largest logits need not be the k
+// first candidates. Logits differ by 2^-24 at least, and values below 2^28 are rounded by 2^-26 at most: up to SEL_ROOM distinct
+// logits have distinct values.
+constexpr double SEL_ROOM = 134217728.0;          // 2^27
+__device__ __noinline__ void rank_row_by_value(const __half* x, unsigned vocab, unsigned at0, int n, double score, double lse,
+                                               unsigned long long* val, unsigned* idx, int places) {
+    __shared__ unsigned long long red_o[SEL_THREADS / 32];
+    __shared__ unsigned red_j[SEL_THREADS / 32];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    unsigned long long last = ~0ull;
+    unsigned last_j = 0;
+    for (int i = 0; i < n; i++) {
+        unsigned long long best = 0;
+        unsigned best_j = ~0u;
+        for (unsigned j = tid; j < vocab; j += SEL_THREADS) {
+            const unsigned long long o = ord64(score + ((double)beam_logit(x[j]) - lse));
+            if ((o < last || (o == last && j > last_j)) && o > best) { best = o; best_j = j; }       // (j ascends, no o is 0)
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            const unsigned long long y = __shfl_xor_sync(0xffffffffu, best, o);
+            const unsigned j = __shfl_xor_sync(0xffffffffu, best_j, o);
+            if (y > best || (y == best && j < best_j)) { best = y; best_j = j; }
+        }
+        __syncthreads();
+        if (lane == 0) { red_o[warp] = best; red_j[warp] = best_j; }
+        __syncthreads();
+        for (int v = 0; v < SEL_THREADS / 32; v++)
+            if (red_o[v] > best || (red_o[v] == best && red_j[v] < best_j)) { best = red_o[v]; best_j = red_j[v]; }
+        last = best;
+        last_j = best_j;
+        if (tid == 0) {
+            val[i] = best;
+            idx[i] = at0 + best_j;
+        }
+    }
+    for (int i = n + tid; i < places; i += SEL_THREADS) {
+        val[i] = 0;
+        idx[i] = ~0u;
+    }
+    __syncthreads();
+}
+
 // keys: (ord16 of the logit) << 16 | 0xffff - index in the chunk: unique, larger = earlier in the order
 template <int W>
 __global__ void __launch_bounds__(SEL_THREADS, 4) k_beam_select(SelLaunch p) {
@@ -170,7 +214,7 @@ __global__ void __launch_bounds__(SEL_THREADS, 4) k_beam_select(SelLaunch p) {
     __shared__ int red_i[SEL_THREADS / 32];
     __shared__ float red_f[SEL_THREADS / 32];
     __shared__ double red_d[SEL_THREADS / 32];
-    __shared__ int count_sh, listed_sh, last_sh;
+    __shared__ int count_sh, listed_sh, last_sh, large_sh;
     const BeamArgs& a = p.a;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int row = blockIdx.x / p.splits, split = blockIdx.x - row * p.splits, entry = row / a.beams;
@@ -434,7 +478,7 @@ __global__ void __launch_bounds__(SEL_THREADS, 4) k_beam_select(SelLaunch p) {
         asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(seen) : "l"(p.counters + entry) : "memory");
         last_sh = seen == (unsigned)(a.beams * p.splits - 1);
         if (last_sh) p.counters[entry] = 0;
-        count_sh = 0;
+        count_sh = large_sh = 0;
     }
     __syncthreads();
     if (!last_sh) return;
@@ -482,6 +526,7 @@ __global__ void __launch_bounds__(SEL_THREADS, 4) k_beam_select(SelLaunch p) {
                 const unsigned key = __ldcg(p.keys + ((long long)r * p.splits + s) * a.k + j);
                 o = ord64(score + ((double)ord16_value(key >> 16) - lse[w]));
                 at = (unsigned)w * (unsigned)a.vocab + (unsigned)first + (0xffffu - (key & 0xffffu));
+                if (fabs(score) >= SEL_ROOM) large_sh = 1;
             }
         }
         val[i] = o;
@@ -511,6 +556,17 @@ __global__ void __launch_bounds__(SEL_THREADS, 4) k_beam_select(SelLaunch p) {
     __syncthreads();
     bv = border_val;
     bi = border_idx;
+    if (large_sh)
+        for (int w = 0; w < a.beams; w++) {       // (the lists' candidates bound the result from below, whatever their order)
+            const int r = entry * a.beams + w, l0 = w * p.splits;
+            const double score = beam_score(a.scores[r]);
+            if (fabs(score) < SEL_ROOM || dead_row(a, r) || (a.finished && a.finished[r])) continue;
+            unsigned long long most = 0;          // a list begins with its largest value
+            for (int s = 0; s < p.splits; s++) most = max(most, val[(l0 + s) * a.k]);
+            if (most >= bv)
+                rank_row_by_value(a.logits + r * a.pitch, (unsigned)a.vocab, (unsigned)w * (unsigned)a.vocab, min(a.k, a.vocab), score, lse[w],
+                                  val + l0 * a.k, idx + l0 * a.k, p.splits * a.k);
+        }
     for (int i = tid; i < total; i += SEL_THREADS) {
         const unsigned long long o = val[i];
         const unsigned at = idx[i];

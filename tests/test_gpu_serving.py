@@ -554,6 +554,30 @@ def test_beam_selection_first_step_and_nothing_left(tl):
     assert np.array_equal(tl.beam_select(z, [0.0], 1, 9)[2][0], np.arange(9))              # -0 equals +0
 
 
+@pytest.mark.parametrize("batch,beams,vocab,k", [(2, 4, 5000, 8), (3, 2, 20000, 100), (1, 8, 70001, 16), (300, 3, 900, 5), (2, 128, 300, 128)])
+def test_beam_selection_where_scores_leave_no_room_for_logits(tl, batch, beams, vocab, k):
+    """Scores so large that many candidates are equal in 64 bits: the lowest beams, then the lowest tokens, whatever their logits."""
+    r = np.random.default_rng([34, beams, vocab])
+    rows = batch * beams
+    x = r.choice([0.0, -0.5, 3.0, 5.0], (rows, vocab)).astype(np.float16)
+    x[r.random((rows, vocab)) < 0.2] = -np.inf
+    for n, big in enumerate((-1e30, 3e38, 2.0 ** 90)):
+        s = np.full(rows, big, np.float32)
+        if n == 0:
+            s[::beams * 2] = -4.0                            # some entries have a beam with room
+        want = so.beam_select(x, s, beams, k)
+        got = tl.beam_select(x, s, beams, k)
+        assert np.array_equal(got[1], want[1]) and np.array_equal(got[2], want[2]), big
+        close(got[0], want[0], np.abs(want[0]) * 2.0 ** -24 + 2.0 ** -21)
+    # below 2^60 the steps are 128: the few logits within half a step of 0 are equal, and so are the many at -400
+    x = np.full((rows, vocab), -400, np.float16)
+    for row in x:
+        row[r.permutation(vocab)[:min(vocab, k // 2 + 1)]] = r.choice([0.0, 2.0, 9.0], min(vocab, k // 2 + 1))
+    s = np.full(rows, 2.0 ** 60, np.float32)
+    want, got = so.beam_select(x, s, beams, k), tl.beam_select(x, s, beams, k)
+    assert np.array_equal(got[1], want[1]) and np.array_equal(got[2], want[2]) and np.array_equal(got[0], want[0].astype(np.float32))
+
+
 @pytest.mark.parametrize("batch,beams,vocab", [(5, 4, 3001), (3, 128, 200)])
 def test_beam_selection_writes_the_scores_in_place(tl, batch, beams, vocab):
     """Both kernels: the second shape has more candidates than one CTA joins."""
