@@ -368,7 +368,8 @@ TL_API int tl_paged_attn_workspace(int n_heads, int n_kv_heads, int head_dim, si
  * finished (may be NULL): a beam with finished[row] != 0 has one candidate, pad_token, at its score; its logits are not used. A score
  * of -inf makes a dead beam; NaN logits count as -inf and +inf as 65504, NaN scores as -inf. beams, k <= 128. out_scores may be
  * scores where k == beams. workspace:
- * tl_beam_select_workspace bytes, zeroed once before its first use; it serves calls of any sizes that ask for no more. */
+ * tl_beam_select_workspace bytes, zeroed once before its first use; it serves calls of any sizes that ask for no more, all smaller
+ * batches of the same beams, vocab and k among them. */
 TL_API int tl_beam_select_f16(const tl_half* logits, long long row_stride, const float* scores, const unsigned char* finished,
                               int pad_token, int batch, int beams, int vocab, int k, float* out_scores, int* out_parents,
                               int* out_tokens, void* workspace, size_t workspace_bytes, tl_stream stream);

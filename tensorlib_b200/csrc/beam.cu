@@ -593,15 +593,21 @@ __global__ void __launch_bounds__(SEL_THREADS, 4) k_beam_select(SelLaunch p) {
 }
 
 // Chunks of a row: four CTAs an SM where the rows alone are fewer, but no chunk below one vector a thread, and no more
-// candidates than the join holds; 0 = the plain kernel.
-int sel_splits(int batch, int beams, int vocab, int k) {
+// candidates than the join holds: between `least` and `most`, whatever the batch; least = 0: the plain kernel. (148: the workspace
+// is asked for where there may be no device.)
+constexpr int SEL_CTAS = 4 * 148;
+struct SelSplits { int least, most; };
+SelSplits sel_split_limits(int beams, int vocab, int k) {
     const int least = (int)(((long long)vocab + SEL_MAX_CHUNK - 1) / SEL_MAX_CHUNK);
-    if (least > SEL_MAX_SPLITS || (long long)beams * least * k > SEL_MAX_MERGE) return 0;
-    const long long rows = (long long)batch * beams;
-    long long want = 4 * 148 / rows;
-    want = want < 16 ? want : 16;
-    while (want > least && (beams * want * k > 1024 || vocab / want < SEL_THREADS * 4)) want--;
-    return (int)(want > least ? want : least);
+    if (least > SEL_MAX_SPLITS || (long long)beams * least * k > SEL_MAX_MERGE) return {0, 0};
+    int most = 16;
+    while (most > least && (beams * most * k > 1024 || vocab / most < SEL_THREADS * 4)) most--;
+    return {least, most > least ? most : least};
+}
+int sel_splits(int batch, int beams, int vocab, int k) {
+    const SelSplits limits = sel_split_limits(beams, vocab, k);
+    const long long want = SEL_CTAS / ((long long)batch * beams);
+    return (int)(want < limits.least ? limits.least : (want < limits.most ? want : limits.most));
 }
 int sel_chunk(int vocab, int splits) { return ((vocab + splits - 1) / splits + 7) / 8 * 8; }
 
@@ -617,9 +623,12 @@ int launch_sel(const SelLaunch& p, cudaStream_t st) {
 }  // namespace
 
 size_t beam_workspace_bytes(int batch, int beams, int vocab, int k) {
-    const int splits = sel_splits(batch > 0 ? batch : 1, beams, vocab, k);
-    const size_t rows = (size_t)(batch < SEL_ENTRIES ? batch : SEL_ENTRIES) * beams;
-    return SEL_ENTRIES * 4 + rows * splits * (sizeof(SelStat) + 4 * (size_t)k);
+    // Never less than what a smaller batch asks for, whose rows may be cut into more chunks: rows times chunks are at most
+    // rows * most and SEL_CTAS, or rows * least where that is more.
+    const SelSplits limits = sel_split_limits(beams, vocab, k);
+    const size_t rows = (size_t)(batch < SEL_ENTRIES ? batch : SEL_ENTRIES) * beams, least = rows * limits.least, most = rows * limits.most;
+    const size_t cut = most < (size_t)SEL_CTAS ? most : (size_t)SEL_CTAS;
+    return SEL_ENTRIES * 4 + (cut > least ? cut : least) * (sizeof(SelStat) + 4 * (size_t)k);
 }
 
 int launch_beam_select(const BeamArgs& a, cudaStream_t st) {

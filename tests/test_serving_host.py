@@ -174,6 +174,18 @@ def test_beam_calls_refuse():
         refused(lib.tl_beam_reorder_f16(*a, None))
 
 
+def test_a_workspace_for_a_batch_serves_the_smaller_ones():
+    lib, need = tl.load(), C.c_size_t(0)
+    for beams, vocab, k in ((4, 32000, 8), (1, 32000, 1), (8, 128256, 16), (1, 131072, 64), (5, 1001, 10), (16, 50000, 16), (64, 65537, 128), (3, 1 << 22, 4),
+                            (128, 32000, 64), (1, 2000000, 128)):
+        most = 0
+        for batch in [*range(1, 700), 4095, 4096, 4097, 5000]:
+            assert lib.tl_beam_select_workspace(batch, beams, vocab, k, C.byref(need)) == 0
+            assert need.value >= most, (beams, vocab, k, batch)
+            most = need.value
+            assert lib.tl_beam_select_f16(P, vocab, P, None, 0, batch, beams, vocab, k, P, P, P, P, need.value - 1, None) == 1
+
+
 @pytest.mark.skipif(tl.device_count() != 0, reason="host-only behaviour: a GPU is present")
 def test_sound_calls_without_a_device_report_that():
     lib = tl.load()
