@@ -140,7 +140,7 @@ __global__ void __launch_bounds__(ROT_THREADS, rot_ctas(HALF)) k_rotary(RotLaunc
         unsigned tt, h0;
         p.plane[w].by_heads_at_once.divmod(r, tt, h0);
         const int left = (int)tt < tokens_at_once ? heads - (int)h0 : 0;       // rows of a token: 0, at_once, .. below this
-        const __half* in_token = p.plane[w].in + (long long)(t0 + (int)tt) * p.plane[w].in_token + h0 * p.plane[w].in_head + d;
+        const __half* in_token = p.plane[w].in + (long long)(t0 + tt) * p.plane[w].in_token + h0 * p.plane[w].in_head + d;
         __half* const out0 = p.plane[w].out + h0 * p.plane[w].out_head + d;
         // a thread's rows under way: heads of one token, or, where all its heads are moved at once, tokens
         auto move = [&](auto by_token_c) {
@@ -207,20 +207,21 @@ __global__ void __launch_bounds__(ROT_THREADS) k_rotary_any(RotLaunch p) {
     pdl_wait();
     const RotaryArgs& a = p.a;
     const int pairs = a.rot / 2;
-    for (int t = blockIdx.x; t < a.tokens; t += gridDim.x) {
+    // (unsigned counters: a step beyond the last token or item may pass 2^31)
+    for (unsigned t = blockIdx.x; t < (unsigned)a.tokens; t += gridDim.x) {
         const int pos = a.positions[t];
         __syncthreads();
         if (pos < 0) continue;                    // padding: nothing is written
         for (int i = threadIdx.x; i < pairs; i += ROT_THREADS) cs[i] = turn_of(a, pos, i);
-        if (threadIdx.x == 0 && p.paged) slot_sh = slot_of(p, t, pos);
+        if (threadIdx.x == 0 && p.paged) slot_sh = slot_of(p, (int)t, pos);
         __syncthreads();
         const long long slot = p.paged ? slot_sh : -1;
         for (int w = 0; w < p.planes; w++) {
             const RotPlane& q = p.plane[w];
             if (q.paged && slot < 0) continue;
-            for (int k = threadIdx.x; k < q.heads * p.items; k += ROT_THREADS) {
+            for (unsigned k = threadIdx.x; k < (unsigned)(q.heads * p.items); k += ROT_THREADS) {
                 unsigned h, i;
-                p.by_items.divmod((unsigned)k, h, i);
+                p.by_items.divmod(k, h, i);
                 const __half* in = q.in + t * q.in_token + h * q.in_head;
                 __half* out = q.out + (q.paged ? slot : t * q.out_token) + h * q.out_head;
                 if ((int)i < pairs) {
@@ -293,7 +294,7 @@ int launch_rotary(const RotaryArgs& a, const PagedView* cache, cudaStream_t st) 
     if (vec == 1) {
         p.items = pairs + (a.head_dim - a.rot);
         p.by_items = FastDiv((unsigned)p.items);
-        return launch_pdl(k_rotary_any, a.tokens < 148 * 64 ? a.tokens : 148 * 64, ROT_THREADS, (size_t)pairs * 8, st, true, p);
+        return launch_pdl(k_rotary_any, a.tokens < sm_count() * 64 ? a.tokens : sm_count() * 64, ROT_THREADS, (size_t)pairs * 8, st, true, p);
     }
     p.by_items = FastDiv((unsigned)p.items);
     p.by_pairs = FastDiv((unsigned)(pairs > 0 ? pairs : 1));
@@ -316,7 +317,7 @@ int launch_rotary(const RotaryArgs& a, const PagedView* cache, cudaStream_t st) 
     const long long rounds = (a.tokens + most * resident - 1) / (most * resident);
     p.group = (int)((a.tokens + rounds * resident - 1) / (rounds * resident));
     p.turn_stride = (pairs + 3) / 4 * 4;
-    const dim3 grid((unsigned)((a.tokens + p.group - 1) / p.group), p.group == 1 ? p.planes : 1);
+    const dim3 grid((unsigned)(((long long)a.tokens + p.group - 1) / p.group), p.group == 1 ? p.planes : 1);
     const size_t smem = (size_t)p.group * p.turn_stride * 8;
     return vec == 8 ? launch_vec<8>(p, grid, smem, st) : (vec == 4 ? launch_vec<4>(p, grid, smem, st) : launch_vec<2>(p, grid, smem, st));
 }

@@ -91,6 +91,32 @@ def test_rotary_of_a_strided_slice(tl):
         assert (got[..., hd:] == 7).all()
 
 
+@pytest.mark.parametrize("hd,rot", [(8, 8), (7, 6)])
+def test_rotary_of_the_most_tokens(tl, hd, rot):
+    """2^31 - 1 tokens, all padding but the last; they share one row of in and out."""
+    lib, T = tl.load(), 2 ** 31 - 1
+    x, f, last = normal(np.random.default_rng(8), 1, 1, hd), tl.rotary_frequencies(rot)[0], np.array([5], np.int32)
+    dx, do, df, dp = tl.DeviceBuffer.from_numpy(x), tl.DeviceBuffer.from_numpy(np.zeros(hd, np.float16)), tl.DeviceBuffer.from_numpy(f), tl.DeviceBuffer(4 * T)
+    tl.check(lib.tl_memset(dp.ptr, 0xff, dp.nbytes, None), "memset")
+    tl.check(lib.tl_memcpy_h2d(dp.ptr + 4 * (T - 1), last.ctypes.data, 4, None), "h2d")
+    tl.synchronize()
+    tl.check(lib.tl_rotary_f16(dx.ptr, do.ptr, dp.ptr, df.ptr, 1.0, T, 1, hd, rot, 0, 0, 0, hd, 0, hd, None), "rotary")
+    want, tol = so.rotary(x, last, f)
+    close(do.to_numpy(np.float16, x.shape), want, tol)
+    assert tl.device_status() == 0
+
+
+def test_rotary_of_the_widest_token(tl):
+    """49981 heads of 42966 elements, two below 2^31 in all; they share one row of in and out."""
+    heads, hd = 49981, 42966
+    assert heads * hd == 2 ** 31 - 2
+    x = normal(np.random.default_rng(9), 1, 1, hd)
+    dx, do, dp = tl.DeviceBuffer.from_numpy(x), tl.DeviceBuffer.from_numpy(np.zeros(hd + 64, np.float16)), tl.DeviceBuffer.from_numpy(np.zeros(1, np.int32))
+    tl.check(tl.load().tl_rotary_f16(dx.ptr, do.ptr, dp.ptr, None, 1.0, 1, heads, hd, 0, 0, 0, heads * hd, 0, heads * hd, 0, None), "rotary")
+    got = do.to_numpy(np.float16, (hd + 64,))
+    assert np.array_equal(got[:hd], x[0, 0]) and (got[hd:] == 0).all() and tl.device_status() == 0
+
+
 # ---- the way into the cache ------------------------------------------------------------------------------------------
 def filled_cache(tl, r, layers, page, kv, hd, lens, by_head=False, spare=3, max_pages=None, garbage=True):
     """A cache whose row i holds lens[i] tokens in random pages, with anything at all in the slots never written."""
