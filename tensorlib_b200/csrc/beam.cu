@@ -30,7 +30,7 @@ __global__ void __launch_bounds__(BEAM_THREADS) k_beam_any(BeamArgs a) {
     for (int w = 0; w < a.beams; w++) {
         const __half* x = a.logits + (long long)(b * a.beams + w) * a.pitch;
         float m = -INFINITY;
-        for (int j = tid; j < a.vocab; j += BEAM_THREADS) m = fmaxf(m, beam_logit(x[j]));
+        for (unsigned j = tid; j < (unsigned)a.vocab; j += BEAM_THREADS) m = fmaxf(m, beam_logit(x[j]));    // (a step may pass 2^31)
         m = warp_max(m);
         __syncthreads();
         if (lane == 0) red[warp] = m;
@@ -40,7 +40,7 @@ __global__ void __launch_bounds__(BEAM_THREADS) k_beam_any(BeamArgs a) {
         __syncthreads();
         double s = 0.0;
         if (M > -INFINITY)
-            for (int j = tid; j < a.vocab; j += BEAM_THREADS) s += (double)expf(beam_logit(x[j]) - (float)M);
+            for (unsigned j = tid; j < (unsigned)a.vocab; j += BEAM_THREADS) s += (double)expf(beam_logit(x[j]) - (float)M);
         for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
         if (lane == 0) red[warp] = s;
         __syncthreads();

@@ -667,6 +667,24 @@ def test_beam_selection_of_other_sizes_in_the_same_workspace(tl):
         close(out[0].to_numpy(np.float32, (batch, k)), got, np.abs(got) * 2.0 ** -24 + 2.0 ** -21, n)
 
 
+def test_beam_selection_of_the_largest_vocabulary(tl):
+    """2^31 - 1 equal logits but for two: the last, and one in the middle."""
+    lib, vocab, need = tl.load(), 2 ** 31 - 1, C.c_size_t(0)
+    tl.check(lib.tl_beam_select_workspace(1, 1, vocab, 1, C.byref(need)), "ws")
+    dx, ds = tl.DeviceBuffer(2 * vocab), tl.DeviceBuffer.from_numpy(np.array([-1.5], np.float32))
+    w, out = tl.DeviceBuffer.from_numpy(np.zeros(max(16, need.value), np.uint8)), [tl.DeviceBuffer(4) for _ in range(3)]
+    tl.check(lib.tl_memset(dx.ptr, 0, dx.nbytes, None), "memset")
+    for at, value in ((vocab - 1, 4.0), (1 << 30, 3.0)):
+        one = np.array([value], np.float16)
+        tl.check(lib.tl_memcpy_h2d(dx.ptr + 2 * at, one.ctypes.data, 2, None), "h2d")
+        tl.synchronize()
+    tl.check(lib.tl_beam_select_f16(dx.ptr, vocab, ds.ptr, None, 0, 1, 1, vocab, 1, *(o.ptr for o in out), w.ptr, w.nbytes, None), "select")
+    want = -1.5 + np.array([4.0]) - np.log(vocab - 2 + np.exp(4.0) + np.exp(3.0))
+    close(out[0].to_numpy(np.float32, (1,)), want, np.abs(want) * 2.0 ** -24 + 2.0 ** -21)
+    assert out[2].to_numpy(np.int32, (1,)).tolist() == [vocab - 1] and out[1].to_numpy(np.int32, (1,)) == 0
+    assert tl.device_status() == 0
+
+
 @pytest.mark.parametrize("outer,rows,pitch,used", [(1, 1, 8, 8), (2, 5, 24, 17), (3, 4, 70000, 69993), (2, 7, 33, 33), (4, 64, 4096, 1000)])
 def test_beam_reorder(tl, outer, rows, pitch, used):
     r = np.random.default_rng([outer, rows, pitch])
