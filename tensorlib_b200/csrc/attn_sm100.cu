@@ -316,11 +316,11 @@ int launch_flash_prefill(const __half* q, const __half* k, const __half* v, __ha
     TL_REQUIRE(flash_prefill_supported(q, k, v, out, T, S, pos0, heads, head_dim, ldq, ldk, ldv, ldo),
                "flash prefill: unsupported shape or alignment (head_dim must be %d)", HD);
     static PerDeviceOnce once;
-    if (once.needed()) {
-        TL_CUDA(cudaFuncSetAttribute(k_flash_prefill, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)FA_SMEM));
-        TL_CUDA(cudaFuncSetAttribute(k_flash_prefill, cudaFuncAttributePreferredSharedMemoryCarveout,
-                                     (int)cudaSharedmemCarveoutMaxShared));
-    }
+    TL_CUDA(once.run([] {
+        const cudaError_t e = cudaFuncSetAttribute(k_flash_prefill, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)FA_SMEM);
+        return e != cudaSuccess ? e : cudaFuncSetAttribute(k_flash_prefill, cudaFuncAttributePreferredSharedMemoryCarveout,
+                                                           (int)cudaSharedmemCarveoutMaxShared);
+    }));
     CUtensorMap mq, mk, mv;
     TL_PROPAGATE(make_tensor_map_f16(&mq, q, T, HD, ldq, HD, heads, BQ));
     TL_PROPAGATE(make_tensor_map_f16(&mk, k, S, HD, ldk, HD, heads, BKV));

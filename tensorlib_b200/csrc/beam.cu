@@ -616,7 +616,7 @@ int launch_sel(const SelLaunch& p, cudaStream_t st) {
     const size_t total = (size_t)p.a.beams * p.splits * p.a.k, join = total * 24 + (size_t)p.a.beams * 8;
     const size_t list = (size_t)(SEL_THREADS * W + SEL_ASIDE) * 20 + (SEL_LONG + 8 * SEL_ASIDE) * 4, smem = list > join ? list : join;
     static PerDeviceOnce once;
-    if (once.needed()) TL_CUDA(cudaFuncSetAttribute(k_beam_select<W>, cudaFuncAttributeMaxDynamicSharedMemorySize, SEL_MAX_MERGE * 24 + 128 * 8));
+    TL_CUDA(once.run([&] { return cudaFuncSetAttribute(k_beam_select<W>, cudaFuncAttributeMaxDynamicSharedMemorySize, SEL_MAX_MERGE * 24 + 128 * 8); }));
     return launch_pdl(k_beam_select<W>, p.a.batch * p.a.beams * p.splits, SEL_THREADS, smem, st, true, p);
 }
 

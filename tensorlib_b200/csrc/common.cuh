@@ -5,6 +5,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdarg>
 #include <cstddef>
 #include <cstdint>
@@ -20,15 +21,24 @@ bool initialized();
 int sm_count();
 
 // Kernel attributes (opt-in shared-memory size) belong to a device: a process that moves between
-// devices with tl_init must set them once on each. One of these per kernel instantiation.
+// devices with tl_init must set them once on each. One of these per kernel instantiation. A device
+// counts as done only after its attributes are set: a second thread on its first call sets them too
+// instead of launching without them, and a failure is tried again.
 struct PerDeviceOnce {
-    unsigned long long done = 0;   // bit d: configured on device d (d < 64)
-    bool needed() {
-        int dev = 0;
-        if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return true;
-        if (done & (1ull << dev)) return false;
-        done |= 1ull << dev;
-        return true;
+    std::atomic<unsigned long long> done{0};   // bit d: configured on device d (d < 64)
+    template <typename Set>
+    cudaError_t run_on(int dev, Set&& set) {
+        const unsigned long long bit = dev >= 0 && dev < 64 ? 1ull << dev : 0;
+        if (done.load(std::memory_order_acquire) & bit) return cudaSuccess;
+        const cudaError_t e = set();
+        if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+        return e;
+    }
+    template <typename Set>
+    cudaError_t run(Set&& set) {
+        int dev = -1;
+        const cudaError_t e = cudaGetDevice(&dev);
+        return e != cudaSuccess ? e : run_on(dev, set);
     }
 };
 

@@ -866,9 +866,7 @@ int mega_smem_bytes(int max_k) {
 
 int launch_decode_flow(const FlowArgs& args, int grid, int smem, cudaStream_t st) {
     static PerDeviceOnce once;
-    if (once.needed()) {
-        TL_CUDA(cudaFuncSetAttribute(k_decode_flow, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
-    }
+    TL_CUDA(once.run([&] { return cudaFuncSetAttribute(k_decode_flow, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024); }));
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(grid);
     cfg.blockDim = dim3(MEGA_THREADS);

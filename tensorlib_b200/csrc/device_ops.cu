@@ -234,8 +234,7 @@ int table_for_unary(int op, const __half** out) {
 int launch_lookup(__half* out, const __half* in, size_t n, const __half* tab, cudaStream_t st) {
     if (n >= (1u << 20) && n % 8 == 0 && al16(out) && al16(in)) {
         static PerDeviceOnce once;
-        if (once.needed())
-            TL_CUDA(cudaFuncSetAttribute(k_lookup_smem, cudaFuncAttributeMaxDynamicSharedMemorySize, 65536 * 2));
+        TL_CUDA(once.run([&] { return cudaFuncSetAttribute(k_lookup_smem, cudaFuncAttributeMaxDynamicSharedMemorySize, 65536 * 2); }));
         k_lookup_smem<<<std::max(1, sm_count()), 1024, 65536 * 2, st>>>(reinterpret_cast<uint4*>(out), reinterpret_cast<const uint4*>(in),
                                                                         n / 8, reinterpret_cast<const uint4*>(tab));
     } else {

@@ -852,13 +852,12 @@ template <int EPI, bool NORM, int CW, int NST>
 int launch_ring_cfg(const RingArgs& a, cudaStream_t st, bool pdl) {
     using Cfg = RingCfg<CW, NST>;
     static PerDeviceOnce once;
-    if (once.needed()) {
-        TL_CUDA(cudaFuncSetAttribute(k_gemv_ring<EPI, NORM, CW, NST>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                     CW == 16 ? 227 * 1024 : 113 * 1024));
-        if (CW != 16)
-            TL_CUDA(cudaFuncSetAttribute(k_gemv_ring<EPI, NORM, CW, NST>, cudaFuncAttributePreferredSharedMemoryCarveout,
-                                         (int)cudaSharedmemCarveoutMaxShared));
-    }
+    TL_CUDA(once.run([] {
+        const cudaError_t e = cudaFuncSetAttribute(k_gemv_ring<EPI, NORM, CW, NST>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                   CW == 16 ? 227 * 1024 : 113 * 1024);
+        return e != cudaSuccess || CW == 16 ? e : cudaFuncSetAttribute(k_gemv_ring<EPI, NORM, CW, NST>, cudaFuncAttributePreferredSharedMemoryCarveout,
+                                                                       (int)cudaSharedmemCarveoutMaxShared);
+    }));
     // persistent CTAs, each with a contiguous share of the units balanced to +-1; a CTA's last stage may
     // be partly filled (it streams only its own rows), so every SM gets work as soon as there is half
     // a stage of units per CTA: N = 4096 spreads over all 148 SMs instead of 128 full stages
@@ -915,8 +914,7 @@ int launch_gemv(const __half* x, const __half* W, __half* y, int M, int N, int K
     }
     if (gemv_ring_rows_supported(x, W, M, N, K, ldw, ldx)) {   // up to eight rows at the weight traffic of one
         static PerDeviceOnce once;
-        if (once.needed())
-            TL_CUDA(cudaFuncSetAttribute(k_gemv_ring_rows<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)RowsCfg::smem_bytes()));
+        TL_CUDA(once.run([&] { return cudaFuncSetAttribute(k_gemv_ring_rows<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)RowsCfg::smem_bytes()); }));
         RingArgs a{};
         a.x = x; a.W0 = W; a.N_each = N; a.K = K; a.total_units = N / 2; a.y = y;
         a.status = device_status_word(); a.wait_weights = weights_constant ? 0 : 1;
@@ -986,8 +984,7 @@ template <int EPI_B>
 int launch_ring2(const RingArgs& a, const RingArgs& b, cudaStream_t st, bool pdl) {
     using Cfg = RingCfg<16, 3>;
     static PerDeviceOnce once;
-    if (once.needed())
-        TL_CUDA(cudaFuncSetAttribute(k_gemv_ring2<EPI_B>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
+    TL_CUDA(once.run([&] { return cudaFuncSetAttribute(k_gemv_ring2<EPI_B>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024); }));
     const int units = std::max(a.total_units, b.total_units);
     const int grid = std::max(1, std::min(sm_count(), (units + 7) / 8));
     return launch_pdl(k_gemv_ring2<EPI_B>, dim3(grid), dim3(Cfg::THREADS), Cfg::smem_bytes(std::max(a.K, b.K)), st, pdl, a, b);

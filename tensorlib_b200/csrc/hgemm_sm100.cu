@@ -1030,9 +1030,7 @@ int launch_k(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mb
              const GemmArgs& a, int tiles, cudaStream_t st) {
     constexpr size_t smem = (size_t)STAGES * (A_BYTES + BN * BK * 2) + 1024 + 256;
     static PerDeviceOnce once;
-    if (once.needed()) {
-        TL_CUDA(cudaFuncSetAttribute(k_hgemm<BN, EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    }
+    TL_CUDA(once.run([&] { return cudaFuncSetAttribute(k_hgemm<BN, EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem); }));
     const int grid = std::max(1, std::min(tiles, sm_count()));
     return launch_pdl(k_hgemm<BN, EPI>, dim3(grid), dim3(GEMM_THREADS), smem, st, true, ma, mb, mb2, mb3, a);
 }
@@ -1047,9 +1045,7 @@ int launch_any_bn(int bn, const CUtensorMap& ma, const CUtensorMap& mb, const CU
 template <int BN, int KS, int MSUB, int EPI>
 int launch_splitk_cfg(const CUtensorMap& ma, const CUtensorMap& mb, const GemmArgs& a, int tiles, cudaStream_t st) {
     static PerDeviceOnce once;
-    if (once.needed()) {
-        TL_CUDA(cudaFuncSetAttribute(k_hgemm_splitk<BN, KS, MSUB, EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SplitCfg<BN, KS, MSUB>::SMEM));
-    }
+    TL_CUDA(once.run([&] { return cudaFuncSetAttribute(k_hgemm_splitk<BN, KS, MSUB, EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SplitCfg<BN, KS, MSUB>::SMEM); }));
     return launch_pdl(k_hgemm_splitk<BN, KS, MSUB, EPI>, dim3(tiles * KS), dim3(GEMM_THREADS), SplitCfg<BN, KS, MSUB>::SMEM, st, true, ma, mb, a);
 }
 template <int EPI>
@@ -1067,9 +1063,7 @@ template <int EPI, int MSUB>
 int launch_pair_cfg(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mb2, const CUtensorMap& mb3,
                     const GemmArgs& a, int pair_tiles, cudaStream_t st) {
     static PerDeviceOnce once;
-    if (once.needed()) {
-        TL_CUDA(cudaFuncSetAttribute(k_hgemm_pair<EPI, MSUB>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PairCfg<MSUB>::SMEM));
-    }
+    TL_CUDA(once.run([&] { return cudaFuncSetAttribute(k_hgemm_pair<EPI, MSUB>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PairCfg<MSUB>::SMEM); }));
     const int grid = 2 * std::max(1, std::min(pair_tiles, sm_count() / 2));
     return launch_pdl(k_hgemm_pair<EPI, MSUB>, dim3(grid), dim3(PairCfg<MSUB>::THREADS), PairCfg<MSUB>::SMEM, st, true, ma, mb, mb2, mb3, a);
 }

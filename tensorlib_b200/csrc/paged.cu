@@ -528,7 +528,7 @@ unsigned page_grid(const CopyArgs& a, long long pages) { return copy_grid((pages
 template <int SLAB>
 static int launch_fork(const PagedView& c, const int* parents, cudaStream_t st) {
     static PerDeviceOnce once;
-    if (once.needed()) TL_CUDA(cudaFuncSetAttribute(k_fork<SLAB>, cudaFuncAttributeMaxDynamicSharedMemorySize, FORK_SMEM));
+    TL_CUDA(once.run([&] { return cudaFuncSetAttribute(k_fork<SLAB>, cudaFuncAttributeMaxDynamicSharedMemorySize, FORK_SMEM); }));
     return launch_pdl(k_fork<SLAB>, (unsigned)((c.max_pages + SLAB - 1) / SLAB + 1), FORK_THREADS, (size_t)c.n_rows * SLAB * 4, st, true, c.table,
                       c.lengths, c.refs, parents, c.n_rows, c.max_pages, c.n_pages, device_status_word());
 }

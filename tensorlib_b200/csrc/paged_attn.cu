@@ -605,7 +605,7 @@ template <int HDP, int NT>
 int launch_tiled(const TiledLaunch& p, cudaStream_t st) {
     using F = TiledShape<HDP, NT>;
     static PerDeviceOnce once;
-    if (once.needed()) TL_CUDA(cudaFuncSetAttribute(k_paged_attn<HDP, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::SMEM));
+    TL_CUDA(once.run([&] { return cudaFuncSetAttribute(k_paged_attn<HDP, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::SMEM); }));
     TiledLaunch q = p;
     const int grid = (sm_count() < FL_MAX_SMS ? sm_count() : FL_MAX_SMS) * F::CTAS;
     q.by_grid = FastDiv((unsigned)grid);

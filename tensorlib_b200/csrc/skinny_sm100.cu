@@ -435,18 +435,14 @@ int workspace_for(cudaStream_t st, Workspace* out) {
 template <int NB>
 int launch_nb(const CUtensorMap& mw, const CUtensorMap& mx, const SkinnyArgs& a, int grid, cudaStream_t st) {
     static PerDeviceOnce once;
-    if (once.needed()) {
-        TL_CUDA(cudaFuncSetAttribute(k_skinny<NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SkinnyCfg<NB>::SMEM));
-    }
+    TL_CUDA(once.run([&] { return cudaFuncSetAttribute(k_skinny<NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SkinnyCfg<NB>::SMEM); }));
     return launch_pdl(k_skinny<NB>, dim3(grid), dim3(SK_THREADS), SkinnyCfg<NB>::SMEM, st, true, mw, mx, a);
 }
 
 template <int NB>
 int launch_cluster(const CUtensorMap& mw, const CUtensorMap& mx, const SkinnyArgs& a, int grid, int cluster, cudaStream_t st) {
     static PerDeviceOnce once;
-    if (once.needed()) {
-        TL_CUDA(cudaFuncSetAttribute(k_skinny_cluster<NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SkinnyCfg<NB>::SMEM));
-    }
+    TL_CUDA(once.run([&] { return cudaFuncSetAttribute(k_skinny_cluster<NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SkinnyCfg<NB>::SMEM); }));
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)grid);
     cfg.blockDim = dim3(SK_THREADS);
