@@ -502,11 +502,16 @@ ROPE_SCALINGS = {"unscaled": 0, "linear": 1, "base": 2, "parts": 3, "ramp": 4}
 
 
 def _shaped(a, dtype, shape, what: str) -> np.ndarray:
-    """a as a contiguous array of that shape; a kernel trusts the sizes that it is told. fp16 operands are not converted."""
+    """a as a contiguous array of that shape; a kernel trusts the sizes that it is told. fp16 operands are not converted, and whole
+    numbers have to be that and to fit (2^32 + 5 is no position 5)."""
     a = np.asarray(a)
     if a.shape != tuple(shape) or (dtype == np.float16 and a.dtype != dtype):
         raise ValueError(f"{what}: {a.dtype}{list(a.shape)}, expected {np.dtype(dtype)}{list(shape)}")
-    return np.ascontiguousarray(a, dtype=dtype)
+    with np.errstate(invalid="ignore"):
+        b = np.ascontiguousarray(a, dtype=dtype)
+    if np.issubdtype(b.dtype, np.integer) and not np.array_equal(a, b):
+        raise ValueError(f"{what}: values that are no {np.dtype(dtype)}")
+    return b
 
 
 def rotary_frequencies(rot_dim: int, base: float = 10000.0, scaling: str = "unscaled", factor: float = 1.0,

@@ -134,6 +134,25 @@ def test_helpers_refuse_arrays_of_other_sizes():
             call()
 
 
+def test_helpers_refuse_numbers_that_do_not_fit():
+    """Whole numbers of 32 bits, 8 for the marks of finished beams: nothing is cut off or wrapped round."""
+    h = lambda *s: np.zeros(s, np.float16)  # noqa: E731
+    c = tl.PagedCache.__new__(tl.PagedCache)
+    c.shape, c.by_head, c._attn_work, c._table, c._lengths, c._refs = (1, 4, 8, 2, 16), False, None, None, None, None
+    c.c = cache(n_layers=1, n_pages=4, page_size=8, n_kv_heads=2, head_dim=16, n_rows=3, max_pages=2)._obj
+    f = tl.rotary_frequencies(16)[0]
+    for bad in (2 ** 32 + 5, 2 ** 31, -2 ** 31 - 1, 1.5, np.nan, np.inf):
+        for call in (lambda: tl.rotary(h(3, 2, 16), [0, bad, 1], f), lambda: c.fork([0, 1, bad]), lambda: c.reserve([1, bad, 0]),
+                     lambda: c.copy([0, bad], [1, 2]), lambda: c.copy([0, 1], [2, bad]), lambda: c.set_state(np.zeros((3, 2)), [0, 0, bad], np.zeros(4)),
+                     lambda: c.append(0, None, h(2, 2, 16), h(2, 2, 16), [0, bad]), lambda: c.append(0, None, h(2, 2, 16), h(2, 2, 16), [0, 1], rows=[bad, 0]),
+                     lambda: c.attend(0, h(1, 4, 16), rows=[bad]), lambda: tl.beam_reorder(h(1, 3, 8), h(1, 3, 8), [0, bad, 0], 8),
+                     lambda: tl.beam_select(h(2, 9), np.zeros(2), 2, 2, finished=[0, bad])):
+            with pytest.raises(ValueError):
+                call()
+    with pytest.raises(ValueError):
+        tl.beam_select(h(2, 9), np.zeros(2), 2, 2, finished=[0, 256])
+
+
 def test_attention_refuses():
     lib = tl.load()
     ws = 1 << 25
