@@ -91,6 +91,28 @@ def test_rotary_of_a_strided_slice(tl):
         assert (got[..., hd:] == 7).all()
 
 
+@pytest.mark.parametrize("T,heads,hd,rot,half", [(1500, 40, 128, 128, False), (4099, 3, 64, 64, False), (9000, 1, 128, 64, True), (1481, 32, 128, 128, True),
+                                                 (3000, 5, 80, 40, False), (2222, 12, 96, 48, True), (1200, 2, 36, 20, True), (20011, 2, 10, 6, False),
+                                                 (1300, 300, 8, 8, False), (800, 2, 1024, 1024, False), (1000, 4, 512, 512, True), (70000, 1, 16, 2, False)])
+def test_rotary_of_many_tokens(tl, T, heads, hd, rot, half):
+    """More tokens than CTAs are resident: a CTA turns several, padding among them."""
+    r = np.random.default_rng([T, heads, hd])
+    x, old = normal(r, T, heads, hd, std=2.0), normal(r, T, heads, hd)
+    pos = r.integers(0, 1 << 20, T).astype(np.int32)
+    pos[r.random(T) < 0.1] = -1
+    f, mag = tl.rotary_frequencies(rot, scaling="parts" if rot > 2 else "unscaled", factor=4.0, trained_len=2048, low=1, high=4)
+    live = pos >= 0
+    for inverse in (False, True):
+        want, tol = so.rotary(x[live], pos[live], f, mag, half, inverse)
+        got = tl.rotary(x, pos, f, mag, half, inverse, out=old)
+        close(got[live], want, tol)
+        assert np.array_equal(got[~live], old[~live])
+        got = tl.rotary(x, pos, f, mag, half, inverse, in_place=True)
+        close(got[live], want, tol, "in place")
+        assert np.array_equal(got[~live], x[~live])
+    assert tl.device_status() == 0
+
+
 @pytest.mark.parametrize("hd,rot", [(8, 8), (7, 6)])
 def test_rotary_of_the_most_tokens(tl, hd, rot):
     """2^31 - 1 tokens, all padding but the last; they share one row of in and out."""
@@ -178,6 +200,42 @@ def test_append_stores_at_the_row_and_position(tl, page, kv, hd, heads, rot, hal
     assert tl.device_status() == 0
 
 
+@pytest.mark.parametrize("T,page,kv,hd,heads,rot,half,by_head", [(3001, 16, 8, 128, 32, 128, False, False), (2500, 24, 3, 80, 15, 40, True, True),
+                                                                 (5000, 16, 1, 64, 1, 64, True, False), (2000, 64, 32, 128, 32, 128, True, False),
+                                                                 (4000, 5, 2, 7, 4, 6, False, False), (2222, 16, 2, 64, 0, 64, False, True),
+                                                                 (1700, 8, 4, 32, 64, 0, False, False), (1333, 16, 2, 36, 9, 20, True, False)])
+def test_append_of_a_prompt(tl, T, page, kv, hd, heads, rot, half, by_head):
+    """Thousands of tokens of three rows in any order: a CTA moves several, all three tensors of them."""
+    r = np.random.default_rng([T, page, kv, hd])
+    lens = [T // 2, T // 3, T - T // 2 - T // 3]
+    c, k, v, table, refs = filled_cache(tl, r, 2, page, kv, hd, lens, by_head, garbage=False)
+    rows = np.repeat(np.arange(3), lens).astype(np.int32)
+    pos = np.concatenate([np.arange(n) for n in lens]).astype(np.int32)
+    order = r.permutation(T)
+    rows, pos = rows[order], pos[order]
+    pos[r.random(T) < 0.05] = -1
+    live = pos >= 0
+    q = normal(r, T, heads, hd) if heads else None
+    nk, nv = normal(r, T, kv, hd), normal(r, T, kv, hd)
+    f = tl.rotary_frequencies(rot)[0] if rot else None
+    got_q = c.append(1, q, nk, nv, pos, f, 0.75, half, rows)
+    fr = np.zeros(0) if f is None else f
+    if heads:
+        wq, tq = so.rotary(q[live], pos[live], fr, 0.75, half)
+        close(got_q[live], wq, tq, "q")
+        assert (got_q[~live] == 0).all()
+    wk, tk = so.rotary(nk[live], pos[live], fr, 0.75, half)
+    gk, gv = c.pools()
+    at = table[rows[live], pos[live] // page], pos[live] % page
+    close(gk[1][at], wk, tk, "k")
+    assert np.array_equal(gv[1][at], nv[live])
+    seen = np.zeros(k.shape[1:3], bool)
+    seen[at] = True
+    for got, old in ((gk, k), (gv, v)):          # nothing else has changed
+        assert np.array_equal(got[0], old[0]) and np.array_equal(got[1][~seen], old[1][~seen])
+    assert tl.device_status() == 0
+
+
 def test_append_never_follows_bad_ids(tl):
     r = np.random.default_rng(9)
     page, kv, hd = 8, 2, 32
@@ -241,6 +299,17 @@ def test_attention_split_over_the_length(tl, B, low, high, kv, group, hd, page):
     c, k, v, table, _ = filled_cache(tl, r, 1, page, kv, hd, lens)
     q = normal(r, B, kv * group, hd, std=1.5)
     check_attention(tl, c, k[0], v[0], table, lens, page, q)
+    assert tl.device_status() == 0
+
+
+@pytest.mark.parametrize("B,low,high,kv,group,hd,page", [(11, 0, 1000, 2, 16, 128, 16), (1, 20011, 20011, 1, 9, 128, 16), (3, 1, 7000, 2, 12, 112, 24),
+                                                         (100, 0, 90, 1, 10, 128, 8), (5, 100, 3000, 2, 25, 128, 64)])
+def test_attention_of_wide_groups(tl, B, low, high, kv, group, hd, page):
+    """Nine and more query heads a KV head at 97..128 elements."""
+    r = np.random.default_rng([B, high, group])
+    lens = r.integers(low, high + 1, B).tolist()
+    c, k, v, table, _ = filled_cache(tl, r, 1, page, kv, hd, lens)
+    check_attention(tl, c, k[0], v[0], table, lens, page, normal(r, B, kv * group, hd, std=1.5))
     assert tl.device_status() == 0
 
 
@@ -433,6 +502,24 @@ def test_pages_over_many_steps(tl, seed, pages, page, rows, width, layers, kv, h
 
 def want_contents(step):
     return step % 5 == 4 or step > 36
+
+
+def test_fork_of_many_rows(tl):
+    """More rows than 32 bytes each fill shared memory with."""
+    r = np.random.default_rng(23)
+    rows, width, pages = 7001, 11, 300
+    c, pg = tl.PagedCache(1, pages, 2, 1, 8, rows, width), so.Pages(pages, 2, rows, width)
+    n = r.integers(0, width + 1, rows)
+    pg.table = np.where(np.arange(width) < n[:, None], r.integers(0, pages, (rows, width)), -1).astype(np.int32)
+    pg.lengths = (2 * n).astype(np.int32)
+    pg.refs = np.bincount(pg.table[pg.table >= 0], minlength=pages).astype(np.int32)
+    c.set_state(pg.table, pg.lengths, pg.refs)
+    for share in (0.9, 0.3, 1.0):
+        parents = np.where(r.random(rows) < share, r.integers(-1, rows, rows), np.arange(rows))
+        c.fork(parents)
+        pg.fork(parents)
+        same_books(c, pg)
+    assert tl.device_status() == 0
 
 
 def test_pages_refuse_without_changing_anything(tl):
@@ -638,6 +725,69 @@ def test_beam_selection_with_row_strides(tl, stride, off):
     tl.check(lib.tl_beam_select_f16(dx.ptr + 2 * off, stride, ds.ptr, None, 0, 2, 3, vocab, k, outs[0].ptr, outs[1].ptr, outs[2].ptr, w.ptr, w.nbytes, None), "select")
     want = so.beam_select(x, s, 3, k)
     assert np.array_equal(outs[1].to_numpy(np.int32, (2, k)), want[1]) and np.array_equal(outs[2].to_numpy(np.int32, (2, k)), want[2])
+
+
+def select_rows(tl, x, s, beams, k, stride, off):
+    """Selection from rows `stride` apart that start `off` values into a buffer of 60000s; checked against the values in 64 bits: each
+    beam's tokens are its first ones by (logit, lowest token), and what is left out is no better but for the rounding of the log-sums."""
+    rows, vocab = x.shape
+    batch = rows // beams
+    lib, need = tl.load(), C.c_size_t(0)
+    flat = np.full(off + rows * stride + 8, 60000, np.float16)
+    flat[off:off + rows * stride].reshape(rows, stride)[:, :vocab] = x
+    tl.check(lib.tl_beam_select_workspace(batch, beams, vocab, k, C.byref(need)), "ws")
+    w, dx, ds = (tl.DeviceBuffer.from_numpy(a) for a in (np.zeros(max(16, need.value), np.uint8), flat, np.asarray(s, np.float32)))
+    out = [tl.DeviceBuffer.from_numpy(np.full(batch * k, -7, np.int32)) for _ in range(3)]
+    tl.check(lib.tl_beam_select_f16(dx.ptr + 2 * off, stride, ds.ptr, None, 0, batch, beams, vocab, k, *(o.ptr for o in out), w.ptr, w.nbytes, None), "select")
+    values = so.beam_values(x, s).reshape(batch, beams * vocab)
+    parents, tokens = (o.to_numpy(np.int32, (batch, k)) for o in out[1:])
+    at = (parents - np.arange(batch)[:, None] * beams).astype(np.int64) * vocab + tokens
+    assert at.min() >= 0 and at.max() < beams * vocab and all(len(set(a)) == k for a in at)
+    logits = np.minimum(np.where(np.isnan(x), -np.inf, x.astype(np.float64)), 65504.0)
+    for b in range(batch):
+        for beam in range(beams):
+            chosen = tokens[b][parents[b] == b * beams + beam]
+            row = logits[b * beams + beam]
+            assert np.array_equal(chosen, np.argsort(-row, kind="stable")[:len(chosen)]), (b, beam)
+    got, want = np.take_along_axis(values, at, 1), -np.sort(-values, axis=1)[:, :k]
+    with np.errstate(invalid="ignore"):
+        assert ((got == want) | (np.abs(got - want) <= 2.0 ** -20)).all()
+    close(out[0].to_numpy(np.float32, (batch, k)), got, np.abs(got) * 2.0 ** -24 + 2.0 ** -21)
+
+
+@pytest.mark.parametrize("batch,beams,vocab,k,stride,off", [(1, 16, 20001, 64, 20001, 0), (1, 16, 20001, 64, 20004, 3), (1, 16, 40000, 64, 40000, 0),
+                                                            (2, 128, 25003, 8, 25003, 1), (300, 2, 20480, 16, 20480, 0), (600, 1, 9001, 1, 9001, 5),
+                                                            (1, 8, 16385, 128, 16392, 0), (40, 16, 8193, 33, 8200, 7)])
+def test_beam_selection_over_several_windows(tl, batch, beams, vocab, k, stride, off):
+    """Rows (chunks of them) of more than 8192 logits: random, rising, falling, all equal, masked but for a few, with NaN and infinities,
+    and large where the first window has seen nothing of it."""
+    r = np.random.default_rng([35, batch, beams, vocab, k])
+    rows = batch * beams
+    x = (r.standard_normal((rows, vocab)) * 3).astype(np.float16)
+    for i in range(rows):
+        kind = i % 9
+        if kind == 1:
+            x[i] = np.linspace(-9, 9, vocab)
+        elif kind == 2:
+            x[i] = np.linspace(9, -9, vocab)
+        elif kind == 3:
+            x[i] = 2.5
+        elif kind == 4:
+            keep = r.permutation(vocab)[:20]
+            kept = x[i, keep]
+            x[i] = -np.inf
+            x[i, keep] = kept
+        elif kind == 5:
+            x[i, r.random(vocab) < 0.3] = np.nan
+            x[i, r.integers(vocab)] = -np.inf
+        elif kind == 6:
+            x[i, r.random(vocab) < 0.01] = np.inf
+        elif kind == 7:
+            x[i, vocab // 2:] += np.float16(20)
+        elif kind == 8:
+            x[i] = r.choice([1.0, 1.5, -0.0, 0.0], vocab)
+    select_rows(tl, x, -r.random(rows).astype(np.float32), beams, k, stride, off)
+    assert tl.device_status() == 0
 
 
 def test_beam_selection_of_other_sizes_in_the_same_workspace(tl):
