@@ -143,7 +143,8 @@ int tl_paged_attn_decode_f16(const tl_paged_cache* cache, int layer, const tl_ha
     TL_REQUIRE(layer >= 0 && layer < cache->n_layers, "paged_attn_decode: layer %d out of range", layer);
     TL_REQUIRE(batch >= 0 && n_heads > 0 && n_heads % cache->n_kv_heads == 0, "paged_attn_decode: n_heads must be a multiple of the cache's");
     if (cache->head_dim > 256) return set_error(TL_ERR_UNSUPPORTED, "paged_attn_decode: head_dim above 256");
-    TL_REQUIRE(std::isfinite(scale), "paged_attn_decode: scale must be finite");
+    // scores are exponentiated to base 2
+    TL_REQUIRE(std::isfinite(scale * 1.4426950408889634f), "paged_attn_decode: scale times log2 e must be finite");
     TL_REQUIRE(batch <= 65535 && n_heads <= 65535, "paged_attn_decode: more than 65535 rows or heads");
     if (batch == 0) {
         TL_CHECK_INIT();

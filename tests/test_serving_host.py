@@ -174,6 +174,12 @@ def test_attention_refuses():
         refused(lib.tl_paged_attn_workspace(*bad, C.byref(need)))
 
 
+def test_attention_refuses_a_scale_that_overflows():
+    """Finite, but not times log2 e: a score of 0 would have become a NaN."""
+    for scale in (3e38, -2.4e38):
+        refused(tl.load().tl_paged_attn_decode_f16(cache(), 0, P, P, None, None, 2, 8, scale, 1024, 1024, P, 1 << 25, None))
+
+
 def test_beam_calls_refuse():
     lib = tl.load()
     ws = 1 << 25
