@@ -61,9 +61,10 @@ TL_API int tl_version(void);
 /* Select `device`, verify it is sm_100, make it current for the calling thread. */
 TL_API int tl_init(int device);
 TL_API int tl_device_count(int* count);
-/* Synchronise the device and fetch (then clear) the device status word: 0, or TL_ERR_TIMEOUT if a
- * kernel gave up on one of its bounded waits (mbarrier polls). The reference has no counterpart:
- * its kernels never wait on anything. */
+/* Synchronise the device and fetch (then clear) the device status: 0, or TL_ERR_TIMEOUT if a
+ * kernel gave up on one of its bounded waits (mbarrier polls), or TL_ERR_INVALID_ARGUMENT if one was
+ * given an id outside its table (the serving calls below); if both, the timeout, and the next call the
+ * other. The reference has no counterpart: its kernels never wait on anything. */
 TL_API int tl_device_status(int* status);
 
 /* Host-only introspection of the lookup tables the kernels use for exp / SiLU / RoPE. They are

@@ -232,7 +232,7 @@ class DeviceBuffer:
 
 
 def device_status() -> int:
-    """0, or the status a kernel recorded when one of its bounded waits ran out (synchronises)."""
+    """0, or the status a kernel recorded when one of its bounded waits ran out or an id was outside its table (synchronises)."""
     v = _int(0)
     check(load().tl_device_status(C.byref(v)), "tl_device_status")
     return v.value

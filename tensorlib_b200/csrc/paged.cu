@@ -508,7 +508,7 @@ __global__ void __launch_bounds__(COPY_THREADS, 4) k_gather_rows(const __half* s
 }
 
 CopyArgs copy_args(const PagedView& c) {
-    CopyArgs a{c.k, c.v, c.layer_stride, c.page_stride, c.n_layers, c.n_pages, COPY_THREADS, page_shape(c), FastDiv(2u * c.n_layers), device_status_word()};
+    CopyArgs a{c.k, c.v, c.layer_stride, c.page_stride, c.n_layers, c.n_pages, COPY_THREADS, page_shape(c), FastDiv(2u * c.n_layers), device_id_status_word()};
     if ((long long)c.page_size * c.n_kv_heads * c.head_dim / a.shape.vec <= 2 * COPY_THREADS) a.team = 32;
     return a;
 }
@@ -530,7 +530,7 @@ static int launch_fork(const PagedView& c, const int* parents, cudaStream_t st) 
     static PerDeviceOnce once;
     TL_CUDA(once.run([&] { return cudaFuncSetAttribute(k_fork<SLAB>, cudaFuncAttributeMaxDynamicSharedMemorySize, FORK_SMEM); }));
     return launch_pdl(k_fork<SLAB>, (unsigned)((c.max_pages + SLAB - 1) / SLAB + 1), FORK_THREADS, (size_t)c.n_rows * SLAB * 4, st, true, c.table,
-                      c.lengths, c.refs, parents, c.n_rows, c.max_pages, c.n_pages, device_status_word());
+                      c.lengths, c.refs, parents, c.n_rows, c.max_pages, c.n_pages, device_id_status_word());
 }
 int launch_paged_fork(const PagedView& c, const int* parents, cudaStream_t st) {
     // 32 bytes of a row at a time; less where many rows fill shared memory
@@ -550,7 +550,7 @@ int launch_paged_reserve(const PagedView& c, const int* new_tokens, int* result,
     wk.copies = reinterpret_cast<CowItem*>(w + 64);
     wk.need = reinterpret_cast<int*>(w + 64 + sizeof(CowItem) * (size_t)c.n_rows);
     wk.freed = wk.need + c.n_rows;
-    TL_PROPAGATE(launch_pdl(k_reserve, 1, RES_THREADS, 0, st, true, c, new_tokens, result, wk, device_status_word()));
+    TL_PROPAGATE(launch_pdl(k_reserve, 1, RES_THREADS, 0, st, true, c, new_tokens, result, wk, device_id_status_word()));
     const CopyArgs a = copy_args(c);
     return TL_LAUNCH_COPY(k_copy_shared, page_grid(a, c.n_rows), COPY_THREADS, 0, st, true, a, wk);
 }
@@ -586,9 +586,9 @@ int launch_gather_rows(const __half* src, __half* dst, const int* parents, int o
     const int pieces = (int)(vecs <= GATHER_VECS ? 1 : (vecs + GATHER_VECS - 1) / GATHER_VECS);
     const unsigned grid = copy_grid((long long)outer * rows * pieces);
     return vec ? launch_pdl(k_gather_rows<uint4>, grid, COPY_THREADS, 0, st, true, src, dst, parents, outer, rows, used, so, sr, dso, dsr,
-                            pieces, device_status_word())
+                            pieces, device_id_status_word())
                : launch_pdl(k_gather_rows<__half>, grid, COPY_THREADS, 0, st, true, src, dst, parents, outer, rows, used, so, sr, dso, dsr,
-                            pieces, device_status_word());
+                            pieces, device_id_status_word());
 }
 
 }  // namespace tlb

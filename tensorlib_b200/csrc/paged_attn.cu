@@ -639,7 +639,7 @@ int launch_paged_attn(const PagedView& c, const PagedAttnArgs& a, cudaStream_t s
     p.head_dim = c.head_dim; p.by_page = c.by_page;
     p.q = a.q; p.out = a.out; p.lse = a.lse; p.q_row = a.q_row; p.o_row = a.o_row;
     p.batch = a.batch; p.n_heads = a.n_heads; p.group = a.n_heads / c.n_kv_heads; p.scale = a.scale;
-    p.status = device_status_word();
+    p.status = device_id_status_word();
     const bool fast = c.aligned16() && (reinterpret_cast<uintptr_t>(a.q) & 3) == 0 && a.q_row % 2 == 0;
     if (!fast) return launch_pdl(k_paged_attn_any, dim3(a.n_heads, a.batch), ANY_WARPS * 32, 0, st, true, p);
     // the cost of the whole batch has to fit 31 bits

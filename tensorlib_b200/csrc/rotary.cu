@@ -264,7 +264,7 @@ int launch_rotary(const RotaryArgs& a, const PagedView* cache, cudaStream_t st) 
     if (a.tokens == 0) return TL_OK;
     RotLaunch p{};
     p.a = a;
-    p.status = device_status_word();
+    p.status = device_id_status_word();
     if (a.n_heads > 0)
         p.plane[p.planes++] = RotPlane{a.q, a.q_out, a.q_token, a.q_head, a.qo_token, a.qo_head, a.n_heads, true, false};
     if (cache) {

@@ -16,7 +16,7 @@ bool g_init = false;
 int g_device = -1;
 int g_sms = 0;
 Tables g_tables{};
-int* g_status = nullptr;
+int* g_status = nullptr;             // two words: bounded waits, ids
 std::mutex g_mu;
 
 struct RopeTable {
@@ -44,8 +44,9 @@ int init_device() { return g_device; }
 int sm_count() { return g_sms; }
 const Tables& tables() { return g_tables; }
 int* device_status_word() { return g_status; }
+int* device_id_status_word() { return g_status + 1; }
 
-// `value` is a copy of the status word fetched at a synchronisation point. Non-zero: clear the
+// `value` is a copy of the waits' status word fetched at a synchronisation point. Non-zero: clear the
 // word on the device and report the failure to the caller instead of returning results computed
 // from partial or stale data.
 int consume_device_status(int value) {
@@ -195,20 +196,23 @@ int tl_init(int device) {
     g_device = device;
     g_sms = prop.multiProcessorCount;
     TL_PROPAGATE(build_tables());
-    TL_CUDA(cudaMalloc(&g_status, sizeof(int)));
-    TL_CUDA(cudaMemset(g_status, 0, sizeof(int)));
+    TL_CUDA(cudaMalloc(&g_status, 2 * sizeof(int)));
+    TL_CUDA(cudaMemset(g_status, 0, 2 * sizeof(int)));
     g_init = true;
     return TL_OK;
 }
 
 // Synchronises the device, then reports (and clears) the status word kernels set when a bounded
-// device-side wait gave up.
+// device-side wait gave up, or else the one they set when an id was outside its table.
 int tl_device_status(int* status) {
     TL_CHECK_INIT();
     TL_REQUIRE(status != nullptr, "status is null");
     TL_CUDA(cudaDeviceSynchronize());
-    TL_CUDA(cudaMemcpy(status, g_status, sizeof(int), cudaMemcpyDeviceToHost));
-    if (*status != 0) TL_CUDA(cudaMemset(g_status, 0, sizeof(int)));
+    int words[2];
+    TL_CUDA(cudaMemcpy(words, g_status, sizeof words, cudaMemcpyDeviceToHost));
+    const int which = words[0] == 0;
+    *status = words[which];
+    if (*status != 0) TL_CUDA(cudaMemset(g_status + which, 0, sizeof(int)));
     return TL_OK;
 }
 

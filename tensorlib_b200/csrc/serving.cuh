@@ -7,7 +7,9 @@
 
 namespace tlb {
 
-int* device_status_word();
+// What kernels here set to TL_ERR_INVALID_ARGUMENT for an id outside its table. It is not the word of the bounded waits: that one says
+// that the results of the call which finds it are not valid, and its value is not to be lost.
+int* device_id_status_word();
 int init_device();
 
 // Calls may come from a thread whose current device is another one: the pointers belong to the device of tl_init.

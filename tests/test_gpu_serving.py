@@ -855,6 +855,25 @@ def test_beam_reorder(tl, outer, rows, pitch, used):
         assert np.array_equal(got, want) and tl.device_status() == 1
 
 
+# ---- bad ids and the rest of the library ---------------------------------------------------------------------------
+def test_bad_ids_are_no_concern_of_a_model(tl):
+    """An id outside its table is reported by tl_device_status, not by the next call of a model, and hides no timeout."""
+    from tensorlib_b200 import synth
+    lib = tl.load()
+    m = tl.Llama2(synth.TINY, numerics=tl.FAST)
+    m.init_random(7)
+    want = m.generate([3, 5, 7], 8)[0]
+    c = tl.PagedCache(1, 6, 4, 1, 8, 2, 3)
+    c.fork([0, 9])
+    assert np.array_equal(m.generate([3, 5, 7], 8)[0], want)
+    assert tl.device_status() == 1 and tl.device_status() == 0
+    tl.check(lib.tl_selftest_unposted_exchange(256, None), "tl_selftest_unposted_exchange")
+    c.fork([0, 9])
+    tl.synchronize()
+    assert tl.device_status() == 6 and tl.device_status() == 1 and tl.device_status() == 0
+    m.close()
+
+
 # ---- together ------------------------------------------------------------------------------------------------------
 def test_a_beam_search_over_pages_matches_one_over_copied_sequences(tl):
     """Select, fork, reserve, append and attend for 3 entries of 4 beams over 2 layers and 30 steps, against beams that carry
