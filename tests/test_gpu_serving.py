@@ -855,6 +855,52 @@ def test_beam_reorder(tl, outer, rows, pitch, used):
         assert np.array_equal(got, want) and tl.device_status() == 1
 
 
+# ---- nothing to do, threads ----------------------------------------------------------------------------------------
+def test_calls_with_nothing_to_do(tl):
+    h = lambda *n: np.zeros(n, np.float16)  # noqa: E731
+    f = tl.rotary_frequencies(16)[0]
+    c = tl.PagedCache(1, 4, 8, 2, 16, 3, 2)
+    assert tl.rotary(h(0, 2, 16), [], f).shape == (0, 2, 16)
+    assert c.append(0, h(0, 4, 16), h(0, 2, 16), h(0, 2, 16), [], f).shape == (0, 4, 16)
+    out, lse = c.attend(0, h(0, 4, 16))
+    assert out.shape == (0, 4, 16) and lse.shape == (0, 4)
+    c.copy([], [])
+    assert c.reserve([0, 0, 0]) == 0
+    moved, live = c.compact()
+    assert (moved == -1).all() and live == 0
+    assert all(a.shape == (0, 3) for a in tl.beam_select(h(0, 9), [], 2, 3))
+    dst = normal(np.random.default_rng(1), 2, 3, 8)
+    assert np.array_equal(tl.beam_reorder(h(2, 3, 8), dst, [0, 0, 0], 0), dst) and tl.beam_reorder(h(0, 3, 8), h(0, 3, 8), [0, 0, 0], 8).shape == (0, 3, 8)
+    table, lengths, refs = c.state()
+    assert (table == -1).all() and (lengths == 0).all() and (refs == 0).all() and tl.device_status() == 0
+
+
+def test_host_threads_with_workspaces_of_their_own(tl):
+    """Four threads at once, each with its own cache and arrays: every result as from one alone."""
+    from concurrent.futures import ThreadPoolExecutor
+
+    def work(i):
+        r = np.random.default_rng([61, i])
+        hd, lens = (64, 96, 192, 256)[i], [300, 0, 17, 1200]
+        c, k, v, table, _ = filled_cache(tl, r, 1, 16, 2, hd, lens)
+        x, s = normal(r, 8, 5000 + i, std=3), -r.random(8).astype(np.float32)
+        q = normal(r, 4, 6, hd, std=1.5)
+        want = so.beam_select(x, s, 4, 8)
+        for _ in range(10):
+            check_attention(tl, c, k[0], v[0], table, lens, 16, q)
+            got = tl.beam_select(x, s, 4, 8)
+            assert want[3] < 1e-6 or (np.array_equal(got[1], want[1]) and np.array_equal(got[2], want[2]))
+            assert c.reserve([1, 0, 0, 0]) in (0, 5)
+            lens[0] = int(c.state()[1][0])
+            lens[0] -= 1
+            c.set_state(*(a if j != 1 else lens for j, a in enumerate(c.state())))
+        return True
+
+    with ThreadPoolExecutor(4) as pool:
+        assert all(pool.map(work, range(4)))
+    assert tl.device_status() == 0
+
+
 # ---- bad ids and the rest of the library ---------------------------------------------------------------------------
 def test_bad_ids_are_no_concern_of_a_model(tl):
     """An id outside its table is reported by tl_device_status, not by the next call of a model, and hides no timeout."""
