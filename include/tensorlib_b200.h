@@ -290,8 +290,8 @@ TL_API int tl_rmsnorm_gateup_swiglu_f16(const tl_half* x, const tl_half* norm_w,
  *   TL_ROPE_BASE    base * factor^(rot_dim / (rot_dim - 2))
  *   TL_ROPE_PARTS   with x = the pair's turns over trained_len: / factor where x <= low, kept where x >= high, and between
  *                   them both blended linearly in x
- *   TL_ROPE_RAMP    the same blend, linear in the pair's index between those that turn `high` and `low` times, and a
- *                   magnitude of 0.1 ln(factor) + 1
+ *   TL_ROPE_RAMP    the same blend, linear in the pair's index between those that turn `high` and `low` times (rounded outwards,
+ *                   kept within 0 and rot_dim - 1), and a magnitude of 0.1 ln(factor) + 1
  * factor, trained_len, low and high are ignored where the scaling does not use them. No device needed. */
 enum { TL_ROPE_UNSCALED = 0, TL_ROPE_LINEAR = 1, TL_ROPE_BASE = 2, TL_ROPE_PARTS = 3, TL_ROPE_RAMP = 4 };
 TL_API int tl_rotary_frequencies(int rot_dim, double base, int scaling, double factor, double trained_len, double low,

@@ -52,11 +52,13 @@ int tl_rotary_frequencies(int rot_dim, double base, int scaling, double factor, 
     if (scaling == TL_ROPE_BASE && rot_dim > 2) b = base * std::pow(factor, (double)rot_dim / (rot_dim - 2));
     *magnitude_host = 1.0f;
     double lo = 0, hi = 0;
+    bool all = false;                             // not even the first pair turns more than `low` times
     if (scaling == TL_ROPE_RAMP) {
         // pair index at which a pair turns x times over the trained length
         auto index_of = [&](double turns) { return rot_dim * std::log(trained_len / (turns * two_pi)) / (2 * std::log(base)); };
         lo = std::fmax(std::floor(index_of(high)), 0.0);
         hi = std::fmin(std::ceil(index_of(low)), rot_dim - 1.0);
+        all = index_of(low) <= 0;
         *magnitude_host = (float)(0.1 * std::log(factor) + 1.0);
     }
     for (int i = 0; i < n; i++) {
@@ -67,7 +69,7 @@ int tl_rotary_frequencies(int rot_dim, double base, int scaling, double factor, 
             f = (1 - s) * f / factor + s * f;
         }
         if (scaling == TL_ROPE_RAMP) {
-            const double s = std::fmin(1.0, std::fmax(0.0, (i - lo) / std::fmax(hi - lo, 0.001)));
+            const double s = all ? 1.0 : std::fmin(1.0, std::fmax(0.0, (i - lo) / std::fmax(hi - lo, 0.001)));
             f = (1 - s) * f + s * f / factor;
         }
         freqs_host[i] = f;

@@ -35,6 +35,16 @@ def test_frequencies_follow_their_formulas():
         assert np.allclose(g, (1 - w) * f + w * f / 8, rtol=1e-12, atol=0)
 
 
+def test_ramp_where_no_pair_turns_as_often_as_low():
+    """trained_len below 2 pi low: every pair, the first among them, is on the scaled side."""
+    for rot, trained, low in ((64, 6.0, 1.0), (64, 3.0, 1.0), (2, 1.0, 1.0), (128, 2 * math.pi * 4, 4.0 * (1 + 1e-9)), (8, 0.01, 2.0)):
+        f = tl.rotary_frequencies(rot)[0]
+        g = tl.rotary_frequencies(rot, scaling="ramp", factor=8.0, trained_len=trained, low=low, high=32)[0]
+        assert np.allclose(g, f / 8, rtol=1e-13, atol=0), (rot, trained, low, g / f)
+    # and as soon as the first one does, it is kept
+    assert tl.rotary_frequencies(64, scaling="ramp", factor=8.0, trained_len=7.0, low=1.0, high=32)[0][0] == 1.0
+
+
 def test_frequencies_refuse():
     for kw in (dict(rot_dim=0), dict(rot_dim=3), dict(rot_dim=8, base=1.0), dict(rot_dim=8, base=math.nan),
                dict(rot_dim=8, scaling="linear", factor=0.5), dict(rot_dim=8, scaling="parts", factor=2.0),
