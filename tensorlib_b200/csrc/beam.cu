@@ -161,46 +161,67 @@ __device__ __forceinline__ bool dead_row(const BeamArgs& a, int row) {
     return !(s > -INFINITY);
 }
 
-// The k best of one row by (value, lowest token), into its lists' places in the join: k passes over the row by the whole CTA. For rows
-// whose score is so large that distinct logits may have the same value in 64 bits, so that the k largest logits need not be the k
-// first candidates. Logits differ by 2^-24 at least, and values below 2^28 are rounded by 2^-26 at most: up to SEL_ROOM distinct
-// logits have distinct values.
+// A row's lists hold its largest logits, and so its largest values, but where distinct logits have the same value in 64 bits not the
+// first tokens of the least value that is taken. For rows whose score makes that possible: logits differ by 2^-24 at least, and values
+// below 2^28 are rounded by 2^-26 at most, so up to SEL_ROOM distinct logits have distinct values. The n-th largest value
+// in the lists is the row's n-th largest; what lies above it stays, and the entries that equal it become the lowest tokens that do,
+// found by the whole CTA in one pass that ends when there are enough.
 constexpr double SEL_ROOM = 134217728.0;          // 2^27
-__device__ __noinline__ void rank_row_by_value(const __half* x, unsigned vocab, unsigned at0, int n, double score, double lse,
-                                               unsigned long long* val, unsigned* idx, int places) {
-    __shared__ unsigned long long red_o[SEL_THREADS / 32];
-    __shared__ unsigned red_j[SEL_THREADS / 32];
+__device__ __noinline__ void settle_ties(const __half* x, unsigned vocab, unsigned at0, int n, double score, double lse, unsigned long long* val,
+                                         unsigned* idx, int places) {
+    constexpr int EACH = 8;                       // tokens of a thread at a time
+    __shared__ unsigned first[128];               // the lowest tokens of that value
+    __shared__ int found_sh[SEL_THREADS / 32], above_sh;
+    __shared__ unsigned long long least_sh;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    unsigned long long last = ~0ull;
-    unsigned last_j = 0;
-    for (int i = 0; i < n; i++) {
-        unsigned long long best = 0;
-        unsigned best_j = ~0u;
-        for (unsigned j = tid; j < vocab; j += SEL_THREADS) {
-            const unsigned long long o = ord64(score + ((double)beam_logit(x[j]) - lse));
-            if ((o < last || (o == last && j > last_j)) && o > best) { best = o; best_j = j; }       // (j ascends, no o is 0)
+    __syncthreads();
+    for (int i = tid; i < places; i += SEL_THREADS) {
+        if (idx[i] == ~0u) continue;
+        int above = 0, equal = 0;
+        for (int j = 0; j < places; j++) {        // (places that no candidate fills are 0, below every value)
+            above += val[j] > val[i];
+            equal += val[j] == val[i];
         }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            const unsigned long long y = __shfl_xor_sync(0xffffffffu, best, o);
-            const unsigned j = __shfl_xor_sync(0xffffffffu, best_j, o);
-            if (y > best || (y == best && j < best_j)) { best = y; best_j = j; }
-        }
-        __syncthreads();
-        if (lane == 0) { red_o[warp] = best; red_j[warp] = best_j; }
-        __syncthreads();
-        for (int v = 0; v < SEL_THREADS / 32; v++)
-            if (red_o[v] > best || (red_o[v] == best && red_j[v] < best_j)) { best = red_o[v]; best_j = red_j[v]; }
-        last = best;
-        last_j = best_j;
-        if (tid == 0) {
-            val[i] = best;
-            idx[i] = at0 + best_j;
-        }
+        if (above < n && above + equal >= n) { least_sh = val[i]; above_sh = above; }        // the same from all that write
     }
-    for (int i = n + tid; i < places; i += SEL_THREADS) {
-        val[i] = 0;
-        idx[i] = ~0u;
+    __syncthreads();
+    const unsigned long long least = least_sh;
+    const int need = n - above_sh;
+    int got = 0;
+    for (unsigned j0 = 0; j0 < vocab && got < need; j0 += SEL_THREADS * EACH) {
+        unsigned hits = 0;
+#pragma unroll
+        for (int e = 0; e < EACH; e++) {
+            const unsigned j = j0 + tid * EACH + e;
+            if (j < vocab && ord64(score + ((double)beam_logit(x[j]) - lse)) == least) hits |= 1u << e;
+        }
+        int upto = __popc(hits);
+        const int mine = upto;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += y;
+        }
+        __syncthreads();
+        if (lane == 31) found_sh[warp] = upto;
+        __syncthreads();
+        int at = got + upto - mine;
+        for (int w = 0; w < SEL_THREADS / 32; w++) {
+            if (w < warp) at += found_sh[w];
+            got += found_sh[w];
+        }
+        for (int e = 0; e < EACH; e++)
+            if (hits >> e & 1u) {
+                if (at < need) first[at] = j0 + tid * EACH + e;
+                at++;
+            }
+    }
+    __syncthreads();
+    for (int i = tid; i < places; i += SEL_THREADS) {
+        if (val[i] != least || idx[i] == ~0u) continue;
+        int before = 0;
+        for (int j = 0; j < i; j++) before += val[j] == least;
+        idx[i] = before < min(need, got) ? at0 + first[before] : ~0u;  // (~0: a place that no candidate fills)
     }
     __syncthreads();
 }
@@ -557,15 +578,17 @@ __global__ void __launch_bounds__(SEL_THREADS, 4) k_beam_select(SelLaunch p) {
     bv = border_val;
     bi = border_idx;
     if (large_sh)
-        for (int w = 0; w < a.beams; w++) {       // (the lists' candidates bound the result from below, whatever their order)
+        for (int w = 0; w < a.beams; w++) {
             const int r = entry * a.beams + w, l0 = w * p.splits;
             const double score = beam_score(a.scores[r]);
             if (fabs(score) < SEL_ROOM || dead_row(a, r) || (a.finished && a.finished[r])) continue;
             unsigned long long most = 0;          // a list begins with its largest value
             for (int s = 0; s < p.splits; s++) most = max(most, val[(l0 + s) * a.k]);
-            if (most >= bv)
-                rank_row_by_value(a.logits + r * a.pitch, (unsigned)a.vocab, (unsigned)w * (unsigned)a.vocab, min(a.k, a.vocab), score, lse[w],
-                                  val + l0 * a.k, idx + l0 * a.k, p.splits * a.k);
+            int above = 0;
+            for (int i0 = 0; i0 < total && above < a.k; i0 += SEL_THREADS) above += __syncthreads_count(i0 + tid < total && val[i0 + tid] > most);
+            if (above < a.k)                      // else (a beam marked by -1e9, say) none of it is taken
+                settle_ties(a.logits + r * a.pitch, (unsigned)a.vocab, (unsigned)w * (unsigned)a.vocab, min(a.k, a.vocab), score, lse[w],
+                            val + l0 * a.k, idx + l0 * a.k, p.splits * a.k);
         }
     for (int i = tid; i < total; i += SEL_THREADS) {
         const unsigned long long o = val[i];

@@ -691,6 +691,27 @@ def test_beam_selection_where_scores_leave_no_room_for_logits(tl, batch, beams, 
     assert np.array_equal(got[1], want[1]) and np.array_equal(got[2], want[2]) and np.array_equal(got[0], want[0].astype(np.float32))
 
 
+@pytest.mark.parametrize("batch,beams,vocab,k", [(3, 8, 32000, 16), (1, 4, 700, 100), (2, 16, 20001, 64), (1, 3, 50, 120)])
+def test_beam_selection_with_beams_marked_by_a_large_score(tl, batch, beams, vocab, k):
+    """One live beam an entry and the others at -1e9 or lower, as for a search's first step: the live one's candidates come first, and
+    where there are too few of them (masked ones count as -inf) the marked beams' follow, in order."""
+    r = np.random.default_rng([36, beams, vocab, k])
+    rows = batch * beams
+    for mark in (-1e9, -1e20, -3e38):
+        x = (r.standard_normal((rows, vocab)) * 3).astype(np.float16)
+        live = np.arange(batch) * beams + r.integers(0, beams, batch)
+        s = np.full(rows, mark, np.float32)
+        s[live] = -r.random(batch)
+        for some in (vocab, k // 2):                     # the live beam's tokens that are not masked
+            for row in live:
+                x[row, r.permutation(vocab)[some:]] = -np.inf
+            want = so.beam_select(x, s, beams, k)
+            got = tl.beam_select(x, s, beams, k)
+            sure = want[0] > mark / 2 if mark == -1e9 else np.ones(want[0].shape, bool)      # at -1e9 the log-sums' rounding decides
+            assert np.array_equal(got[1][sure], want[1][sure]) and np.array_equal(got[2][sure], want[2][sure]), (mark, some)
+            close(got[0], want[0], np.abs(want[0]) * 2.0 ** -24 + 2.0 ** -21)
+
+
 @pytest.mark.parametrize("batch,beams,vocab", [(5, 4, 3001), (3, 128, 200)])
 def test_beam_selection_writes_the_scores_in_place(tl, batch, beams, vocab):
     """Both kernels: the second shape has more candidates than one CTA joins."""
