@@ -280,8 +280,10 @@ TL_API int tl_rmsnorm_gateup_swiglu_f16(const tl_half* x, const tl_half* norm_w,
  * The reference keeps one contiguous cache per layer for one sequence (Transformer.cpp:22-23), rotates interleaved pairs by
  * consecutive positions (CPU.cpp:427-461) and samples greedily (llama2.cpp:55-61); these operators are what a server of many
  * sequences or beams needs beside that. They only enqueue on `stream`, allocate nothing and can be captured into a graph.
- * A workspace belongs to the caller: calls that share one must be ordered behind one another, and so must graphs that
- * captured it. Ids that the kernels find outside their tables (rows, pages, parents, lengths) are never followed: the
+ * A workspace belongs to the caller and serves one operator (reserve and compact may share theirs): attention and selection count
+ * on finding their counters as their last call left them, at different places, and the other two write there; in a workspace that
+ * another operator has used since it was zeroed their results are wrong or missing. Calls that share a workspace must be ordered
+ * behind one another, and so must graphs that captured it. Ids that the kernels find outside their tables (rows, pages, parents, lengths) are never followed: the
  * entry is skipped and tl_device_status() reports TL_ERR_INVALID_ARGUMENT. */
 
 /* Rotation frequencies, on the host: freqs_host[rot_dim / 2] in radians a position, pair i has base^(-2 i / rot_dim), and the
@@ -310,7 +312,7 @@ TL_API int tl_rotary_f16(const tl_half* in, tl_half* out, const int* positions, 
  * by head. Row r (one sequence or beam) holds lengths[r] tokens; token t lies in page page_table[r * max_pages + t / page_size],
  * slot t % page_size. Entries behind a row's last page are -1 (fill a new table with tl_memset 0xff), ref_counts[p] is the number
  * of table entries that name page p, and a page with count 0 is free. Rows may share pages. The pointers a call does not use
- * may be NULL. Rows of head_dim values that all start on 16 bytes take the fast kernels; any other layout works too. */
+ * may be NULL, but not page_table. Rows of head_dim values that all start on 16 bytes take the fast kernels; any other layout works too. */
 typedef struct tl_paged_cache {
     tl_half* k_pages; tl_half* v_pages;
     long long layer_stride, page_stride, token_stride, head_stride;
@@ -353,8 +355,9 @@ TL_API int tl_rotary_append_f16(const tl_paged_cache* cache, int layer, const tl
                                 long long q_out_token_stride, long long kv_token_stride, tl_stream stream);
 /* Attention of one query per batch entry over all lengths[row] tokens of its row: out_h = sum_t softmax_t(scale q_h.k_t) v_t, query
  * head h reading KV head h / (n_heads / n_kv_heads). q, out: [batch] rows of n_heads * head_dim values, row strides in elements.
- * rows[b]: the row of entry b, -1 for a padding entry (rows == NULL: row b). lse, if not NULL: fp32 [batch, n_heads],
- * log sum_t exp(scale q_h.k_t). An empty row gives zeros and -inf. head_dim <= 256, and batch * n_heads * (max_pages * page_size / 64 + 3)
+ * rows[b]: the row of entry b, -1 for a padding entry, which counts as an empty row (rows == NULL: row b). lse, if not NULL: fp32 [batch, n_heads],
+ * log sum_t exp(scale q_h.k_t). An empty row gives zeros and -inf. An infinity among the
+ * values read gives an infinity or a NaN in its element. head_dim <= 256, and batch * n_heads * (max_pages * page_size / 64 + 3)
  * has to stay below 2^31 (TL_ERR_UNSUPPORTED). workspace: tl_paged_attn_workspace bytes (at
  * most 32 MB), zeroed once before its first use; calls leave it as the next one needs it, whatever that one's sizes. */
 TL_API int tl_paged_attn_decode_f16(const tl_paged_cache* cache, int layer, const tl_half* q, tl_half* out, float* lse, const int* rows,

@@ -15,8 +15,8 @@ __device__ __forceinline__ float beam_logit(__half h) {
 }
 __device__ __forceinline__ double beam_score(float s) { return s != s ? -INFINITY : (double)fminf(s, 3.402823466e38f); }
 
-// Plain form for what one CTA cannot join or 32 chunks cannot hold (many beams times many results, vocabularies beyond 2 million;
-// four beams of 32000, which the kernel below takes 8 us for: 865 us): one CTA a batch entry; lse of its rows, then k rounds of an arg-maximum over what comes after
+// Plain form for what one CTA cannot join or 32 chunks cannot hold (many beams times many results, vocabularies beyond 2 million):
+// right, and two orders of magnitude slower (four beams of 32000, which the kernel below takes 8 us for: 865 us): one CTA a batch entry; lse of its rows, then k rounds of an arg-maximum over what comes after
 // the last one chosen.
 __global__ void __launch_bounds__(BEAM_THREADS) k_beam_any(BeamArgs a) {
     extern __shared__ double lse[];               // [beams], and the scores [beams]: out_scores may be their place
@@ -97,9 +97,10 @@ __global__ void __launch_bounds__(BEAM_THREADS) k_beam_any(BeamArgs a) {
 // between and cut back to the k best. The last CTA of a batch entry joins: the rows' log-sums, the candidates' values in 64
 // bits, and a border and ranks over the sorted lists.
 //
-// Bound: with many rows instructions, some 19 for a warp's 32 logits, before HBM (each logit is read once); with few rows the chain
-// load -> border -> list -> arrival -> log-sum -> ranks. Measured on a B200: 512 rows of 32000 logits, 16 of eight beams each,
-// 21 us (floor 4.7; 3.6 of them the join), four rows 8.3 us. Rows in several chunks took 30 us, for the part of a chunk that does
+// Bound: with few rows the chain load -> border -> list -> arrival -> log-sum -> ranks; with many no unit (half the issue slots, a third
+// of the exponentials' pipe) but what a row costs beyond its stream. Measured on a B200: 512 rows of 32000 logits, 16 of eight beams
+// each, 21 us (floor 4.7), of which the last window is done at 10, its list is ranked and the CTA arrives at 13.4, and the join takes
+// 4; 19 warp instructions for 32 logits, of which the stream is 6 by the source. Four rows 8.5 us. Rows in several chunks took 30 us, for the part of a chunk that does
 // not shrink with it.
 constexpr int SEL_THREADS = 256;
 constexpr int SEL_ASIDE = 256;                    // vectors set aside that wait for the end; more are taken apart

@@ -3,8 +3,9 @@
 // of contiguous state by parent. A page is free when its reference count is 0; there is no other free list, so every choice
 // of a page (the lowest free ones, ascending) follows from the counts alone and repeats from run to run.
 //
-// Bookkeeping is integer work on small arrays, bound by latency (freeing, forking and reserving 128 rows of some 130 pages with
-// copies of 62 MB: 21 us on a B200, about half of it the copies); the copies are bound by HBM, each byte read and written once
+// Bookkeeping is integer work on small arrays, bound by latency (freeing, forking and reserving 128 rows of some 130 pages, a token
+// each, with copies of 62 MB: 22 us on a B200, about half of it the copies; a row's new pages are handed out by one thread, one after
+// the other, which a prompt of thousands of pages waits for); the copies are bound by HBM, each byte read and written once
 // (504 pages of 32 KB in 64 pools 337 us, rows of 1.4 MB 191 us: 6.3 and 6.6 TB/s).
 #include "serving.cuh"
 

@@ -29,7 +29,7 @@ struct OnLibraryDevice {
     }
 };
 
-// n / d for n < 2^31 by one multiplication: m = ceil(2^32 * 2^s / d) with 2^s >= d, so the error term n * (m d - 2^(32+s))
+// n / d for n < 2^31 by one multiplication (Granlund and Montgomery, Division by Invariant Integers using Multiplication): m = ceil(2^32 * 2^s / d) with 2^s >= d, so the error term n * (m d - 2^(32+s))
 // stays below 2^(32+s) (round-up method); d = 1 .. 2^31 - 1. The top bit of m is implied, hence the extra addition.
 struct FastDiv {
     unsigned int m, s, d;
